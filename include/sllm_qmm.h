@@ -370,6 +370,131 @@ sllm_status sllm_attention_noalloc_dev(sllm_kv_cache *kv, int layer, const sllm_
                                        const float *q_dev, const float *k_dev, const float *v_dev, int seq_len,
                                        int start_pos, float *out_dev, void *stream);
 
+/* --------------------------------------------------------------------------
+ * Batches of sequences: a cache of pages that sequences share, the attention
+ * section of a batch over it, and adapters beside a shared projection. No
+ * counterparts in the reference, whose generations each keep a cache of their
+ * own (KVCacheF32, float32_ops.go:11-14, one per clone of the model).
+ * ------------------------------------------------------------------------ */
+
+typedef enum {
+    SLLM_CACHE_F32 = 0, /* K and V rows as computed */
+    SLLM_CACHE_F16 = 1  /* rounded to f16 (to nearest even; beyond its range: infinity) when appended */
+} sllm_cache_type;
+
+/*
+ * K and V of n_layers layers in n_pages pages of page_rows positions (16, 32,
+ * 64, 128 or 256) and n_kv_heads heads of d_k (a multiple of 8, at most 256)
+ * elements: two device pools, [layer][page][kv head][row of the page][d_k]
+ * (sllm_page_cache_data gives their addresses), zeroed. A sequence is a list
+ * of pages and a length in rows, the same for every layer. Sequences may hold
+ * a page together; a page with several holders is copied (in every layer, its
+ * filled rows) when one of them is to append rows to it. Pages are taken lowest
+ * number first, sequence numbers too, so tables follow from the order of calls.
+ * The bookkeeping is the host's and immediate; what it asks of the device (the
+ * copies) is enqueued on the given stream. Work on one cache, its attention
+ * calls included, has to be ordered on the device: one stream, or streams
+ * ordered by the caller's events. Calls may come from several threads. None may
+ * be made on a stream under capture, except sllm_page_attention_dev and those
+ * without a stream argument. Calls need the cache's device as the current one
+ * (else SLLM_ERR_ARG). A cache that is destroyed lives on until its last batch is.
+ */
+typedef struct sllm_page_cache sllm_page_cache;
+sllm_status sllm_page_cache_create(int n_layers, int n_kv_heads, int d_k, int page_rows, int n_pages, int type,
+                                   sllm_page_cache **out);
+void sllm_page_cache_destroy(sllm_page_cache *pc);
+sllm_status sllm_page_cache_data(const sllm_page_cache *pc, void **k_dev, void **v_dev);
+/* Pages that nobody holds. */
+sllm_status sllm_page_cache_vacant(const sllm_page_cache *pc, int *pages);
+/* A new sequence without rows. */
+sllm_status sllm_page_seq_add(sllm_page_cache *pc, int *seq);
+/* `count` new sequences that begin with the first `rows` rows of `seq`, holding
+ * its pages with it: nothing is copied before one of the holders appends. */
+sllm_status sllm_page_seq_fork(sllm_page_cache *pc, int seq, int rows, int count, int *out);
+/* The same with pages of their own, copied on `stream`. SLLM_ERR_OOM (and
+ * nothing changed) where there are too few vacant pages. */
+sllm_status sllm_page_seq_copy(sllm_page_cache *pc, int seq, int rows, int count, int *out, void *stream);
+/* `rows` more rows for a sequence, whose contents the caller writes (a stored
+ * session); batches append by sllm_page_batch_begin. SLLM_ERR_OOM (and nothing
+ * changed) where there are too few vacant pages. */
+sllm_status sllm_page_seq_extend(sllm_page_cache *pc, int seq, int rows, void *stream);
+/* The sequence keeps its first `rows` rows; pages behind them are let go. */
+sllm_status sllm_page_seq_truncate(sllm_page_cache *pc, int seq, int rows);
+/* Sequences end and let their pages go (each named once). Contents stay until
+ * the pages are taken again. */
+sllm_status sllm_page_seq_free(sllm_page_cache *pc, const int *seqs, int count);
+sllm_status sllm_page_seq_length(const sllm_page_cache *pc, int seq, int *rows);
+/* The sequences' page numbers, a row of `width` for each, -1 behind a table's
+ * end; *most (may be NULL) the longest table's length. width 0: only that. */
+sllm_status sllm_page_seq_tables(const sllm_page_cache *pc, const int *seqs, int count, int *pages, int width,
+                                 int *most);
+/* Held pages move to the lowest numbers: with n held, those numbered n and
+ * above go, in order, to the vacant ones below n (whole pages, on `stream`).
+ * *used (may be NULL): n. Afterwards the first n pages of each layer are all
+ * that is to be stored, say, of the cache. */
+sllm_status sllm_page_cache_compact(sllm_page_cache *pc, int *used, void *stream);
+
+/*
+ * The steps of up to max_seqs sequences at a time, max_rows rows in all, for
+ * a model of n_heads query heads (n_kv_heads x 1..8). A batch owns the device
+ * memory that its attention calls need, so those allocate nothing.
+ * sllm_page_batch_begin begins a step: rows[i] (0: none) rows are appended to
+ * sequence seqs[i] (each named once), pages taken and shared tail pages copied;
+ * then one sllm_page_attention_dev per layer fills and reads them. SLLM_ERR_OOM
+ * (and nothing changed) where there are too few vacant pages. A step ends with
+ * the next begin; freeing, cutting or moving (compaction, a tail page copied for
+ * another step) one of its sequences ends it too: attention calls are refused
+ * (SLLM_ERR_ARG) until the next begin.
+ */
+typedef struct sllm_page_batch sllm_page_batch;
+sllm_status sllm_page_batch_create(sllm_page_cache *pc, int n_heads, int max_seqs, int max_rows,
+                                   sllm_page_batch **out);
+void sllm_page_batch_destroy(sllm_page_batch *batch);
+sllm_status sllm_page_batch_begin(sllm_page_batch *batch, const int *seqs, const int *rows, int count, void *stream);
+
+/*
+ * The attention section of `layer` for the batch's step (forwardBlock,
+ * model_f32.go:398-466, as sllm_attention_dev for one sequence): q (rows x
+ * n_heads*d_k), k and v (rows x n_kv_heads*d_k) hold the sequences' new rows
+ * one sequence after the other, in the order of begin. Adds the biases,
+ * RMSNorms with QNormW / KNormW, rotates (a row's position is its number in its
+ * sequence), writes the k and v rows into their pages in the cache's type, and
+ * then every row's causal attention over its sequence's rows (as the pages
+ * hold them) to out (rows x n_heads*d_k). q, k, v and out must be 16-byte
+ * aligned; q, k and v are not modified, rows of the pools beyond those appended
+ * neither. Asynchronous on `stream`. A captured call follows the batch's
+ * later steps when it is replayed (their begin calls stay outside the graph), as long as
+ * they fit the buffers that it was captured with (begin says SLLM_ERR_SHAPE where not);
+ * q, k, v and out must then hold max_rows rows.
+ */
+sllm_status sllm_page_attention_dev(sllm_page_batch *batch, int layer, const sllm_attn_params *p, const float *q_dev,
+                                    const float *k_dev, const float *v_dev, float *out_dev, void *stream);
+
+typedef enum { SLLM_LORA_F32 = 0, SLLM_LORA_F16 = 1, SLLM_LORA_BF16 = 2 } sllm_lora_type;
+
+/*
+ * Up to max_adapters low-rank adapters of one projection of `rows` outputs and
+ * `cols` (a multiple of 32) inputs, ranks up to max_rank (at most 256), kept in
+ * device memory in `type`. sllm_lora_set_load puts one into a slot (a: rank x cols,
+ * b: rows x rank, row-major in host memory in the set's type; rank 0 empties
+ * the slot); it is synchronous and waits for the device.
+ */
+typedef struct sllm_lora_set sllm_lora_set;
+sllm_status sllm_lora_set_create(int rows, int cols, int max_adapters, int max_rank, int type, sllm_lora_set **out);
+void sllm_lora_set_destroy(sllm_lora_set *set);
+sllm_status sllm_lora_set_load(sllm_lora_set *set, int slot, int rank, const void *a, const void *b, float scale);
+
+/*
+ * dst[r] = y[r] + scale_a B_a (A_a x[r]) with a = ids[r], for x_rows rows (x:
+ * x_rows x cols, y and dst: x_rows x rows; ids in device memory). Rows whose id
+ * names no loaded adapter (-1, say) get dst[r] = y[r]. dst may be y: the
+ * output of the shared projection (sllm_matmul_dev and its kin) then gets the
+ * adapters' part in place. Products and sums in fp32. x must be 16-byte aligned.
+ * Asynchronous on `stream`; uses the stream's workspace (sllm_workspace_reserve).
+ */
+sllm_status sllm_lora_add_dev(const sllm_lora_set *set, const float *x_dev, int x_rows, const int *ids_dev,
+                              const float *y_dev, float *dst_dev, void *stream);
+
 /* Host-buffer form of sllm_matmul_swiglu_dev (synchronous; h only). */
 sllm_status sllm_matmul_swiglu_into_f32(const sllm_weight *w_gate, const sllm_weight *w_up, const float *x,
                                         int x_rows, int x_cols, float *h);

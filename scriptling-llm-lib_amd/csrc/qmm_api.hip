@@ -13,6 +13,7 @@
 
 #include "qmm_device.hpp"
 #include "qmm_internal.hpp"
+#include "qmm_pages.hpp"
 
 struct sllm_weight {
     int fmt = 0;     // the QType at the ABI
@@ -855,6 +856,10 @@ sllm_status hip_error(hipError_t e, const char *what) {
     g_err = std::string(what) + ": " + hipGetErrorString(e);
     return SLLM_ERR_DEVICE;
 }
+
+sllm_status library_init() { return ensure_init(); }
+bool stream_capturing(hipStream_t s) { return capturing(s); }
+sllm_status stream_workspace(hipStream_t s, size_t need, void **out, size_t *cap) { return workspace(s, need, out, cap); }
 
 Tuning &tuning() {
     static Tuning t;

@@ -1,0 +1,632 @@
+// The page cache of a batch of sequences: who holds which page (host), the copies
+// (device), and the C entry points of the cache, its sequences and its batches.
+//
+// A page is a number of rows (positions) of every kv head of every layer; a sequence is a
+// list of pages. Sequences that begin alike hold the same pages (fork); a shared page
+// that one of them is to write is copied first, its filled rows alone. All decisions
+// are the host's and follow from the calls' order (the lowest vacant page is taken first),
+// so a program can foresee them.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstring>
+#include <new>
+#include <string>
+#include <unordered_map>
+
+#include "qmm_pages.hpp"
+
+struct sllm_page_cache {
+    std::shared_ptr<sllm::PageCache> c;
+};
+struct sllm_page_batch {
+    sllm::PageBatch b;
+};
+
+namespace sllm {
+
+namespace {
+
+typedef int v4i __attribute__((ext_vector_type(4)));
+constexpr int kCopyJobs = 256;  // copies per launch, by value (kernel arguments: 4 KiB)
+struct CopyJobs {
+    PageCopy j[kCopyJobs];
+};
+
+// One workgroup per (copy, K or V of a layer, kv head): the rows of one head of a page are one
+// run of rows x d_k elements (a multiple of 16 bytes). HBM-bound: every byte is read
+// and written once, four 16-byte loads of a thread in flight before its first store.
+__global__ void __launch_bounds__(256) page_copy_kernel(CopyJobs jobs, char *pool_k, char *pool_v, int n_pages, int n_kv,
+                                                        int page_rows, int row_bytes) {
+    const PageCopy j = jobs.j[blockIdx.x];
+    const int layer = blockIdx.y >> 1, head = blockIdx.z;
+    char *pool = blockIdx.y & 1 ? pool_v : pool_k;
+    const size_t run = (size_t)page_rows * row_bytes;
+    const v4i *src = (const v4i *)(pool + (((size_t)layer * n_pages + j.src) * n_kv + head) * run);
+    v4i *dst = (v4i *)(pool + (((size_t)layer * n_pages + j.dst) * n_kv + head) * run);
+    const int n = j.rows * row_bytes / 16;
+    for (int i = threadIdx.x; i < n; i += 4 * 256) {
+        v4i v[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+            if (i + 256 * u < n) v[u] = src[i + 256 * u];
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+            if (i + 256 * u < n) dst[i + 256 * u] = v[u];
+    }
+}
+
+// A C entry ends with a status, whatever the host's allocations do.
+template <class F>
+sllm_status guarded(F f) {
+    try {
+        return f();
+    } catch (const std::bad_alloc &) {
+        return set_error(SLLM_ERR_OOM, "out of memory");
+    } catch (...) {
+        return set_error(SLLM_ERR_ARG, "internal error");
+    }
+}
+
+sllm_status on_device(int device) {
+    int dev = 0;
+    SLLM_HIP(hipGetDevice(&dev));
+    if (dev != device) return set_error(SLLM_ERR_ARG, "the page cache is another device's");
+    return SLLM_OK;
+}
+
+// The pages that appending rows[i] rows to each sequence takes, and whether there are so
+// many; then the appending: the sequences' tables and lengths, and the copies of shared
+// tail pages.
+sllm_status append(PageCache &c, const int *seqs, const int *rows, int n, std::vector<PageCopy> *copies) {
+    std::unordered_map<int, int> lost;  // holders that tail pages lose to copies
+    int64_t need = 0;
+    for (int i = 0; i < n; i++) {
+        const PageSeq &q = c.seqs[(size_t)seqs[i]];
+        if (!rows[i]) continue;
+        if ((int64_t)q.len + rows[i] > INT32_MAX - 512) return set_error(SLLM_ERR_SHAPE, "sequence too long");
+        need += (((int64_t)q.len + rows[i] + c.page_rows - 1) >> c.shift) - (int64_t)q.pages.size();
+        if (q.len & (c.page_rows - 1)) {
+            int &l = lost[q.pages.back()];
+            if (c.refs[(size_t)q.pages.back()] - l > 1) {
+                l++;
+                need++;
+            }
+        }
+    }
+    if (need > c.n_vacant)
+        return set_error(SLLM_ERR_OOM, "page cache: " + std::to_string(need) + " pages needed, " +
+                                           std::to_string(c.n_vacant) + " vacant");
+    copies->reserve(copies->size() + lost.size() + (size_t)n);
+    for (int i = 0; i < n; i++) {
+        PageSeq &q = c.seqs[(size_t)seqs[i]];
+        if (rows[i]) q.pages.reserve((size_t)(((int64_t)q.len + rows[i] + c.page_rows - 1) >> c.shift));
+    }
+    // nothing below allocates
+    for (int i = 0; i < n; i++) {
+        PageSeq &q = c.seqs[(size_t)seqs[i]];
+        if (!rows[i]) continue;
+        const int filled = q.len & (c.page_rows - 1);
+        if (filled && c.refs[(size_t)q.pages.back()] > 1) {
+            const int to = c.take();
+            copies->push_back({q.pages.back(), to, filled});
+            c.drop(q.pages.back());
+            q.pages.back() = to;
+            q.version++;
+        }
+        q.len += rows[i];
+        while ((int64_t)q.pages.size() < (((int64_t)q.len + c.page_rows - 1) >> c.shift)) q.pages.push_back(c.take());
+    }
+    return SLLM_OK;
+}
+
+int new_seq(PageCache &c) {
+    if (!c.spare.empty()) {
+        const int s = c.spare.back();
+        c.spare.pop_back();
+        c.seqs[(size_t)s].live = true;
+        return s;
+    }
+    c.seqs.emplace_back();
+    c.spare.reserve(c.seqs.size());  // ending a sequence does not allocate
+    c.seqs.back().live = true;
+    return (int)c.seqs.size() - 1;
+}
+
+void end_seq(PageCache &c, int s) {
+    PageSeq &q = c.seqs[(size_t)s];
+    for (int p : q.pages) c.drop(p);
+    q.pages.clear();
+    q.len = 0;
+    q.live = false;
+    q.version++;
+    c.spare.insert(std::lower_bound(c.spare.begin(), c.spare.end(), s, [](int a, int b) { return a > b; }), s);
+}
+
+}  // namespace
+
+PageCache::~PageCache() {
+    if (k) (void)hipFree(k);
+    if (v) (void)hipFree(v);
+}
+
+int PageCache::take() {
+    while (!vacant[first_word]) first_word++;
+    const int p = (int)(first_word * 64) + __builtin_ctzll(vacant[first_word]);
+    vacant[first_word] &= vacant[first_word] - 1;
+    n_vacant--;
+    refs[(size_t)p] = 1;
+    return p;
+}
+
+void PageCache::drop(int page) {
+    if (--refs[(size_t)page]) return;
+    vacant[(size_t)page / 64] |= 1ull << (page % 64);
+    n_vacant++;
+    first_word = std::min(first_word, (size_t)page / 64);
+}
+
+PageBatch::~PageBatch() {
+    for (int i = 0; i < kSlots; i++) {
+        if (done[i]) {
+            (void)hipEventSynchronize(done[i]);
+            (void)hipEventDestroy(done[i]);
+        }
+        if (host[i]) (void)hipHostFree(host[i]);
+    }
+    if (dev) (void)hipFree(dev);
+    for (void *p : retired) (void)hipFree(p);
+    if (qrot) (void)hipFree(qrot);
+}
+
+sllm_status launch_page_copies(const PageCache &c, const PageCopy *jobs, size_t n, hipStream_t s) {
+    CopyJobs j;
+    for (size_t at = 0; at < n; at += kCopyJobs) {
+        const size_t m = std::min<size_t>(kCopyJobs, n - at);
+        std::memcpy(j.j, jobs + at, m * sizeof(PageCopy));
+        hipLaunchKernelGGL(page_copy_kernel, dim3((unsigned)m, (unsigned)c.n_layers * 2, (unsigned)c.n_kv), dim3(256), 0, s,
+                           j, c.k, c.v, c.n_pages, c.n_kv, c.page_rows, c.d_k * c.elem());
+        SLLM_HIP(hipGetLastError());
+    }
+    return SLLM_OK;
+}
+
+}  // namespace sllm
+
+using namespace sllm;
+
+extern "C" {
+
+sllm_status sllm_page_cache_create(int n_layers, int n_kv_heads, int d_k, int page_rows, int n_pages, int type,
+                                   sllm_page_cache **out) {
+    if (!out) return set_error(SLLM_ERR_ARG, "null pointer");
+    *out = nullptr;
+    if (n_layers <= 0 || n_kv_heads <= 0 || d_k <= 0 || n_pages <= 0)
+        return set_error(SLLM_ERR_ARG, "page cache dimensions must be positive");
+    if (d_k % 8 != 0 || d_k > 256) return set_error(SLLM_ERR_SHAPE, "d_k must be a multiple of 8, at most 256");
+    if (page_rows < 16 || page_rows > 256 || (page_rows & (page_rows - 1)))
+        return set_error(SLLM_ERR_SHAPE, "page_rows must be 16, 32, 64, 128 or 256");
+    if (n_layers > 32767 || n_kv_heads > 65535) return set_error(SLLM_ERR_SHAPE, "too many layers or kv heads");
+    if (type != SLLM_CACHE_F32 && type != SLLM_CACHE_F16) return set_error(SLLM_ERR_ARG, "unknown cache type");
+    // one side of the pool, in 64 bits: each factor is bounded above but the pages
+    const double bytes_d = (double)n_layers * n_kv_heads * d_k * page_rows * n_pages * 4;
+    if (bytes_d > 1e15) return set_error(SLLM_ERR_OOM, "page cache allocation failed");
+    return guarded([&]() -> sllm_status {
+        sllm_status st = library_init();
+        if (st != SLLM_OK) return st;
+        auto c = std::make_shared<PageCache>();
+        c->n_layers = n_layers;
+        c->n_kv = n_kv_heads;
+        c->d_k = d_k;
+        c->page_rows = page_rows;
+        c->shift = __builtin_ctz((unsigned)page_rows);
+        c->n_pages = n_pages;
+        c->type = type;
+        SLLM_HIP(hipGetDevice(&c->device));
+        c->refs.assign((size_t)n_pages, 0);
+        c->vacant.assign(((size_t)n_pages + 63) / 64, ~0ull);
+        if (n_pages % 64) c->vacant.back() = (1ull << (n_pages % 64)) - 1;
+        c->n_vacant = n_pages;
+        const size_t bytes = (size_t)n_layers * n_pages * n_kv_heads * page_rows * d_k * c->elem();
+        if (hipMalloc(&c->k, bytes) != hipSuccess || hipMalloc(&c->v, bytes) != hipSuccess) {
+            (void)hipGetLastError();
+            return set_error(SLLM_ERR_OOM, "page cache allocation failed");
+        }
+        SLLM_HIP(hipMemsetAsync(c->k, 0, bytes, nullptr));
+        SLLM_HIP(hipMemsetAsync(c->v, 0, bytes, nullptr));
+        SLLM_HIP(hipStreamSynchronize(nullptr));
+        *out = new sllm_page_cache{std::move(c)};
+        return SLLM_OK;
+    });
+}
+
+void sllm_page_cache_destroy(sllm_page_cache *pc) { delete pc; }
+
+sllm_status sllm_page_cache_data(const sllm_page_cache *pc, void **k_dev, void **v_dev) {
+    if (!pc || !k_dev || !v_dev) return set_error(SLLM_ERR_ARG, "null pointer");
+    *k_dev = pc->c->k;
+    *v_dev = pc->c->v;
+    return SLLM_OK;
+}
+
+sllm_status sllm_page_cache_vacant(const sllm_page_cache *pc, int *pages) {
+    if (!pc || !pages) return set_error(SLLM_ERR_ARG, "null pointer");
+    std::lock_guard<std::mutex> lk(pc->c->mu);
+    *pages = pc->c->n_vacant;
+    return SLLM_OK;
+}
+
+sllm_status sllm_page_seq_add(sllm_page_cache *pc, int *seq) {
+    if (!pc || !seq) return set_error(SLLM_ERR_ARG, "null pointer");
+    return guarded([&] {
+        std::lock_guard<std::mutex> lk(pc->c->mu);
+        *seq = new_seq(*pc->c);
+        return SLLM_OK;
+    });
+}
+
+// fork (copies null) and copy: `count` new sequences of the first `rows` rows of `seq`
+static sllm_status duplicate(PageCache &c, int seq, int rows, int count, int *out, std::vector<PageCopy> *copies) {
+    if (!c.live(seq)) return set_error(SLLM_ERR_ARG, "no such sequence");
+    if (count < 0) return set_error(SLLM_ERR_ARG, "count must not be negative");
+    if (rows < 0 || rows > c.seqs[(size_t)seq].len) return set_error(SLLM_ERR_ARG, "rows outside 0 .. the sequence's length");
+    const int pages = (int)(((int64_t)rows + c.page_rows - 1) >> c.shift);
+    if (copies && (int64_t)pages * count > c.n_vacant)
+        return set_error(SLLM_ERR_OOM, "page cache: " + std::to_string((int64_t)pages * count) + " pages needed, " +
+                                           std::to_string(c.n_vacant) + " vacant");
+    if (copies) copies->reserve((size_t)pages * count);
+    c.seqs.reserve(c.seqs.size() + (size_t)count);
+    int made = 0;
+    try {
+        for (; made < count; made++) {
+            const int s = new_seq(c);
+            out[made] = s;
+            PageSeq &q = c.seqs[(size_t)s];
+            try {
+                q.pages.reserve((size_t)pages);
+            } catch (...) {
+                end_seq(c, s);
+                throw;
+            }
+            q.len = rows;
+            for (int i = 0; i < pages; i++) {
+                const int p = c.seqs[(size_t)seq].pages[(size_t)i];
+                if (copies) {
+                    const int to = c.take();
+                    copies->push_back({p, to, std::min(c.page_rows, rows - (i << c.shift))});
+                    q.pages.push_back(to);
+                } else {
+                    c.refs[(size_t)p]++;
+                    q.pages.push_back(p);
+                }
+            }
+        }
+    } catch (...) {
+        while (made > 0) end_seq(c, out[--made]);
+        throw;
+    }
+    return SLLM_OK;
+}
+
+sllm_status sllm_page_seq_fork(sllm_page_cache *pc, int seq, int rows, int count, int *out) {
+    if (!pc || (!out && count > 0)) return set_error(SLLM_ERR_ARG, "null pointer");
+    return guarded([&] {
+        std::lock_guard<std::mutex> lk(pc->c->mu);
+        return duplicate(*pc->c, seq, rows, count, out, nullptr);
+    });
+}
+
+sllm_status sllm_page_seq_copy(sllm_page_cache *pc, int seq, int rows, int count, int *out, void *stream) {
+    if (!pc || (!out && count > 0)) return set_error(SLLM_ERR_ARG, "null pointer");
+    return guarded([&]() -> sllm_status {
+        PageCache &c = *pc->c;
+        std::lock_guard<std::mutex> lk(c.mu);
+        sllm_status st = on_device(c.device);
+        if (st != SLLM_OK) return st;
+        if (stream_capturing((hipStream_t)stream))
+            return set_error(SLLM_ERR_ARG, "a page cache's sequences cannot change under capture");
+        std::vector<PageCopy> copies;
+        if ((st = duplicate(c, seq, rows, count, out, &copies)) != SLLM_OK) return st;
+        return launch_page_copies(c, copies.data(), copies.size(), (hipStream_t)stream);
+    });
+}
+
+sllm_status sllm_page_seq_extend(sllm_page_cache *pc, int seq, int rows, void *stream) {
+    if (!pc) return set_error(SLLM_ERR_ARG, "null pointer");
+    return guarded([&]() -> sllm_status {
+        PageCache &c = *pc->c;
+        std::lock_guard<std::mutex> lk(c.mu);
+        if (!c.live(seq)) return set_error(SLLM_ERR_ARG, "no such sequence");
+        if (rows < 0) return set_error(SLLM_ERR_ARG, "rows must not be negative");
+        sllm_status st = on_device(c.device);
+        if (st != SLLM_OK) return st;
+        if (stream_capturing((hipStream_t)stream))
+            return set_error(SLLM_ERR_ARG, "a page cache's sequences cannot change under capture");
+        std::vector<PageCopy> copies;
+        if ((st = append(c, &seq, &rows, 1, &copies)) != SLLM_OK) return st;
+        return launch_page_copies(c, copies.data(), copies.size(), (hipStream_t)stream);
+    });
+}
+
+sllm_status sllm_page_seq_truncate(sllm_page_cache *pc, int seq, int rows) {
+    if (!pc) return set_error(SLLM_ERR_ARG, "null pointer");
+    PageCache &c = *pc->c;
+    std::lock_guard<std::mutex> lk(c.mu);
+    if (!c.live(seq)) return set_error(SLLM_ERR_ARG, "no such sequence");
+    PageSeq &q = c.seqs[(size_t)seq];
+    if (rows < 0 || rows > q.len) return set_error(SLLM_ERR_ARG, "rows outside 0 .. the sequence's length");
+    if (rows < q.len) q.version++;
+    q.len = rows;
+    while ((int64_t)q.pages.size() > (((int64_t)rows + c.page_rows - 1) >> c.shift)) {
+        c.drop(q.pages.back());
+        q.pages.pop_back();
+    }
+    return SLLM_OK;
+}
+
+sllm_status sllm_page_seq_free(sllm_page_cache *pc, const int *seqs, int count) {
+    if (!pc || (!seqs && count > 0)) return set_error(SLLM_ERR_ARG, "null pointer");
+    if (count < 0) return set_error(SLLM_ERR_ARG, "count must not be negative");
+    return guarded([&]() -> sllm_status {
+        PageCache &c = *pc->c;
+        std::lock_guard<std::mutex> lk(c.mu);
+        std::vector<int> s(seqs, seqs + count);
+        std::sort(s.begin(), s.end());
+        for (size_t i = 0; i < s.size(); i++) {
+            if (!c.live(s[i])) return set_error(SLLM_ERR_ARG, "no such sequence");
+            if (i && s[i] == s[i - 1]) return set_error(SLLM_ERR_ARG, "a sequence is named twice");
+        }
+        for (int q : s) end_seq(c, q);
+        return SLLM_OK;
+    });
+}
+
+sllm_status sllm_page_seq_length(const sllm_page_cache *pc, int seq, int *rows) {
+    if (!pc || !rows) return set_error(SLLM_ERR_ARG, "null pointer");
+    std::lock_guard<std::mutex> lk(pc->c->mu);
+    if (!pc->c->live(seq)) return set_error(SLLM_ERR_ARG, "no such sequence");
+    *rows = pc->c->seqs[(size_t)seq].len;
+    return SLLM_OK;
+}
+
+sllm_status sllm_page_seq_tables(const sllm_page_cache *pc, const int *seqs, int count, int *pages, int width, int *most) {
+    if (!pc || (count > 0 && !seqs)) return set_error(SLLM_ERR_ARG, "null pointer");
+    if (count < 0 || width < 0 || (width > 0 && count > 0 && !pages)) return set_error(SLLM_ERR_ARG, "bad table size");
+    const PageCache &c = *pc->c;
+    std::lock_guard<std::mutex> lk(pc->c->mu);
+    int longest = 0;
+    for (int i = 0; i < count; i++) {
+        if (!c.live(seqs[i])) return set_error(SLLM_ERR_ARG, "no such sequence");
+        longest = std::max(longest, (int)c.seqs[(size_t)seqs[i]].pages.size());
+    }
+    if (most) *most = longest;
+    if (!width) return SLLM_OK;
+    if (width < longest) return set_error(SLLM_ERR_ARG, "width is less than the longest table");
+    for (int i = 0; i < count; i++) {
+        const std::vector<int> &t = c.seqs[(size_t)seqs[i]].pages;
+        int *row = pages + (size_t)i * width;
+        std::copy(t.begin(), t.end(), row);
+        std::fill(row + t.size(), row + width, -1);
+    }
+    return SLLM_OK;
+}
+
+sllm_status sllm_page_cache_compact(sllm_page_cache *pc, int *used, void *stream) {
+    if (!pc) return set_error(SLLM_ERR_ARG, "null pointer");
+    return guarded([&]() -> sllm_status {
+        PageCache &c = *pc->c;
+        std::lock_guard<std::mutex> lk(c.mu);
+        sllm_status st = on_device(c.device);
+        if (st != SLLM_OK) return st;
+        if (stream_capturing((hipStream_t)stream))
+            return set_error(SLLM_ERR_ARG, "a page cache's sequences cannot change under capture");
+        const int n = c.n_pages - c.n_vacant;
+        std::vector<PageCopy> copies;
+        std::unordered_map<int, int> to;
+        int gap = 0;
+        for (int p = n; p < c.n_pages; p++) {
+            if (!c.refs[(size_t)p]) continue;
+            while (c.refs[(size_t)gap]) gap++;
+            copies.push_back({p, gap, c.page_rows});
+            to[p] = gap++;
+        }
+        if ((st = launch_page_copies(c, copies.data(), copies.size(), (hipStream_t)stream)) != SLLM_OK) return st;
+        for (const PageCopy &j : copies) {
+            c.refs[(size_t)j.dst] = c.refs[(size_t)j.src];
+            c.refs[(size_t)j.src] = 0;
+            c.vacant[(size_t)j.dst / 64] &= ~(1ull << (j.dst % 64));
+            c.vacant[(size_t)j.src / 64] |= 1ull << (j.src % 64);
+        }
+        c.first_word = 0;
+        if (!copies.empty())
+            for (PageSeq &q : c.seqs) {
+                bool moved = false;
+                for (int &p : q.pages) {
+                    if (p < n) continue;
+                    p = to[p];
+                    moved = true;
+                }
+                q.version += moved;
+            }
+        if (used) *used = n;
+        return SLLM_OK;
+    });
+}
+
+sllm_status sllm_page_batch_create(sllm_page_cache *pc, int n_heads, int max_seqs, int max_rows, sllm_page_batch **out) {
+    if (!out) return set_error(SLLM_ERR_ARG, "null pointer");
+    *out = nullptr;
+    if (!pc) return set_error(SLLM_ERR_ARG, "null pointer");
+    if (max_seqs <= 0 || max_rows <= 0) return set_error(SLLM_ERR_ARG, "max_seqs and max_rows must be positive");
+    const PageCache &c = *pc->c;
+    if (n_heads <= 0 || n_heads % c.n_kv != 0 || n_heads / c.n_kv > 8)
+        return set_error(SLLM_ERR_SHAPE, "n_heads must be a multiple of n_kv_heads, at most 8 times it");
+    if ((int64_t)max_rows * n_heads > (1 << 26)) return set_error(SLLM_ERR_SHAPE, "max_rows x n_heads must stay below 2^26");
+    return guarded([&]() -> sllm_status {
+        sllm_status st = on_device(c.device);
+        if (st != SLLM_OK) return st;
+        auto b = std::make_unique<sllm_page_batch>();
+        b->b.c = pc->c;
+        b->b.n_heads = n_heads;
+        b->b.max_seqs = max_seqs;
+        b->b.max_rows = max_rows;
+        b->b.seqs.reserve((size_t)max_seqs);
+        b->b.versions.reserve((size_t)max_seqs);
+        if (hipMalloc(&b->b.qrot, (size_t)max_rows * n_heads * c.d_k * sizeof(float)) != hipSuccess) {
+            b->b.qrot = nullptr;
+            (void)hipGetLastError();
+            return set_error(SLLM_ERR_OOM, "page batch allocation failed");
+        }
+        for (hipEvent_t &e : b->b.done) SLLM_HIP(hipEventCreateWithFlags(&e, hipEventDisableTiming));
+        *out = b.release();
+        return SLLM_OK;
+    });
+}
+
+void sllm_page_batch_destroy(sllm_page_batch *batch) { delete batch; }
+
+sllm_status sllm_page_batch_begin(sllm_page_batch *batch, const int *seqs, const int *rows, int count, void *stream) {
+    if (!batch || (count > 0 && (!seqs || !rows))) return set_error(SLLM_ERR_ARG, "null pointer");
+    PageBatch &b = batch->b;
+    if (count < 0 || count > b.max_seqs) return set_error(SLLM_ERR_ARG, "count outside 0 .. max_seqs");
+    hipStream_t s = (hipStream_t)stream;
+    return guarded([&]() -> sllm_status {
+        std::lock_guard<std::mutex> lb(b.mu);
+        PageCache &c = *b.c;
+        std::lock_guard<std::mutex> lk(c.mu);
+        int64_t total = 0, pages = 0;
+        std::vector<int> sorted(seqs, seqs + count);
+        std::sort(sorted.begin(), sorted.end());
+        for (int i = 0; i < count; i++) {
+            if (!c.live(seqs[i])) return set_error(SLLM_ERR_ARG, "no such sequence");
+            if (i && sorted[(size_t)i] == sorted[(size_t)i - 1]) return set_error(SLLM_ERR_ARG, "a sequence is named twice");
+            if (rows[i] < 0) return set_error(SLLM_ERR_ARG, "rows must not be negative");
+            total += rows[i];
+            pages += ((int64_t)c.seqs[(size_t)seqs[i]].len + rows[i] + c.page_rows - 1) >> c.shift;
+        }
+        if (total > b.max_rows) return set_error(SLLM_ERR_SHAPE, "more rows than max_rows");
+        sllm_status st = on_device(c.device);
+        if (st != SLLM_OK) return st;
+        if (stream_capturing(s)) return set_error(SLLM_ERR_ARG, "a batch's step cannot begin under capture");
+        // room for the step on the device and in the next staging slot
+        const size_t bytes = (size_t)(kStepHeader + 4 * (int64_t)b.max_rows + pages) * sizeof(int);
+        if (b.dev_cap < bytes) {
+            if (b.captured)
+                return set_error(SLLM_ERR_SHAPE, "the step has more pages than the batch held when it was captured");
+            void *p = nullptr;
+            const size_t want = 2 * bytes + 4096;
+            if (hipMalloc(&p, want) != hipSuccess) {
+                (void)hipGetLastError();
+                return set_error(SLLM_ERR_OOM, "page batch allocation failed");
+            }
+            if (b.dev) b.retired.push_back(b.dev);
+            b.dev = (int *)p;
+            b.dev_cap = want;
+        }
+        const int slot = b.slot;
+        SLLM_HIP(hipEventSynchronize(b.done[slot]));
+        if (b.host_cap[slot] < bytes) {
+            if (b.host[slot]) (void)hipHostFree(b.host[slot]);
+            b.host[slot] = nullptr;
+            b.host_cap[slot] = 0;
+            if (hipHostMalloc((void **)&b.host[slot], b.dev_cap, hipHostMallocDefault) != hipSuccess) {
+                (void)hipGetLastError();
+                return set_error(SLLM_ERR_OOM, "page batch staging allocation failed");
+            }
+            b.host_cap[slot] = b.dev_cap;
+        }
+        std::vector<PageCopy> copies;
+        if ((st = append(c, seqs, rows, count, &copies)) != SLLM_OK) return st;
+        int *h = (int *)b.host[slot];
+        std::memset(h, 0, kStepHeader * sizeof(int));
+        h[0] = (int)total;
+        StepRow *hr = (StepRow *)(h + kStepHeader);
+        int *ht = h + kStepHeader + 4 * (size_t)b.max_rows;
+        int at = 0;
+        for (int i = 0; i < count; i++) {
+            const PageSeq &q = c.seqs[(size_t)seqs[i]];
+            for (int r = 0; r < rows[i]; r++) {
+                const int pos = q.len - rows[i] + r;
+                *hr++ = {q.pages[(size_t)(pos >> c.shift)], pos & (c.page_rows - 1), pos, at};
+            }
+            std::copy(q.pages.begin(), q.pages.end(), ht + at);
+            at += (int)q.pages.size();
+        }
+        b.seqs.assign(seqs, seqs + count);
+        b.versions.resize((size_t)count);
+        for (int i = 0; i < count; i++) b.versions[(size_t)i] = c.seqs[(size_t)seqs[i]].version;
+        b.rows = (int)total;
+        b.begun = true;
+        if ((st = launch_page_copies(c, copies.data(), copies.size(), s)) != SLLM_OK) return st;
+        SLLM_HIP(hipMemcpyAsync(b.dev, h, bytes, hipMemcpyHostToDevice, s));
+        SLLM_HIP(hipEventRecord(b.done[slot], s));
+        b.slot = (slot + 1) % PageBatch::kSlots;
+        return SLLM_OK;
+    });
+}
+
+sllm_status sllm_page_attention_dev(sllm_page_batch *batch, int layer, const sllm_attn_params *p, const float *q,
+                                    const float *k, const float *v, float *out, void *stream) {
+    if (!batch || !p || !q || !k || !v || !out) return set_error(SLLM_ERR_ARG, "null pointer");
+    PageBatch &b = batch->b;
+    std::lock_guard<std::mutex> lb(b.mu);
+    PageCache &c = *b.c;
+    if (layer < 0 || layer >= c.n_layers) return set_error(SLLM_ERR_ARG, "layer out of range");
+    if (p->n_heads != b.n_heads || p->n_kv_heads != c.n_kv || p->d_k != c.d_k)
+        return set_error(SLLM_ERR_ARG, "n_heads / n_kv_heads / d_k differ from the batch's");
+    if (p->rope_half_dim < 0 || 2 * p->rope_half_dim > p->d_k)
+        return set_error(SLLM_ERR_ARG, "rope_half_dim outside 0 .. d_k / 2");
+    if (p->rope_half_dim > 0 && !p->rope_freqs) return set_error(SLLM_ERR_ARG, "null rope_freqs");
+    if (p->q_bias_len < 0 || p->k_bias_len < 0 || p->v_bias_len < 0)
+        return set_error(SLLM_ERR_ARG, "negative bias length");
+    if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & 15)
+        return set_error(SLLM_ERR_ARG, "q, k, v and out must be 16-byte aligned");
+    {
+        std::lock_guard<std::mutex> lk(c.mu);
+        if (!b.begun) return set_error(SLLM_ERR_ARG, "the batch has no step: sllm_page_batch_begin first");
+        for (size_t i = 0; i < b.seqs.size(); i++)
+            if (c.seqs[(size_t)b.seqs[i]].version != b.versions[i])
+                return set_error(SLLM_ERR_ARG, "a sequence of the step was freed, cut or moved: begin it again");
+    }
+    sllm_status st = on_device(c.device);
+    if (st != SLLM_OK) return st;
+    hipStream_t s = (hipStream_t)stream;
+    const bool capture = stream_capturing(s);
+    if (!b.rows && !capture) return SLLM_OK;
+    PageAttnArgs a{};
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.out = out;
+    a.n_heads = b.n_heads;
+    a.n_kv = c.n_kv;
+    a.d_k = c.d_k;
+    a.rep = b.n_heads / c.n_kv;
+    a.shift = c.shift;
+    a.n_pages = c.n_pages;
+    a.q_bias = p->q_bias_len ? p->q_bias : nullptr;
+    a.k_bias = p->k_bias_len ? p->k_bias : nullptr;
+    a.v_bias = p->v_bias_len ? p->v_bias : nullptr;
+    a.qb_len = p->q_bias_len;
+    a.kb_len = p->k_bias_len;
+    a.vb_len = p->v_bias_len;
+    a.q_norm = p->q_norm_w;
+    a.k_norm = p->k_norm_w;
+    a.eps = p->norm_eps;
+    a.freqs = p->rope_freqs;
+    a.half_dim = p->rope_half_dim;
+    a.scale = 1.0f / (float)__builtin_sqrt((double)c.d_k);
+    const size_t loff = (size_t)layer * c.n_pages * c.n_kv * c.page_rows * c.d_k * c.elem();
+    a.pool_k = c.k + loff;
+    a.pool_v = c.v + loff;
+    a.step = b.dev;
+    a.rows = (const StepRow *)(b.dev + kStepHeader);
+    a.tables = b.dev + kStepHeader + 4 * (size_t)b.max_rows;
+    a.qrot = b.qrot;
+    a.grid_rows = capture ? b.max_rows : b.rows;
+    a.type = c.type;
+    b.captured |= capture;
+    return launch_page_attention(a, s);
+}
+
+}  // extern "C"

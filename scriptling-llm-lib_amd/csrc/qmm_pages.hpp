@@ -1,0 +1,112 @@
+// A cache of pages for many sequences, its batches, and the kernels' view of them.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstddef>
+#include <cstdint>
+#include <memory>
+#include <mutex>
+#include <vector>
+
+#include "qmm_internal.hpp"
+
+namespace sllm {
+
+// Rows of a page to copy to another page, in every layer, of K and of V.
+struct PageCopy {
+    int src, dst, rows;
+};
+
+struct PageSeq {
+    bool live = false;
+    int len = 0;
+    // raised whenever rows of the sequence move or end (free, truncate, a copied tail
+    // page, compact): a batch begun before that is refused
+    uint32_t version = 0;
+    std::vector<int> pages;  // ceil(len / page_rows) page ids
+};
+
+// The pools [layer][page][kv head][row of the page][d_k], and who holds which page.
+struct PageCache {
+    int n_layers = 0, n_kv = 0, d_k = 0, page_rows = 0, shift = 0, n_pages = 0, type = 0, device = 0;
+    char *k = nullptr, *v = nullptr;
+    std::vector<int> refs;          // sequences holding each page
+    std::vector<uint64_t> vacant;   // bit per page without holders
+    int n_vacant = 0;
+    size_t first_word = 0;          // no vacant page in words below
+    std::vector<PageSeq> seqs;
+    std::vector<int> spare;         // dead sequence ids, the lowest last
+    std::mutex mu;
+
+    ~PageCache();
+    int elem() const { return type == SLLM_CACHE_F16 ? 2 : 4; }
+    // pages that appending `rows` rows to sequence s takes; `gone`: holders that tail pages
+    // lose to copies made before in the same call
+    bool live(int s) const { return s >= 0 && s < (int)seqs.size() && seqs[(size_t)s].live; }
+    int take();           // the lowest vacant page (n_vacant > 0), held once
+    void drop(int page);  // one holder less
+};
+
+// What the kernels read of a step, in device memory at addresses that stay
+// for the batch's life, so that captured launches follow later steps.
+struct StepRow {
+    int page, slot;  // where the row's K and V go
+    int pos;         // its position
+    int table;       // its sequence's page ids, at tables[table]
+};
+
+struct PageBatch {
+    std::shared_ptr<PageCache> c;
+    int n_heads = 0, max_seqs = 0, max_rows = 0;
+    std::vector<int> seqs;           // the current step's sequences
+    std::vector<uint32_t> versions;  // as they were at its begin
+    int rows = 0;
+    bool begun = false, captured = false;
+    int *dev = nullptr;              // the step: header, rows, tables (device)
+    size_t dev_cap = 0;              // bytes
+    std::vector<void *> retired;
+    float *qrot = nullptr;           // max_rows x n_heads x d_k
+    // staging of a step on the host: a slot is written again when its upload is done
+    static constexpr int kSlots = 4;
+    char *host[kSlots] = {};
+    size_t host_cap[kSlots] = {};
+    hipEvent_t done[kSlots] = {};
+    int slot = 0;
+    std::mutex mu;
+
+    ~PageBatch();
+};
+
+// The attention section of one layer for a batch's step.
+struct PageAttnArgs {
+    const float *q, *k, *v;
+    float *out;
+    int n_heads, n_kv, d_k, rep, shift, n_pages;
+    const float *q_bias, *k_bias, *v_bias;
+    int qb_len, kb_len, vb_len;
+    const float *q_norm, *k_norm;
+    float eps;
+    const float *freqs;
+    int half_dim;
+    float scale;
+    char *pool_k, *pool_v;  // this layer
+    const int *step;        // header: [0] rows
+    const StepRow *rows;
+    const int *tables;
+    float *qrot;
+    int grid_rows;          // rows launched (the step's, or max_rows under capture)
+    int type;
+};
+constexpr int kStepHeader = 16;  // ints
+
+sllm_status launch_page_copies(const PageCache &c, const PageCopy *jobs, size_t n, hipStream_t s);
+sllm_status launch_page_attention(const PageAttnArgs &a, hipStream_t s);
+
+// Of qmm_api.hip: the library's set-up, and whether a stream is under capture.
+sllm_status library_init();
+bool stream_capturing(hipStream_t s);
+// The stream's workspace, grown to at least `need` bytes (not under capture).
+sllm_status stream_workspace(hipStream_t s, size_t need, void **out, size_t *cap);
+
+}  // namespace sllm

@@ -115,11 +115,33 @@ def lib() -> C.CDLL:
     L.sllm_attention_dev.argtypes = [P, i32, C.POINTER(AttnParams), P, P, P, i32, i32, P, P]
     L.sllm_attention_noalloc_dev.argtypes = [P, i32, C.POINTER(AttnParams), P, P, P, i32, i32, P, P]
     L.sllm_workspace_reserve.argtypes = [P, sz]
+    I = C.POINTER(i32)
+    L.sllm_page_cache_create.argtypes = [i32, i32, i32, i32, i32, i32, C.POINTER(P)]
+    L.sllm_page_cache_destroy.argtypes = [P]
+    L.sllm_page_cache_data.argtypes = [P, C.POINTER(P), C.POINTER(P)]
+    L.sllm_page_cache_vacant.argtypes = [P, I]
+    L.sllm_page_seq_add.argtypes = [P, I]
+    L.sllm_page_seq_fork.argtypes = [P, i32, i32, i32, I]
+    L.sllm_page_seq_copy.argtypes = [P, i32, i32, i32, I, P]
+    L.sllm_page_seq_extend.argtypes = [P, i32, i32, P]
+    L.sllm_page_seq_truncate.argtypes = [P, i32, i32]
+    L.sllm_page_seq_free.argtypes = [P, I, i32]
+    L.sllm_page_seq_length.argtypes = [P, i32, I]
+    L.sllm_page_seq_tables.argtypes = [P, I, i32, I, i32, I]
+    L.sllm_page_cache_compact.argtypes = [P, I, P]
+    L.sllm_page_batch_create.argtypes = [P, i32, i32, i32, C.POINTER(P)]
+    L.sllm_page_batch_destroy.argtypes = [P]
+    L.sllm_page_batch_begin.argtypes = [P, I, I, i32, P]
+    L.sllm_page_attention_dev.argtypes = [P, i32, C.POINTER(AttnParams), P, P, P, P, P]
+    L.sllm_lora_set_create.argtypes = [i32, i32, i32, i32, i32, C.POINTER(P)]
+    L.sllm_lora_set_destroy.argtypes = [P]
+    L.sllm_lora_set_load.argtypes = [P, i32, i32, P, P, f32]
+    L.sllm_lora_add_dev.argtypes = [P, P, i32, P, P, P, P]
     for name in exported_names():  # raises AttributeError if a declared symbol is missing
         f = getattr(L, name)
         if name in ("sllm_last_error", "sllm_kernel_info"):
             f.restype = C.c_char_p
-        elif name in ("sllm_weight_destroy", "sllm_kv_cache_destroy"):
+        elif name.endswith("_destroy"):
             f.restype = None
         else:
             f.restype = i32
@@ -450,6 +472,190 @@ def attention_noalloc_dev(kv: KVCache, layer: int, params: AttnParams, q_ptr: in
 def workspace_reserve(stream: int, nbytes: int) -> None:
     """Grow the stream's device workspace to at least nbytes now (before a graph capture)."""
     _check(lib().sllm_workspace_reserve(C.c_void_p(stream), int(nbytes)))
+
+
+CACHE_TYPES = {"f32": 0, "f16": 1}
+LORA_TYPES = {"f32": 0, "f16": 1, "bf16": 2}
+
+
+def _ints(values):
+    return (C.c_int * len(values))(*values)
+
+
+class PageCache:
+    """K and V of many sequences in pages that they may share (sllm_page_cache). Sequences are numbers."""
+
+    def __init__(self, n_layers: int, n_kv_heads: int, d_k: int, page_rows: int, n_pages: int, dtype: str = "f32"):
+        self.handle = None
+        if dtype not in CACHE_TYPES:
+            raise SllmError(1, f"unknown cache type {dtype}")
+        h = C.c_void_p()
+        _check(lib().sllm_page_cache_create(n_layers, n_kv_heads, d_k, page_rows, n_pages, CACHE_TYPES[dtype],
+                                            C.byref(h)))
+        self.handle = h
+        self.n_layers, self.n_kv_heads, self.d_k = n_layers, n_kv_heads, d_k
+        self.page_rows, self.n_pages, self.dtype = page_rows, n_pages, dtype
+
+    def close(self) -> None:
+        if self.handle:
+            lib().sllm_page_cache_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def data(self) -> tuple[int, int]:
+        """Device addresses of the K and V pools: [layer][page][kv head][row][d_k]."""
+        k, v = C.c_void_p(), C.c_void_p()
+        _check(lib().sllm_page_cache_data(self.handle, C.byref(k), C.byref(v)))
+        return k.value, v.value
+
+    def vacant(self) -> int:
+        n = C.c_int()
+        _check(lib().sllm_page_cache_vacant(self.handle, C.byref(n)))
+        return n.value
+
+    def add(self) -> int:
+        s = C.c_int()
+        _check(lib().sllm_page_seq_add(self.handle, C.byref(s)))
+        return s.value
+
+    def fork(self, seq: int, rows: int, count: int = 1) -> list[int]:
+        """New sequences that share the first rows of seq."""
+        out = (C.c_int * max(count, 1))()
+        _check(lib().sllm_page_seq_fork(self.handle, seq, rows, count, out))
+        return list(out[:max(count, 0)])
+
+    def copy(self, seq: int, rows: int, count: int = 1, stream: int = 0) -> list[int]:
+        """New sequences with copies of the first rows of seq."""
+        out = (C.c_int * max(count, 1))()
+        _check(lib().sllm_page_seq_copy(self.handle, seq, rows, count, out, C.c_void_p(stream)))
+        return list(out[:max(count, 0)])
+
+    def extend(self, seq: int, rows: int, stream: int = 0) -> None:
+        _check(lib().sllm_page_seq_extend(self.handle, seq, rows, C.c_void_p(stream)))
+
+    def truncate(self, seq: int, rows: int) -> None:
+        _check(lib().sllm_page_seq_truncate(self.handle, seq, rows))
+
+    def free(self, seqs: list) -> None:
+        _check(lib().sllm_page_seq_free(self.handle, _ints(seqs), len(seqs)))
+
+    def length(self, seq: int) -> int:
+        n = C.c_int()
+        _check(lib().sllm_page_seq_length(self.handle, seq, C.byref(n)))
+        return n.value
+
+    def tables(self, seqs: list) -> np.ndarray:
+        """The sequences' page numbers, one row each, -1 behind a table's end."""
+        ids, most = _ints(seqs), C.c_int()
+        _check(lib().sllm_page_seq_tables(self.handle, ids, len(seqs), None, 0, C.byref(most)))
+        out = np.empty((len(seqs), most.value), np.int32)
+        if out.size:
+            _check(lib().sllm_page_seq_tables(self.handle, ids, len(seqs), out.ctypes.data_as(C.POINTER(C.c_int)),
+                                              most.value, None))
+        return out
+
+    def compact(self, stream: int = 0) -> int:
+        """Held pages to the lowest numbers; returns how many there are."""
+        n = C.c_int()
+        _check(lib().sllm_page_cache_compact(self.handle, C.byref(n), C.c_void_p(stream)))
+        return n.value
+
+
+class PageBatch:
+    """The steps of a batch of a page cache's sequences (sllm_page_batch)."""
+
+    def __init__(self, cache: PageCache, n_heads: int, max_seqs: int, max_rows: int):
+        self.handle = None
+        h = C.c_void_p()
+        _check(lib().sllm_page_batch_create(cache.handle, n_heads, max_seqs, max_rows, C.byref(h)))
+        self.handle, self.cache = h, cache
+        self.n_heads, self.max_seqs, self.max_rows = n_heads, max_seqs, max_rows
+
+    def close(self) -> None:
+        if self.handle:
+            lib().sllm_page_batch_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def begin(self, seqs: list, rows: list, stream: int = 0) -> None:
+        """A step: rows[i] more rows for sequence seqs[i]."""
+        if len(seqs) != len(rows):
+            raise SllmError(1, "seqs and rows differ in length")
+        _check(lib().sllm_page_batch_begin(self.handle, _ints(seqs), _ints(rows), len(seqs), C.c_void_p(stream)))
+
+
+def page_attention_dev(batch: PageBatch, layer: int, params: AttnParams, q_ptr: int, k_ptr: int, v_ptr: int,
+                       out_ptr: int, stream: int = 0) -> None:
+    """The attention section of one layer for the batch's step: as attention_dev, for the new rows of every
+    sequence, one sequence after the other."""
+    _check(lib().sllm_page_attention_dev(batch.handle, layer, C.byref(params), C.c_void_p(q_ptr), C.c_void_p(k_ptr),
+                                         C.c_void_p(v_ptr), C.c_void_p(out_ptr), C.c_void_p(stream)))
+
+
+class LoraSet:
+    """Low-rank adapters of one projection, in device memory (sllm_lora_set)."""
+
+    def __init__(self, rows: int, cols: int, max_adapters: int, max_rank: int, dtype: str = "f16"):
+        self.handle = None
+        if dtype not in LORA_TYPES:
+            raise SllmError(1, f"unknown adapter type {dtype}")
+        h = C.c_void_p()
+        _check(lib().sllm_lora_set_create(rows, cols, max_adapters, max_rank, LORA_TYPES[dtype], C.byref(h)))
+        self.handle = h
+        self.rows, self.cols, self.max_adapters, self.max_rank, self.dtype = rows, cols, max_adapters, max_rank, dtype
+
+    def close(self) -> None:
+        if self.handle:
+            lib().sllm_lora_set_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def load(self, slot: int, a, b, scale: float = 1.0) -> None:
+        """Adapter `slot`: a (rank x cols), b (rows x rank), numpy arrays (bf16: uint16) or CPU tensors of the set's
+        type. None, None empties the slot."""
+        if a is None and b is None:
+            _check(lib().sllm_lora_set_load(self.handle, slot, 0, None, None, 0.0))
+            return
+        ptrs, keep = [], []
+        for m in (a, b):
+            if hasattr(m, "data_ptr"):
+                if m.device.type != "cpu" or str(m.dtype) != "torch." + {"f32": "float32", "f16": "float16",
+                                                                         "bf16": "bfloat16"}[self.dtype]:
+                    raise SllmError(1, f"adapter matrices must be CPU tensors of type {self.dtype}")
+                m = m.contiguous()
+                ptrs.append(m.data_ptr())
+            else:
+                if m.dtype != {"f32": np.float32, "f16": np.float16, "bf16": np.uint16}[self.dtype]:
+                    raise SllmError(1, f"adapter matrices must be arrays of type {self.dtype}")
+                m = np.ascontiguousarray(m)
+                ptrs.append(m.ctypes.data)
+            keep.append(m)
+        rank = keep[0].shape[0]
+        if tuple(keep[0].shape) != (rank, self.cols) or tuple(keep[1].shape) != (self.rows, rank):
+            raise SllmError(1, "adapter matrices must be rank x cols and rows x rank")
+        _check(lib().sllm_lora_set_load(self.handle, slot, rank, C.c_void_p(ptrs[0]), C.c_void_p(ptrs[1]), scale))
+
+
+def lora_add_dev(adapters: LoraSet, x_ptr: int, x_rows: int, ids_ptr: int, y_ptr: int, dst_ptr: int,
+                 stream: int = 0) -> None:
+    """dst[r] = y[r] + scale B (A x[r]) with the adapter ids[r] (device int32; -1: none) of each row."""
+    _check(lib().sllm_lora_add_dev(adapters.handle, C.c_void_p(x_ptr), x_rows, C.c_void_p(ids_ptr), C.c_void_p(y_ptr),
+                                   C.c_void_p(dst_ptr), C.c_void_p(stream)))
 
 
 def argmax_f32_dev(v_ptr: int, n: int, stream: int = 0) -> int:
