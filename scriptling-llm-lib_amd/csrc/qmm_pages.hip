@@ -143,6 +143,114 @@ void end_seq(PageCache &c, int s) {
     c.spare.insert(std::lower_bound(c.spare.begin(), c.spare.end(), s, [](int a, int b) { return a > b; }), s);
 }
 
+// ---- a step's segments and pieces ----
+
+struct Segment {
+    int first;           // the sequence (of the step) whose table it reads
+    int p0, p1;          // positions
+    int tok0, ntok;
+    int shape = 0, block = 0;  // rows of a block (shape), query rows of a block
+    int slot = 0, pieces = 1, piece = 0;
+    bool causal = false, lone = false;  // lone: its rows have no other segment
+};
+
+struct Plan {
+    std::vector<Segment> segs;
+    std::vector<int> tok;
+    std::vector<std::vector<std::pair<int, int>>> parts;  // per sequence: (segment, number of its first row in it)
+};
+
+// Positions that sharing has to save each further sequence for a segment of its own: below,
+// reading them once more costs less than another state to merge.
+constexpr int kWorthSharing = 128;
+
+// Sequences `who` (of the step) have page p in common for p < from (their segments up to there
+// are made); what follows is cut into segments: a run of pages that several hold once for all of these, and so
+// on behind it, at most kMaxParts to a sequence.
+void share(const PageCache &c, const int *seqs, const int *rows, const std::vector<int> &row0, std::vector<int> who, int from,
+           int depth, Plan *plan) {
+    auto table = [&](int i) -> const std::vector<int> & { return c.seqs[(size_t)seqs[i]].pages; };
+    // full pages before the sequence's first new row: every new row sees all of them
+    auto full = [&](int i) { return (c.seqs[(size_t)seqs[i]].len - rows[i]) >> c.shift; };
+    auto own = [&](int i) {
+        Segment s;
+        s.first = i;
+        s.p0 = from << c.shift;
+        s.p1 = c.seqs[(size_t)seqs[i]].len;
+        s.tok0 = (int)plan->tok.size();
+        s.ntok = rows[i];
+        s.causal = rows[i] > 1;
+        s.lone = plan->parts[(size_t)i].empty();
+        for (int r = 0; r < rows[i]; r++) plan->tok.push_back(row0[(size_t)i] + r);
+        plan->parts[(size_t)i].push_back({(int)plan->segs.size(), 0});
+        plan->segs.push_back(s);
+    };
+    // by the next page; those without a further full page are on their own
+    auto key = [&](int i) { return full(i) > from ? table(i)[(size_t)from] : -1; };
+    std::stable_sort(who.begin(), who.end(), [&](int x, int y) { return key(x) < key(y); });
+    for (size_t i = 0; i < who.size();) {
+        size_t j = i + 1;
+        while (j < who.size() && key(who[j]) == key(who[i])) j++;
+        int to = from;
+        if (key(who[i]) >= 0 && j - i > 1 && depth + 1 < kMaxParts)
+            for (bool same = true; same; to += same) {
+                for (size_t k = i; same && k < j; k++)
+                    same = full(who[k]) > to && table(who[k])[(size_t)to] == table(who[i])[(size_t)to];
+            }
+        if (((to - from) << c.shift) < kWorthSharing) {
+            for (; i < j; i++) own(who[i]);
+            continue;
+        }
+        Segment s;
+        s.first = who[i];
+        s.p0 = from << c.shift;
+        s.p1 = to << c.shift;
+        s.tok0 = (int)plan->tok.size();
+        std::vector<int> group(who.begin() + (long)i, who.begin() + (long)j);
+        for (int k : group) {
+            plan->parts[(size_t)k].push_back({(int)plan->segs.size(), (int)plan->tok.size() - s.tok0});
+            for (int r = 0; r < rows[k]; r++) plan->tok.push_back(row0[(size_t)k] + r);
+        }
+        s.ntok = (int)plan->tok.size() - s.tok0;
+        plan->segs.push_back(s);
+        share(c, seqs, rows, row0, std::move(group), to, depth + 1, plan);
+        i = j;
+    }
+}
+
+constexpr int kPieceTile = 32;     // positions: pieces are multiples of it
+constexpr int kTargetPieces = 512; // workgroups that a step is cut into, about
+constexpr int kLeastTiles = 4;     // of a piece: one for every wave
+
+constexpr int kSpareStates = 8192; // of a kv head, beyond what a step's rows need in one piece each
+
+// The segments' blocks and pieces: every piece about as many tiles as a share of all the step's,
+// and no more states than the batch has room for. Returns the number of pieces (for one kv head).
+int cut(Plan *plan, int rep, int n_kv, int slots) {
+    int64_t all = 0;
+    for (Segment &s : plan->segs) {
+        const int64_t nv = (int64_t)s.ntok * rep;
+        s.shape = nv <= kShapeRows[0] ? 0 : nv <= kShapeRows[1] ? 1 : 2;
+        s.block = kShapeRows[s.shape] / rep;
+        all += (int64_t)((s.ntok + s.block - 1) / s.block) * ((s.p1 - s.p0 + kPieceTile - 1) / kPieceTile);
+    }
+    int64_t tiles = std::max<int64_t>(kLeastTiles, (all * n_kv + kTargetPieces - 1) / kTargetPieces);
+    for (;; tiles *= 2) {
+        int64_t used = 0, items = 0;
+        for (Segment &s : plan->segs) {
+            const int64_t n = (s.p1 - s.p0 + kPieceTile - 1) / kPieceTile;
+            s.pieces = (int)((n + tiles - 1) / tiles);
+            s.piece = (int)((n + s.pieces - 1) / s.pieces) * kPieceTile;
+            s.pieces = (s.p1 - s.p0 + s.piece - 1) / s.piece;
+            s.slot = (int)used;
+            if (!(s.lone && s.pieces == 1)) used += (int64_t)s.pieces * s.ntok * rep;
+            items += (int64_t)s.pieces * ((s.ntok + s.block - 1) / s.block);
+        }
+        // (with one piece each they fit: kMaxParts states for every row)
+        if (used <= slots) return (int)items;
+    }
+}
+
 }  // namespace
 
 PageCache::~PageCache() {
@@ -176,7 +284,8 @@ PageBatch::~PageBatch() {
     }
     if (dev) (void)hipFree(dev);
     for (void *p : retired) (void)hipFree(p);
-    if (qrot) (void)hipFree(qrot);
+    for (float *p : {qrot, part, ml})
+        if (p) (void)hipFree(p);
 }
 
 sllm_status launch_page_copies(const PageCache &c, const PageCopy *jobs, size_t n, hipStream_t s) {
@@ -472,8 +581,12 @@ sllm_status sllm_page_batch_create(sllm_page_cache *pc, int n_heads, int max_seq
         b->b.max_rows = max_rows;
         b->b.seqs.reserve((size_t)max_seqs);
         b->b.versions.reserve((size_t)max_seqs);
-        if (hipMalloc(&b->b.qrot, (size_t)max_rows * n_heads * c.d_k * sizeof(float)) != hipSuccess) {
-            b->b.qrot = nullptr;
+        const int rep = n_heads / c.n_kv;
+        b->b.slots = (kMaxParts + 1) * max_rows * rep + kSpareStates;
+        const size_t states = (size_t)b->b.slots * c.n_kv;
+        if (hipMalloc(&b->b.qrot, (size_t)max_rows * n_heads * c.d_k * sizeof(float)) != hipSuccess ||
+            hipMalloc(&b->b.part, states * c.d_k * sizeof(float)) != hipSuccess ||
+            hipMalloc(&b->b.ml, states * 2 * sizeof(float)) != hipSuccess) {
             (void)hipGetLastError();
             return set_error(SLLM_ERR_OOM, "page batch allocation failed");
         }
@@ -508,13 +621,28 @@ sllm_status sllm_page_batch_begin(sllm_page_batch *batch, const int *seqs, const
         sllm_status st = on_device(c.device);
         if (st != SLLM_OK) return st;
         if (stream_capturing(s)) return set_error(SLLM_ERR_ARG, "a batch's step cannot begin under capture");
-        // room for the step on the device and in the next staging slot
-        const size_t bytes = (size_t)(kStepHeader + 4 * (int64_t)b.max_rows + pages) * sizeof(int);
+        std::vector<PageCopy> copies;
+        Plan plan;
+        plan.parts.resize((size_t)count);
+        plan.tok.reserve((size_t)total * kMaxParts);
+        std::vector<int> row0((size_t)count), who;
+        int r0 = 0;
+        for (int i = 0; i < count; i++) {
+            row0[(size_t)i] = r0;
+            r0 += rows[i];
+            if (rows[i]) who.push_back(i);
+        }
+        // room for the step on the device and in the next staging slot: header, rows, parts, segments, rows of
+        // segments, pieces, tables
+        const int64_t most_segs = 2 * (int64_t)count, rep = b.n_heads / c.n_kv;
+        const int64_t most_items = most_segs + kMaxParts * total + 2 * kTargetPieces;
+        const size_t bytes = (size_t)(kStepHeader + total * (4 + 3 * kMaxParts) + 8 * most_segs + 8 * most_items + pages + 32) *
+                             sizeof(int);
         if (b.dev_cap < bytes) {
             if (b.captured)
                 return set_error(SLLM_ERR_SHAPE, "the step has more pages than the batch held when it was captured");
             void *p = nullptr;
-            const size_t want = 2 * bytes + 4096;
+            const size_t want = 2 * bytes + 65536;
             if (hipMalloc(&p, want) != hipSuccess) {
                 (void)hipGetLastError();
                 return set_error(SLLM_ERR_OOM, "page batch allocation failed");
@@ -535,30 +663,76 @@ sllm_status sllm_page_batch_begin(sllm_page_batch *batch, const int *seqs, const
             }
             b.host_cap[slot] = b.dev_cap;
         }
-        std::vector<PageCopy> copies;
         if ((st = append(c, seqs, rows, count, &copies)) != SLLM_OK) return st;
+        share(c, seqs, rows, row0, std::move(who), 0, 0, &plan);
+        const int n_items = cut(&plan, (int)rep, c.n_kv, b.slots);
         int *h = (int *)b.host[slot];
-        std::memset(h, 0, kStepHeader * sizeof(int));
-        h[0] = (int)total;
-        StepRow *hr = (StepRow *)(h + kStepHeader);
-        int *ht = h + kStepHeader + 4 * (size_t)b.max_rows;
-        int at = 0;
+        int at = kStepHeader;
+        auto place = [&](int64_t ints) {
+            const int was = at;
+            at += (int)((ints + 3) & ~(int64_t)3);
+            return was;
+        };
+        h[kStepRows] = (int)total;
+        h[kStepItems] = n_items;
+        h[kStepRowsAt] = place(4 * total);
+        h[kStepPartsAt] = place(2 * kMaxParts * total);
+        h[kStepSegsAt] = place(8 * (int64_t)plan.segs.size());
+        h[kStepTokAt] = place((int64_t)plan.tok.size());
+        h[kStepItemsAt] = place(8 * (int64_t)n_items);
+        std::vector<int> table((size_t)count, -1);  // of the sequences that segments read
+        StepRow *hr = (StepRow *)(h + h[kStepRowsAt]);
+        int *hp = h + h[kStepPartsAt], parts = 0;
         for (int i = 0; i < count; i++) {
             const PageSeq &q = c.seqs[(size_t)seqs[i]];
+            const auto &mine = plan.parts[(size_t)i];
             for (int r = 0; r < rows[i]; r++) {
                 const int pos = q.len - rows[i] + r;
-                *hr++ = {q.pages[(size_t)(pos >> c.shift)], pos & (c.page_rows - 1), pos, at};
+                *hr++ = {q.pages[(size_t)(pos >> c.shift)], pos & (c.page_rows - 1), pos, 4 * parts + (int)mine.size()};
+                for (const auto &m : mine) {
+                    hp[2 * parts] = m.first;
+                    hp[2 * parts++ + 1] = m.second + r;
+                }
             }
-            std::copy(q.pages.begin(), q.pages.end(), ht + at);
-            at += (int)q.pages.size();
         }
+        StepSeg *hs = (StepSeg *)(h + h[kStepSegsAt]);
+        StepItem *hi = (StepItem *)(h + h[kStepItemsAt]);
+        std::copy(plan.tok.begin(), plan.tok.end(), h + h[kStepTokAt]);
+        b.combine = false;
+        for (const Segment &s : plan.segs) {
+            *hs++ = {s.slot, s.ntok, s.pieces, s.piece, s.p0, {0, 0, 0}};
+            int &t = table[(size_t)s.first];
+            if (t < 0) {
+                const std::vector<int> &pg = c.seqs[(size_t)seqs[s.first]].pages;
+                t = at;
+                at += (int)pg.size();
+                std::copy(pg.begin(), pg.end(), h + t);
+            }
+            const bool direct = s.lone && s.pieces == 1;
+            b.combine |= !direct;
+            for (int i = 0; i < s.pieces; i++)
+                for (int k = 0; k < s.ntok; k += s.block) {
+                    StepItem x;
+                    x.table = t;
+                    x.p0 = s.p0 + i * s.piece;
+                    x.p1 = std::min(s.p1, x.p0 + s.piece);
+                    x.tok = s.tok0 + k;
+                    x.ntok = std::min(s.block, s.ntok - k);
+                    x.slot = s.slot + (i * s.ntok + k) * (int)rep;
+                    // a sequence's own rows: row k of n sees n - 1 - k positions less than the last
+                    x.lim0 = s.causal ? std::min(x.p1, s.p1 - (s.ntok - 1 - k)) : x.p1;
+                    x.flags = s.shape | (s.causal ? kItemCausal : 0) | (direct ? kItemDirect : 0);
+                    *hi++ = x;
+                }
+        }
+        b.items = n_items;
         b.seqs.assign(seqs, seqs + count);
         b.versions.resize((size_t)count);
         for (int i = 0; i < count; i++) b.versions[(size_t)i] = c.seqs[(size_t)seqs[i]].version;
         b.rows = (int)total;
         b.begun = true;
         if ((st = launch_page_copies(c, copies.data(), copies.size(), s)) != SLLM_OK) return st;
-        SLLM_HIP(hipMemcpyAsync(b.dev, h, bytes, hipMemcpyHostToDevice, s));
+        SLLM_HIP(hipMemcpyAsync(b.dev, h, (size_t)at * sizeof(int), hipMemcpyHostToDevice, s));
         SLLM_HIP(hipEventRecord(b.done[slot], s));
         b.slot = (slot + 1) % PageBatch::kSlots;
         return SLLM_OK;
@@ -615,15 +789,19 @@ sllm_status sllm_page_attention_dev(sllm_page_batch *batch, int layer, const sll
     a.eps = p->norm_eps;
     a.freqs = p->rope_freqs;
     a.half_dim = p->rope_half_dim;
-    a.scale = 1.0f / (float)__builtin_sqrt((double)c.d_k);
+    a.scale_log2 = (float)(1.4426950408889634 / __builtin_sqrt((double)c.d_k));
     const size_t loff = (size_t)layer * c.n_pages * c.n_kv * c.page_rows * c.d_k * c.elem();
     a.pool_k = c.k + loff;
     a.pool_v = c.v + loff;
     a.step = b.dev;
-    a.rows = (const StepRow *)(b.dev + kStepHeader);
-    a.tables = b.dev + kStepHeader + 4 * (size_t)b.max_rows;
     a.qrot = b.qrot;
+    a.part = b.part;
+    a.ml = b.ml;
+    a.slots = b.slots;
+    // a captured launch serves later steps of the batch too
     a.grid_rows = capture ? b.max_rows : b.rows;
+    a.grid_items = capture ? 2 * kTargetPieces : b.items * c.n_kv;
+    a.combine = capture || b.combine;
     a.type = c.type;
     b.captured |= capture;
     return launch_page_attention(a, s);

@@ -41,20 +41,46 @@ struct PageCache {
 
     ~PageCache();
     int elem() const { return type == SLLM_CACHE_F16 ? 2 : 4; }
-    // pages that appending `rows` rows to sequence s takes; `gone`: holders that tail pages
-    // lose to copies made before in the same call
     bool live(int s) const { return s >= 0 && s < (int)seqs.size() && seqs[(size_t)s].live; }
     int take();           // the lowest vacant page (n_vacant > 0), held once
     void drop(int page);  // one holder less
 };
 
-// What the kernels read of a step, in device memory at addresses that stay
-// for the batch's life, so that captured launches follow later steps.
+// What the kernels read of a step: one buffer at an address that stays (captured launches
+// follow later steps), a header of counts and offsets (in ints) first.
+enum {
+    kStepRows = 0,     // query rows
+    kStepItems = 1,    // pieces
+    kStepRowsAt = 2,   // StepRow of every query row
+    kStepPartsAt = 3,  // the rows' segments: (segment, the row's number in it)
+    kStepSegsAt = 4,   // StepSeg
+    kStepTokAt = 5,    // the segments' query rows
+    kStepItemsAt = 6,  // StepItem
+    kStepHeader = 8
+};
 struct StepRow {
     int page, slot;  // where the row's K and V go
     int pos;         // its position
-    int table;       // its sequence's page ids, at tables[table]
+    int parts;       // its segments: first index * 4 + their number
 };
+// A run of positions and the query rows that attend to it: the pages that several sequences share, or
+// what one sequence has behind those. Its states: [piece][query row][q head of the kv head].
+struct StepSeg {
+    int slot, ntok, pieces, piece;  // first state; query rows; pieces and their length
+    int p0, pad[3];                 // first position
+};
+// A piece of a segment for a block of its query rows.
+struct StepItem {
+    int table;     // page ids of the positions from 0 on (offset)
+    int p0, p1;    // positions
+    int tok, ntok; // the block's query rows
+    int slot;      // state of its first row
+    int lim0;      // positions from here on are not seen by every row
+    int flags;
+};
+enum { kItemShape = 3, kItemCausal = 4, kItemDirect = 8 };  // shape: rows of 16, 32 or 128 to a block
+constexpr int kShapeRows[3] = {16, 32, 128};
+constexpr int kMaxParts = 3;  // segments of a row at most
 
 struct PageBatch {
     std::shared_ptr<PageCache> c;
@@ -67,6 +93,10 @@ struct PageBatch {
     size_t dev_cap = 0;              // bytes
     std::vector<void *> retired;
     float *qrot = nullptr;           // max_rows x n_heads x d_k
+    float *part = nullptr, *ml = nullptr;  // the pieces' states, slots for every kv head
+    int slots = 0;
+    int items = 0;
+    bool combine = false;            // some row has several pieces
     // staging of a step on the host: a slot is written again when its upload is done
     static constexpr int kSlots = 4;
     char *host[kSlots] = {};
@@ -89,16 +119,15 @@ struct PageAttnArgs {
     float eps;
     const float *freqs;
     int half_dim;
-    float scale;
+    float scale_log2;       // log2(e) / sqrt(d_k)
     char *pool_k, *pool_v;  // this layer
-    const int *step;        // header: [0] rows
-    const StepRow *rows;
-    const int *tables;
-    float *qrot;
-    int grid_rows;          // rows launched (the step's, or max_rows under capture)
+    const int *step;
+    float *qrot, *part, *ml;
+    int slots;
+    int grid_rows, grid_items;  // the step's, or under capture what later ones may have
+    bool combine;
     int type;
 };
-constexpr int kStepHeader = 16;  // ints
 
 sllm_status launch_page_copies(const PageCache &c, const PageCopy *jobs, size_t n, hipStream_t s);
 sllm_status launch_page_attention(const PageAttnArgs &a, hipStream_t s);

@@ -590,7 +590,7 @@ def test_refused_steps_change_nothing():
             assert e.value.status == 1
         sq.page_attention_dev(batch, 0, m.params, p, p, p, p, st.cuda_stream)
     with pytest.raises(sq.SllmError) as e:  # the captured call's buffers stay as they are
-        big = sq.PageCache(1, 2, 64, 16, 5000, "f32")
+        big = sq.PageCache(1, 2, 64, 16, 60000, "f32")
         bb = sq.PageBatch(big, 4, 2, 64)
         s = big.add()
         bb.begin([s], [1])
@@ -598,7 +598,7 @@ def test_refused_steps_change_nothing():
         torch.cuda.synchronize()
         with torch.cuda.graph(g2, stream=st):
             sq.page_attention_dev(bb, 0, m.params, p, p, p, p, st.cuda_stream)
-        big.extend(s, 16 * 4900)
+        big.extend(s, 16 * 59000)
         bb.begin([s], [1])
     assert e.value.status == 3
     torch.cuda.synchronize()
