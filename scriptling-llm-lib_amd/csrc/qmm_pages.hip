@@ -632,11 +632,11 @@ sllm_status sllm_page_batch_begin(sllm_page_batch *batch, const int *seqs, const
             r0 += rows[i];
             if (rows[i]) who.push_back(i);
         }
-        // room for the step on the device and in the next staging slot: header, rows, parts, segments, rows of
-        // segments, pieces, tables
+        // room for the step on the device and in the next staging slot: header, rows, rows of segments,
+        // pieces, tables
         const int64_t most_segs = 2 * (int64_t)count, rep = b.n_heads / c.n_kv;
         const int64_t most_items = most_segs + kMaxParts * total + 2 * kTargetPieces;
-        const size_t bytes = (size_t)(kStepHeader + total * (4 + 3 * kMaxParts) + 8 * most_segs + 8 * most_items + pages + 32) *
+        const size_t bytes = (size_t)(kStepHeader + total * (int64_t)(sizeof(StepRow) / 4 + kMaxParts) + 8 * most_items + pages + 32) *
                              sizeof(int);
         if (b.dev_cap < bytes) {
             if (b.captured)
@@ -675,32 +675,32 @@ sllm_status sllm_page_batch_begin(sllm_page_batch *batch, const int *seqs, const
         };
         h[kStepRows] = (int)total;
         h[kStepItems] = n_items;
-        h[kStepRowsAt] = place(4 * total);
-        h[kStepPartsAt] = place(2 * kMaxParts * total);
-        h[kStepSegsAt] = place(8 * (int64_t)plan.segs.size());
+        h[kStepRowsAt] = place((int64_t)(sizeof(StepRow) / 4) * total);
         h[kStepTokAt] = place((int64_t)plan.tok.size());
         h[kStepItemsAt] = place(8 * (int64_t)n_items);
         std::vector<int> table((size_t)count, -1);  // of the sequences that segments read
         StepRow *hr = (StepRow *)(h + h[kStepRowsAt]);
-        int *hp = h + h[kStepPartsAt], parts = 0;
+        b.combine = 0;
         for (int i = 0; i < count; i++) {
             const PageSeq &q = c.seqs[(size_t)seqs[i]];
             const auto &mine = plan.parts[(size_t)i];
+            int pieces = 0;
+            for (const auto &m : mine) pieces += plan.segs[(size_t)m.first].pieces;
+            if (pieces > 1) b.combine = std::max(b.combine, pieces);
             for (int r = 0; r < rows[i]; r++) {
                 const int pos = q.len - rows[i] + r;
-                *hr++ = {q.pages[(size_t)(pos >> c.shift)], pos & (c.page_rows - 1), pos, 4 * parts + (int)mine.size()};
-                for (const auto &m : mine) {
-                    hp[2 * parts] = m.first;
-                    hp[2 * parts++ + 1] = m.second + r;
+                StepRow x = {q.pages[(size_t)(pos >> c.shift)], pos & (c.page_rows - 1), pos, pieces == 1, {}};
+                for (size_t k = 0; k < mine.size(); k++) {
+                    const Segment &s = plan.segs[(size_t)mine[k].first];
+                    x.parts[k] = {s.slot + (mine[k].second + r) * (int)rep, s.ntok * (int)rep,
+                                  std::min(s.pieces, (pos - s.p0) / s.piece + 1), 0};
                 }
+                *hr++ = x;
             }
         }
-        StepSeg *hs = (StepSeg *)(h + h[kStepSegsAt]);
         StepItem *hi = (StepItem *)(h + h[kStepItemsAt]);
         std::copy(plan.tok.begin(), plan.tok.end(), h + h[kStepTokAt]);
-        b.combine = false;
         for (const Segment &s : plan.segs) {
-            *hs++ = {s.slot, s.ntok, s.pieces, s.piece, s.p0, {0, 0, 0}};
             int &t = table[(size_t)s.first];
             if (t < 0) {
                 const std::vector<int> &pg = c.seqs[(size_t)seqs[s.first]].pages;
@@ -709,7 +709,6 @@ sllm_status sllm_page_batch_begin(sllm_page_batch *batch, const int *seqs, const
                 std::copy(pg.begin(), pg.end(), h + t);
             }
             const bool direct = s.lone && s.pieces == 1;
-            b.combine |= !direct;
             for (int i = 0; i < s.pieces; i++)
                 for (int k = 0; k < s.ntok; k += s.block) {
                     StepItem x;
@@ -801,7 +800,7 @@ sllm_status sllm_page_attention_dev(sllm_page_batch *batch, int layer, const sll
     // a captured launch serves later steps of the batch too
     a.grid_rows = capture ? b.max_rows : b.rows;
     a.grid_items = capture ? 2 * kTargetPieces : b.items * c.n_kv;
-    a.combine = capture || b.combine;
+    a.combine = capture ? INT32_MAX : b.combine;
     a.type = c.type;
     b.captured |= capture;
     return launch_page_attention(a, s);

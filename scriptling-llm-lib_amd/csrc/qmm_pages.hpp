@@ -52,22 +52,21 @@ enum {
     kStepRows = 0,     // query rows
     kStepItems = 1,    // pieces
     kStepRowsAt = 2,   // StepRow of every query row
-    kStepPartsAt = 3,  // the rows' segments: (segment, the row's number in it)
-    kStepSegsAt = 4,   // StepSeg
-    kStepTokAt = 5,    // the segments' query rows
-    kStepItemsAt = 6,  // StepItem
+    kStepTokAt = 3,    // the segments' query rows
+    kStepItemsAt = 4,  // StepItem
     kStepHeader = 8
 };
+// The states of one query row in a segment: of the first piece and q head of the kv head, and the
+// distance to those of the next piece; how many pieces the row sees.
+struct StepPart {
+    int first, step, pieces, pad;
+};
+constexpr int kMaxParts = 3;  // segments of a row at most
 struct StepRow {
     int page, slot;  // where the row's K and V go
     int pos;         // its position
-    int parts;       // its segments: first index * 4 + their number
-};
-// A run of positions and the query rows that attend to it: the pages that several sequences share, or
-// what one sequence has behind those. Its states: [piece][query row][q head of the kv head].
-struct StepSeg {
-    int slot, ntok, pieces, piece;  // first state; query rows; pieces and their length
-    int p0, pad[3];                 // first position
+    int direct;      // its one piece writes the output itself
+    StepPart parts[kMaxParts];  // (pieces 0 behind the last)
 };
 // A piece of a segment for a block of its query rows.
 struct StepItem {
@@ -80,7 +79,6 @@ struct StepItem {
 };
 enum { kItemShape = 3, kItemCausal = 4, kItemDirect = 8 };  // shape: rows of 16, 32 or 128 to a block
 constexpr int kShapeRows[3] = {16, 32, 128};
-constexpr int kMaxParts = 3;  // segments of a row at most
 
 struct PageBatch {
     std::shared_ptr<PageCache> c;
@@ -96,7 +94,7 @@ struct PageBatch {
     float *part = nullptr, *ml = nullptr;  // the pieces' states, slots for every kv head
     int slots = 0;
     int items = 0;
-    bool combine = false;            // some row has several pieces
+    int combine = 0;                 // most pieces that a row's states are merged of (0: none has several)
     // staging of a step on the host: a slot is written again when its upload is done
     static constexpr int kSlots = 4;
     char *host[kSlots] = {};
@@ -125,7 +123,7 @@ struct PageAttnArgs {
     float *qrot, *part, *ml;
     int slots;
     int grid_rows, grid_items;  // the step's, or under capture what later ones may have
-    bool combine;
+    int combine;                // most pieces of a row, 0 where none has several
     int type;
 };
 

@@ -16,6 +16,7 @@ namespace sllm {
 namespace {
 
 constexpr int kMaxDk = 256;
+typedef float v2f __attribute__((ext_vector_type(2)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef _Float16 v4h __attribute__((ext_vector_type(4)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
@@ -32,16 +33,27 @@ __device__ __forceinline__ void put4(_Float16 *dst, v4f x) {
 // Bias (model_f32.go:398-420), per-head RMSNorm (:424-435), RoPE (applyRopeInPlaceF32,
 // float32_ops.go:174-188) of every q and k head of a row, and the row's k and v into its page
 // (the append, model_f32.go:445-448), rounded to the cache's type, once.
-// One workgroup per row: the rotation (the same for every head: float32 angle, sine and cosine in 64
-// bits, as the reference) once in LDS; then a wave per head, four dimensions a lane.
-constexpr int kPrepWaves = 8;
-template <class T>
-__global__ void __launch_bounds__(64 * kPrepWaves) page_prep_kernel(PageAttnArgs a) {
+// A workgroup takes heads of one row, LP lanes of four dimensions to a head; the rotation (the same for
+// every head: float32 angle, sine and cosine in 64 bits, as the reference) is formed once in LDS, the first
+// heads' elements loaded before it. Bound by latency: few rows have a workgroup for every 256 / LP heads.
+// (16 rows of 32 + 8 heads of 128, us: one workgroup of eight waves per row, a wave per head 8.2; this 2.7.)
+constexpr int kPrepThreads = 256;
+template <class T, int LP>
+__global__ void __launch_bounds__(kPrepThreads) page_prep_kernel(PageAttnArgs a) {
     __shared__ float rc[kMaxDk / 2], rs[kMaxDk / 2];
-    const int r = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    constexpr int HG = kPrepThreads / LP;
+    const int r = blockIdx.x, sub = threadIdx.x % LP;
     if (r >= a.step[kStepRows]) return;
-    const StepRow row = ((const StepRow *)(a.step + a.step[kStepRowsAt]))[r];
-    const int dk = a.d_k, d = 4 * lane;
+    const StepRow &row = ((const StepRow *)(a.step + a.step[kStepRowsAt]))[r];
+    const int dk = a.d_k, d = 4 * sub, page_rows = 1 << a.shift;
+    auto at_of = [&](int t) {
+        return t < a.n_heads ? ((size_t)r * a.n_heads + t) * dk + d : ((size_t)r * a.n_kv + t - a.n_heads) * dk + d;
+    };
+    auto load = [&](int t) {
+        return t < a.n_heads + a.n_kv && d < dk ? *(const v4f *)((t < a.n_heads ? a.q : a.k) + at_of(t)) : v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    };
+    int t = blockIdx.y * HG + threadIdx.x / LP;
+    v4f x = load(t);
     if ((int)threadIdx.x < a.half_dim) {
         const float ang = a.freqs[threadIdx.x] * (float)row.pos;
         double sd, cd;
@@ -50,24 +62,20 @@ __global__ void __launch_bounds__(64 * kPrepWaves) page_prep_kernel(PageAttnArgs
         rs[threadIdx.x] = (float)sd;
     }
     __syncthreads();
-    const int page_rows = 1 << a.shift;
-    for (int t = wave; t < a.n_heads + a.n_kv; t += kPrepWaves) {
+    for (; t < a.n_heads + a.n_kv; t += gridDim.y * HG, x = load(t)) {
         const bool isq = t < a.n_heads;
         const int h = isq ? t : t - a.n_heads;
-        const int cols = (isq ? a.n_heads : a.n_kv) * dk;
-        const size_t off = (size_t)r * cols + (size_t)h * dk + d;
+        const size_t off = at_of(t);
         const float *bias = isq ? a.q_bias : a.k_bias, *nw = isq ? a.q_norm : a.k_norm;
         const int blen = isq ? a.qb_len : a.kb_len, j0 = h * dk + d;
-        v4f x = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (d < dk) {
-            x = *(const v4f *)((isq ? a.q : a.k) + off);
-            if (bias)
+        if (bias && d < dk)
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-                    if (j0 + i < blen) x[i] = x[i] + bias[j0 + i];
-        }
+            for (int i = 0; i < 4; i++)
+                if (j0 + i < blen) x[i] = x[i] + bias[j0 + i];
         if (nw) {
-            const float ss = wave_sum(((x[0] * x[0] + x[1] * x[1]) + x[2] * x[2]) + x[3] * x[3]);
+            float ss = ((x[0] * x[0] + x[1] * x[1]) + x[2] * x[2]) + x[3] * x[3];
+#pragma unroll
+            for (int o = LP / 2; o > 0; o >>= 1) ss = ss + __shfl_xor(ss, o, LP);
             const float inv = 1.0f / (float)sqrt((double)ss / (double)dk + (double)a.eps);
             if (d < dk)
 #pragma unroll
@@ -75,7 +83,7 @@ __global__ void __launch_bounds__(64 * kPrepWaves) page_prep_kernel(PageAttnArgs
         }
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-            const int f = 2 * lane + i;
+            const int f = 2 * sub + i;
             if (f < a.half_dim) {
                 const float c = rc[f], s = rs[f], x0 = x[2 * i], x1 = x[2 * i + 1];
                 x[2 * i] = x0 * c - x1 * s;
@@ -117,6 +125,7 @@ __global__ void __launch_bounds__(64 * kPrepWaves) page_prep_kernel(PageAttnArgs
 // A result that is not finite (a non-finite K or V element, also one that only other rows of the block
 // see, where the matrix instruction forms 0 * inf) is computed again, row by row, as the formula says.
 constexpr int kWaves = 4;
+constexpr int kFewPieces = 8;    // of a row, up to which one group of lanes merges them
 constexpr float kGrow = 8.0f;  // log2 of how far weights may exceed 1
 
 template <class T>
@@ -130,10 +139,15 @@ struct Kind<_Float16> {
     static constexpr int kTile = 32;
 };
 
+// What is the same for a wave is read through the scalar cache (the step was written before the kernel began):
+// a vector load of a page number would have to wait for the K and V loads before it.
+typedef const int __attribute__((address_space(4))) *ScalarInts;
+
 struct Piece {
     StepItem it;
     int g, rep, dk;
-    const int *table, *tok;
+    ScalarInts table;
+    const int *tok;
     const StepRow *rows;
     // row v of the block: its query row, and how many positions it sees
     __device__ __forceinline__ int row_of(int v) const { return tok[it.tok + v / rep]; }
@@ -268,16 +282,22 @@ __device__ __forceinline__ void run_piece(const PageAttnArgs &a, const Piece &p,
     const int endh = (p1 - 1) & ~15;  // the last half tile with positions
     v4u kr[H][KS];
     VT vr[VE][VB];
-    // positions behind the piece's end read its last one; their weights are 0
-    auto head = [&](const char *pool, int hb) {
-        const int page = p.table[hb >> a.shift];
+    // positions behind the piece's end read its last one; their weights are 0. Page numbers are read a step
+    // before the rows that they place.
+    auto half = [&](int t, int h) { return min(p0 + t * TP + 16 * h, endh); };
+    int pg[H], pgn[H];  // pages of this step's and of the next one's halves
+    auto pages = [&](int t, int *to) {
+#pragma unroll
+        for (int h = 0; h < H; h++) to[h] = p.table[half(t, h) >> a.shift];
+    };
+    auto head = [&](const char *pool, int page, int hb) {
         return (const T *)pool + (((size_t)page * a.n_kv + p.g) * page_rows + (hb & (page_rows - 1))) * dk;
     };
-    auto load_k = [&](int t) {
+    auto load_k = [&](int t, const int *page) {
 #pragma unroll
         for (int h = 0; h < H; h++) {
-            const int hb = min(p0 + t * TP + 16 * h, endh);
-            const T *b = head(a.pool_k, hb) + min(col, p1 - 1 - hb) * dk + (F16 ? 8 : 4) * qd;
+            const int hb = half(t, h);
+            const T *b = head(a.pool_k, page[h], hb) + min(col, p1 - 1 - hb) * dk + (F16 ? 8 : 4) * qd;
 #pragma unroll
             for (int j = 0; j < KS; j++)
                 kr[h][j] = FULL || KD * j + (F16 ? 8 : 4) * qd < dk ? *(const v4u *)(b + KD * j) : v4u{0, 0, 0, 0};
@@ -286,8 +306,8 @@ __device__ __forceinline__ void run_piece(const PageAttnArgs &a, const Piece &p,
     auto load_v = [&](int t) {
 #pragma unroll
         for (int h = 0; h < H; h++) {
-            const int hb = min(p0 + t * TP + 16 * h, endh);
-            const T *b = head(a.pool_v, hb) + VW * col;
+            const int hb = half(t, h);
+            const T *b = head(a.pool_v, pg[h], hb) + VW * col;
 #pragma unroll
             for (int i = 0; i < 4; i++)
 #pragma unroll
@@ -301,7 +321,9 @@ __device__ __forceinline__ void run_piece(const PageAttnArgs &a, const Piece &p,
                 }
         }
     };
-    if (t0 < tiles) load_k(t0);
+    pages(t0, pg);
+    pages(t0 + dt, pgn);
+    if (t0 < tiles) load_k(t0, pg);
     for (int t = t0; t < tiles; t += dt) {
         load_v(t);
         v4f s[MT][H];
@@ -326,7 +348,10 @@ __device__ __forceinline__ void run_piece(const PageAttnArgs &a, const Piece &p,
                             s[mt][h] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[c], qf[mt][j][c], s[mt][h], 0, 0, 0);
                     }
                 }
-        if (t + dt < tiles) load_k(t + dt);
+        if (t + dt < tiles) load_k(t + dt, pgn);
+#pragma unroll
+        for (int h = 0; h < H; h++) pg[h] = pgn[h];
+        pages(t + 2 * dt, pgn);
         const int tp = p0 + t * TP;
         const bool masked = tp + TP > p.it.lim0;  // some row does not see all of the tile
 #pragma unroll
@@ -490,18 +515,20 @@ template <class T, int NB, bool FULL>
 __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(NB <= 2 ? 2 : 1)))
 page_attn_kernel(PageAttnArgs a) {
     extern __shared__ __attribute__((aligned(16))) float lds[];
-    const int n = a.step[kStepItems] * a.n_kv;
+    const ScalarInts step = (ScalarInts)(uintptr_t)a.step;
+    const int n = step[kStepItems] * a.n_kv;
     Piece p;
     p.rep = a.rep;
     p.dk = a.d_k;
-    p.rows = (const StepRow *)(a.step + a.step[kStepRowsAt]);
-    p.tok = a.step + a.step[kStepTokAt];
-    const StepItem *items = (const StepItem *)(a.step + a.step[kStepItemsAt]);
+    p.rows = (const StepRow *)(a.step + step[kStepRowsAt]);
+    p.tok = a.step + step[kStepTokAt];
+    const ScalarInts items = step + step[kStepItemsAt];
     for (int w = blockIdx.x; w < n; w += gridDim.x) {
         const int i = w / a.n_kv;
         p.g = w - i * a.n_kv;
-        p.it = items[i];
-        p.table = a.step + p.it.table;
+        const ScalarInts it = items + 8 * i;
+        p.it = {it[0], it[1], it[2], it[3], it[4], it[5], it[6], it[7]};
+        p.table = (ScalarInts)(uintptr_t)(a.step + p.it.table);
         switch (p.it.flags & kItemShape) {
         case 0: run_piece<T, NB, FULL, 1, 1>(a, p, lds); break;
         case 1: run_piece<T, NB, FULL, 2, 1>(a, p, lds); break;
@@ -510,35 +537,72 @@ page_attn_kernel(PageAttnArgs a) {
     }
 }
 
-// The states of one (row, q head), LP lanes of four dimensions, in the order of the row's segments and their
-// pieces; rows with one piece are written already.
-template <int LP>
+// The states of one (row, q head), merged by G groups of LP lanes of four dimensions, a group every G-th piece,
+// the groups' in LDS. Rows with one piece are written already. Bound by latency: one group takes
+// few pieces, eight long lists, four pieces' states in flight.
+template <int LP, int G>
 __global__ void __launch_bounds__(256) page_combine_kernel(PageAttnArgs a) {
-    const int x = blockIdx.x * (256 / LP) + threadIdx.x / LP, d = threadIdx.x % LP * 4;
+    constexpr int P = 256 / (LP * G);  // pairs per workgroup
+    constexpr int U = 4;
+    __shared__ v4f os[G > 1 ? 256 : 1];
+    __shared__ v2f ss[G > 1 ? G : 1];
+    const int sub = threadIdx.x % LP, grp = threadIdx.x / LP % G, d = sub * 4;
+    const int x = blockIdx.x * P + threadIdx.x / (LP * G);
     const int r = x / a.n_heads, h = x - r * a.n_heads;
+    // (G > 1: all of a workgroup's threads have the same pair)
     if (r >= a.step[kStepRows]) return;
     const StepRow row = ((const StepRow *)(a.step + a.step[kStepRowsAt]))[r];
-    const StepSeg *segs = (const StepSeg *)(a.step + a.step[kStepSegsAt]);
-    const int2 *parts = (const int2 *)(a.step + a.step[kStepPartsAt]) + (row.parts >> 2);
-    const int n = row.parts & 3, g = h / a.rep, j = h - g * a.rep;
-    if (n == 1 && segs[parts[0].x].pieces == 1) return;
-    const size_t base = (size_t)g * a.slots;
+    if (row.direct) return;
+    const int g = h / a.rep, j = h - g * a.rep;
+    const size_t base = (size_t)g * a.slots + j;
+    const int n0 = row.parts[0].pieces, n1 = n0 + row.parts[1].pieces, all = n1 + row.parts[2].pieces;
     const int dc = d < a.d_k ? d : 0;
     float M = -INFINITY, L = 0.0f;
     v4f O = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int i = 0; i < n; i++) {
-        const StepSeg s = segs[parts[i].x];
-        const int c1 = min(s.pieces, (row.pos - s.p0) / s.piece + 1);  // pieces that the row sees
-        const int step = s.ntok * a.rep;
-        size_t at = base + s.slot + parts[i].y * a.rep + j;
-        for (int c = 0; c < c1; c++, at += step) {
-            const float mc = a.ml[2 * at], lc = a.ml[2 * at + 1];
-            const v4f o = *(const v4f *)(a.part + at * a.d_k + dc);
-            const float mn = fmaxf(M, mc);
-            const float f = M == -INFINITY ? 0.0f : exp2_(M - mn), fc = mc == -INFINITY ? 0.0f : exp2_(mc - mn);
-            L = L * f + lc * fc;
-            O = O * f + o * fc;
-            M = mn;
+    for (int c0 = grp; c0 < all; c0 += U * G) {
+        v2f s[U];
+        v4f o[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int c = min(c0 + u * G, all - 1);
+            const int at = c < n0   ? row.parts[0].first + c * row.parts[0].step
+                           : c < n1 ? row.parts[1].first + (c - n0) * row.parts[1].step
+                                    : row.parts[2].first + (c - n1) * row.parts[2].step;
+            s[u] = *(const v2f *)(a.ml + (base + at) * 2);
+            o[u] = *(const v4f *)(a.part + (base + at) * a.d_k + dc);
+        }
+        float mn = M;
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (c0 + u * G < all) mn = fmaxf(mn, s[u][0]);
+        const float f = M == -INFINITY ? 0.0f : exp2_(M - mn);
+        L = L * f;
+        O = O * f;
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (c0 + u * G < all) {
+                const float w = s[u][0] == -INFINITY ? 0.0f : exp2_(s[u][0] - mn);
+                L = L + s[u][1] * w;
+                O = O + o[u] * w;
+            }
+        M = mn;
+    }
+    if constexpr (G > 1) {
+        os[threadIdx.x] = O;
+        if (sub == 0) ss[grp] = v2f{M, L};
+        __syncthreads();
+        if (grp) return;
+        float mn = M;
+#pragma unroll
+        for (int u = 1; u < G; u++) mn = fmaxf(mn, ss[u][0]);
+        const float f = M == -INFINITY ? 0.0f : exp2_(M - mn);
+        L = L * f;
+        O = O * f;
+#pragma unroll
+        for (int u = 1; u < G; u++) {
+            const float w = ss[u][0] == -INFINITY ? 0.0f : exp2_(ss[u][0] - mn);
+            L = L + ss[u][1] * w;
+            O = O + os[threadIdx.x + u * LP] * w;
         }
     }
     if (d < a.d_k) *(v4f *)(a.out + ((size_t)r * a.n_heads + h) * a.d_k + d) = O * (1.0f / L);
@@ -551,9 +615,12 @@ void launch_attn(const PageAttnArgs &a, hipStream_t s) {
     else hipLaunchKernelGGL((page_attn_kernel<T, NB, false>), dim3(a.grid_items), dim3(64 * kWaves), lds, s, a);
 }
 
-template <class T>
+template <class T, int LP>
 sllm_status launch(const PageAttnArgs &a, hipStream_t s) {
-    hipLaunchKernelGGL(page_prep_kernel<T>, dim3(a.grid_rows), dim3(64 * kPrepWaves), 0, s, a);
+    constexpr int hg = kPrepThreads / LP, groups = 256 / LP;
+    const int most = (a.n_heads + a.n_kv + hg - 1) / hg, want = 2048 / a.grid_rows;
+    const int y = want < 1 ? 1 : want < most ? want : most;
+    hipLaunchKernelGGL((page_prep_kernel<T, LP>), dim3(a.grid_rows, y), dim3(kPrepThreads), 0, s, a);
     SLLM_HIP(hipGetLastError());
     switch ((a.d_k + 63) / 64) {
     case 1: launch_attn<T, 1>(a, s); break;
@@ -564,8 +631,10 @@ sllm_status launch(const PageAttnArgs &a, hipStream_t s) {
     SLLM_HIP(hipGetLastError());
     if (!a.combine) return SLLM_OK;
     const int pairs = a.grid_rows * a.n_heads;
-    if (a.d_k <= 128) hipLaunchKernelGGL(page_combine_kernel<32>, dim3((pairs + 7) / 8), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL(page_combine_kernel<64>, dim3((pairs + 3) / 4), dim3(256), 0, s, a);
+    if (a.combine > kFewPieces)
+        hipLaunchKernelGGL((page_combine_kernel<LP, groups>), dim3(pairs), dim3(256), 0, s, a);
+    else
+        hipLaunchKernelGGL((page_combine_kernel<LP, 1>), dim3((pairs + groups - 1) / groups), dim3(256), 0, s, a);
     SLLM_HIP(hipGetLastError());
     return SLLM_OK;
 }
@@ -573,7 +642,8 @@ sllm_status launch(const PageAttnArgs &a, hipStream_t s) {
 }  // namespace
 
 sllm_status launch_page_attention(const PageAttnArgs &a, hipStream_t s) {
-    return a.type == SLLM_CACHE_F16 ? launch<_Float16>(a, s) : launch<float>(a, s);
+    if (a.type == SLLM_CACHE_F16) return a.d_k <= 128 ? launch<_Float16, 32>(a, s) : launch<_Float16, 64>(a, s);
+    return a.d_k <= 128 ? launch<float, 32>(a, s) : launch<float, 64>(a, s);
 }
 
 }  // namespace sllm
