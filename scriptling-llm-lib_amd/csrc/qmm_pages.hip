@@ -636,7 +636,7 @@ sllm_status sllm_page_batch_begin(sllm_page_batch *batch, const int *seqs, const
         // pieces, tables
         const int64_t most_segs = 2 * (int64_t)count, rep = b.n_heads / c.n_kv;
         const int64_t most_items = most_segs + kMaxParts * total + 2 * kTargetPieces;
-        const size_t bytes = (size_t)(kStepHeader + total * (int64_t)(sizeof(StepRow) / 4 + kMaxParts) + 8 * most_items + pages + 32) *
+        const size_t bytes = (size_t)(kStepHeader + total * (int64_t)(sizeof(StepRow) / 4 + kMaxParts) + 16 * most_items + pages + 32) *
                              sizeof(int);
         if (b.dev_cap < bytes) {
             if (b.captured)
@@ -675,9 +675,9 @@ sllm_status sllm_page_batch_begin(sllm_page_batch *batch, const int *seqs, const
         };
         h[kStepRows] = (int)total;
         h[kStepItems] = n_items;
+        StepItem *hi = (StepItem *)(h + place(16 * (int64_t)n_items));
+        const int tok_at = place((int64_t)plan.tok.size());
         h[kStepRowsAt] = place((int64_t)(sizeof(StepRow) / 4) * total);
-        h[kStepTokAt] = place((int64_t)plan.tok.size());
-        h[kStepItemsAt] = place(8 * (int64_t)n_items);
         std::vector<int> table((size_t)count, -1);  // of the sequences that segments read
         StepRow *hr = (StepRow *)(h + h[kStepRowsAt]);
         b.combine = 0;
@@ -698,8 +698,7 @@ sllm_status sllm_page_batch_begin(sllm_page_batch *batch, const int *seqs, const
                 *hr++ = x;
             }
         }
-        StepItem *hi = (StepItem *)(h + h[kStepItemsAt]);
-        std::copy(plan.tok.begin(), plan.tok.end(), h + h[kStepTokAt]);
+        std::copy(plan.tok.begin(), plan.tok.end(), h + tok_at);
         for (const Segment &s : plan.segs) {
             int &t = table[(size_t)s.first];
             if (t < 0) {
@@ -715,12 +714,20 @@ sllm_status sllm_page_batch_begin(sllm_page_batch *batch, const int *seqs, const
                     x.table = t;
                     x.p0 = s.p0 + i * s.piece;
                     x.p1 = std::min(s.p1, x.p0 + s.piece);
-                    x.tok = s.tok0 + k;
                     x.ntok = std::min(s.block, s.ntok - k);
+                    const int *tk = plan.tok.data() + s.tok0 + k;
+                    bool run = true;
+                    for (int u = 1; u < x.ntok; u++) run &= tk[u] == tk[0] + u;
+                    x.tok = run ? tk[0] : tok_at + s.tok0 + k;
                     x.slot = s.slot + (i * s.ntok + k) * (int)rep;
                     // a sequence's own rows: row k of n sees n - 1 - k positions less than the last
                     x.lim0 = s.causal ? std::min(x.p1, s.p1 - (s.ntok - 1 - k)) : x.p1;
-                    x.flags = s.shape | (s.causal ? kItemCausal : 0) | (direct ? kItemDirect : 0);
+                    x.flags = s.shape | (s.causal ? kItemCausal : 0) | (direct ? kItemDirect : 0) | (run ? kItemRun : 0);
+                    const std::vector<int> &pg = c.seqs[(size_t)seqs[s.first]].pages;
+                    for (int u = 0; u < 8; u++) {
+                        const size_t at_page = (size_t)(x.p0 >> c.shift) + (size_t)u;
+                        x.pages[u] = at_page < pg.size() ? pg[at_page] : 0;
+                    }
                     *hi++ = x;
                 }
         }
@@ -799,6 +806,7 @@ sllm_status sllm_page_attention_dev(sllm_page_batch *batch, int layer, const sll
     a.slots = b.slots;
     // a captured launch serves later steps of the batch too
     a.grid_rows = capture ? b.max_rows : b.rows;
+    a.items = capture ? -1 : b.items * c.n_kv;
     a.grid_items = capture ? 2 * kTargetPieces : b.items * c.n_kv;
     a.combine = capture ? INT32_MAX : b.combine;
     a.type = c.type;

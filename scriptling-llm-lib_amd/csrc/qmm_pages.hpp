@@ -51,10 +51,8 @@ struct PageCache {
 enum {
     kStepRows = 0,     // query rows
     kStepItems = 1,    // pieces
-    kStepRowsAt = 2,   // StepRow of every query row
-    kStepTokAt = 3,    // the segments' query rows
-    kStepItemsAt = 4,  // StepItem
-    kStepHeader = 8
+    kStepRowsAt = 2,   // StepRow of every query row (offset in ints)
+    kStepHeader = 16   // then the pieces (StepItem), query rows of segments, StepRows, tables
 };
 // The states of one query row in a segment: of the first piece and q head of the kv head, and the
 // distance to those of the next piece; how many pieces the row sees.
@@ -72,12 +70,13 @@ struct StepRow {
 struct StepItem {
     int table;     // page ids of the positions from 0 on (offset)
     int p0, p1;    // positions
-    int tok, ntok; // the block's query rows
+    int tok, ntok; // the block's query rows: from tok on (kItemRun), or a list there (offset)
     int slot;      // state of its first row
     int lim0;      // positions from here on are not seen by every row
     int flags;
+    int pages[8];  // the first page ids from p0 on: enough for every wave's first rows
 };
-enum { kItemShape = 3, kItemCausal = 4, kItemDirect = 8 };  // shape: rows of 16, 32 or 128 to a block
+enum { kItemShape = 3, kItemCausal = 4, kItemDirect = 8, kItemRun = 16 };  // shape: rows of 16, 32 or 128 to a block
 constexpr int kShapeRows[3] = {16, 32, 128};
 
 struct PageBatch {
@@ -122,6 +121,7 @@ struct PageAttnArgs {
     const int *step;
     float *qrot, *part, *ml;
     int slots;
+    int items;                  // pieces over all kv heads; -1: as the step says
     int grid_rows, grid_items;  // the step's, or under capture what later ones may have
     int combine;                // most pieces of a row, 0 where none has several
     int type;

@@ -146,17 +146,20 @@ typedef const int __attribute__((address_space(4))) *ScalarInts;
 struct Piece {
     StepItem it;
     int g, rep, dk;
-    ScalarInts table;
-    const int *tok;
+    ScalarInts table, first;  // the sequence's page ids; the first ones of the piece
+    const int *step;
     const StepRow *rows;
-    // row v of the block: its query row, and how many positions it sees
-    __device__ __forceinline__ int row_of(int v) const { return tok[it.tok + v / rep]; }
+    // the query row of row v of the block
+    __device__ __forceinline__ int row_of(int v) const {
+        const int t = v / rep;
+        return it.flags & kItemRun ? it.tok + t : step[it.tok + t];
+    }
 };
 
 // Row v's result: the output (direct) or the piece's state.
 __device__ __forceinline__ size_t out_at(const PageAttnArgs &a, const Piece &p, int v) {
-    const int t = v / p.rep, j = v - t * p.rep;
-    return p.it.flags & kItemDirect ? ((size_t)p.tok[p.it.tok + t] * a.n_heads + p.g * p.rep + j) * p.dk
+    const int j = v % p.rep;
+    return p.it.flags & kItemDirect ? ((size_t)p.row_of(v) * a.n_heads + p.g * p.rep + j) * p.dk
                                     : ((size_t)p.g * a.slots + p.it.slot + v) * p.dk;
 }
 __device__ __forceinline__ void put_state(const PageAttnArgs &a, const Piece &p, int v, float m, float l) {
@@ -224,6 +227,56 @@ __device__ __forceinline__ void run_piece(const PageAttnArgs &a, const Piece &p,
     const int page_rows = 1 << a.shift;
     if (v0 >= nv) return;  // (the first wave's rows exist)
 
+    const int tiles = (p1 - p0 + TP - 1) / TP;
+    constexpr int dt = RW == kWaves ? 1 : kWaves;
+    const int t0 = RW == kWaves ? 0 : wave;
+    const int endh = (p1 - 1) & ~15;  // the last half tile with positions
+    v4u kr[H][KS];
+    VT vr[VE][VB];
+    // positions behind the piece's end read its last one; their weights are 0. Page numbers are read a step
+    // before the rows that they place.
+    auto half = [&](int t, int h) { return min(p0 + t * TP + 16 * h, endh); };
+    int pg[H], pgn[H];  // pages of this step's and of the next one's halves
+    auto pages = [&](int t, int *to) {
+#pragma unroll
+        for (int h = 0; h < H; h++) to[h] = p.table[half(t, h) >> a.shift];
+    };
+    auto head = [&](const char *pool, int page, int hb) {
+        return (const T *)pool + (((size_t)page * a.n_kv + p.g) * page_rows + (hb & (page_rows - 1))) * dk;
+    };
+    auto load_k = [&](int t, const int *page) {
+#pragma unroll
+        for (int h = 0; h < H; h++) {
+            const int hb = half(t, h);
+            const T *b = head(a.pool_k, page[h], hb) + min(col, p1 - 1 - hb) * dk + (F16 ? 8 : 4) * qd;
+#pragma unroll
+            for (int j = 0; j < KS; j++)
+                kr[h][j] = FULL || KD * j + (F16 ? 8 : 4) * qd < dk ? *(const v4u *)(b + KD * j) : v4u{0, 0, 0, 0};
+        }
+    };
+    auto load_v = [&](int t) {
+#pragma unroll
+        for (int h = 0; h < H; h++) {
+            const int hb = half(t, h);
+            const T *b = head(a.pool_v, pg[h], hb) + VW * col;
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int u = 0; u < VB; u++) {
+                    VT z;
+#pragma unroll
+                    for (int c = 0; c < VW; c++) z[c] = (T)0.0f;
+                    vr[4 * h + i][u] = FULL || 16 * VW * u + VW * col < dk
+                                           ? *(const VT *)(b + min(4 * qd + i, p1 - 1 - hb) * dk + 16 * VW * u)
+                                           : z;
+                }
+        }
+    };
+    // the first half tiles' pages came with the item (the scalar cache's line of it)
+#pragma unroll
+    for (int h = 0; h < H; h++) pg[h] = p.first[(half(t0, h) >> a.shift) - (p0 >> a.shift)];
+    load_k(t0, pg);
+    pages(t0 + dt, pgn);
     v4f qf[F16 ? 1 : MT][F16 ? 1 : KS];
     v8h qh[F16 ? MT : 1][F16 ? KS : 1], ql[F16 ? MT : 1][F16 ? KS : 1];
     float sc[MT], m[MT], l[MT];
@@ -276,54 +329,6 @@ __device__ __forceinline__ void run_piece(const PageAttnArgs &a, const Piece &p,
         for (int t = 0; t < NT; t++) o[mt][t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
-    const int tiles = (p1 - p0 + TP - 1) / TP;
-    constexpr int dt = RW == kWaves ? 1 : kWaves;
-    const int t0 = RW == kWaves ? 0 : wave;
-    const int endh = (p1 - 1) & ~15;  // the last half tile with positions
-    v4u kr[H][KS];
-    VT vr[VE][VB];
-    // positions behind the piece's end read its last one; their weights are 0. Page numbers are read a step
-    // before the rows that they place.
-    auto half = [&](int t, int h) { return min(p0 + t * TP + 16 * h, endh); };
-    int pg[H], pgn[H];  // pages of this step's and of the next one's halves
-    auto pages = [&](int t, int *to) {
-#pragma unroll
-        for (int h = 0; h < H; h++) to[h] = p.table[half(t, h) >> a.shift];
-    };
-    auto head = [&](const char *pool, int page, int hb) {
-        return (const T *)pool + (((size_t)page * a.n_kv + p.g) * page_rows + (hb & (page_rows - 1))) * dk;
-    };
-    auto load_k = [&](int t, const int *page) {
-#pragma unroll
-        for (int h = 0; h < H; h++) {
-            const int hb = half(t, h);
-            const T *b = head(a.pool_k, page[h], hb) + min(col, p1 - 1 - hb) * dk + (F16 ? 8 : 4) * qd;
-#pragma unroll
-            for (int j = 0; j < KS; j++)
-                kr[h][j] = FULL || KD * j + (F16 ? 8 : 4) * qd < dk ? *(const v4u *)(b + KD * j) : v4u{0, 0, 0, 0};
-        }
-    };
-    auto load_v = [&](int t) {
-#pragma unroll
-        for (int h = 0; h < H; h++) {
-            const int hb = half(t, h);
-            const T *b = head(a.pool_v, pg[h], hb) + VW * col;
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int u = 0; u < VB; u++) {
-                    VT z;
-#pragma unroll
-                    for (int c = 0; c < VW; c++) z[c] = (T)0.0f;
-                    vr[4 * h + i][u] = FULL || 16 * VW * u + VW * col < dk
-                                           ? *(const VT *)(b + min(4 * qd + i, p1 - 1 - hb) * dk + 16 * VW * u)
-                                           : z;
-                }
-        }
-    };
-    pages(t0, pg);
-    pages(t0 + dt, pgn);
-    if (t0 < tiles) load_k(t0, pg);
     for (int t = t0; t < tiles; t += dt) {
         load_v(t);
         v4f s[MT][H];
@@ -348,7 +353,8 @@ __device__ __forceinline__ void run_piece(const PageAttnArgs &a, const Piece &p,
                             s[mt][h] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[c], qf[mt][j][c], s[mt][h], 0, 0, 0);
                     }
                 }
-        if (t + dt < tiles) load_k(t + dt, pgn);
+        // (the last step's is of the last rows again: a branch here would make the waits for V wait for it too)
+        load_k(t + dt, pgn);
 #pragma unroll
         for (int h = 0; h < H; h++) pg[h] = pgn[h];
         pages(t + 2 * dt, pgn);
@@ -515,19 +521,20 @@ template <class T, int NB, bool FULL>
 __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(NB <= 2 ? 2 : 1)))
 page_attn_kernel(PageAttnArgs a) {
     extern __shared__ __attribute__((aligned(16))) float lds[];
+    // one read of memory (a piece's item) before the first K rows are on their way
     const ScalarInts step = (ScalarInts)(uintptr_t)a.step;
-    const int n = step[kStepItems] * a.n_kv;
+    const int n = a.items >= 0 ? a.items : step[kStepItems] * a.n_kv;
     Piece p;
     p.rep = a.rep;
     p.dk = a.d_k;
+    p.step = a.step;
     p.rows = (const StepRow *)(a.step + step[kStepRowsAt]);
-    p.tok = a.step + step[kStepTokAt];
-    const ScalarInts items = step + step[kStepItemsAt];
     for (int w = blockIdx.x; w < n; w += gridDim.x) {
         const int i = w / a.n_kv;
         p.g = w - i * a.n_kv;
-        const ScalarInts it = items + 8 * i;
-        p.it = {it[0], it[1], it[2], it[3], it[4], it[5], it[6], it[7]};
+        const ScalarInts it = step + kStepHeader + 16 * i;
+        p.it = {it[0], it[1], it[2], it[3], it[4], it[5], it[6], it[7], {}};
+        p.first = it + 8;
         p.table = (ScalarInts)(uintptr_t)(a.step + p.it.table);
         switch (p.it.flags & kItemShape) {
         case 0: run_piece<T, NB, FULL, 1, 1>(a, p, lds); break;
