@@ -219,24 +219,28 @@ void share(const PageCache &c, const int *seqs, const int *rows, const std::vect
 }
 
 constexpr int kPieceTile = 32;     // positions: pieces are multiples of it
-constexpr int kTargetPieces = 512; // workgroups that a step is cut into, about
+constexpr int kTargetPieces = 512; // workgroups that run at a time (two per CU)
 constexpr int kLeastTiles = 4;     // of a piece: one for every wave
 
 constexpr int kSpareStates = 8192; // of a kv head, beyond what a step's rows need in one piece each
 
-// The segments' blocks and pieces: every piece about as many tiles as a share of all the step's,
-// and no more states than the batch has room for. Returns the number of pieces (for one kv head).
-int cut(Plan *plan, int rep, int n_kv, int slots) {
+// The segments' blocks and pieces: every piece about as many tiles as a share of all the step's, or a little more where
+// that lets all workgroups run at a time (16 ragged sequences, f32: 35.0 us with 560 workgroups, 32.4 with the fewer
+// ones; 5 prompts: 60.6, 56.2), and no more states than the batch has room for. Returns the number of pieces (for one
+// kv head).
+int cut(Plan *plan, int rep, int n_kv, const int *most, int slots) {
     int64_t all = 0;
     for (Segment &s : plan->segs) {
         const int64_t nv = (int64_t)s.ntok * rep;
-        s.shape = nv <= kShapeRows[0] ? 0 : nv <= kShapeRows[1] ? 1 : 2;
-        s.block = kShapeRows[s.shape] / rep;
+        s.shape = nv <= most[0] ? 0 : nv <= most[1] || !most[2] ? 1 : 2;
+        s.block = most[s.shape] / rep;
         all += (int64_t)((s.ntok + s.block - 1) / s.block) * ((s.p1 - s.p0 + kPieceTile - 1) / kPieceTile);
     }
-    int64_t tiles = std::max<int64_t>(kLeastTiles, (all * n_kv + kTargetPieces - 1) / kTargetPieces);
-    for (;; tiles *= 2) {
-        int64_t used = 0, items = 0;
+    // pieces of up to `tiles` tiles: how many, and their states
+    int64_t used = 0;
+    auto pieces = [&](int64_t tiles) {
+        int64_t items = 0;
+        used = 0;
         for (Segment &s : plan->segs) {
             const int64_t n = (s.p1 - s.p0 + kPieceTile - 1) / kPieceTile;
             s.pieces = (int)((n + tiles - 1) / tiles);
@@ -246,9 +250,16 @@ int cut(Plan *plan, int rep, int n_kv, int slots) {
             if (!(s.lone && s.pieces == 1)) used += (int64_t)s.pieces * s.ntok * rep;
             items += (int64_t)s.pieces * ((s.ntok + s.block - 1) / s.block);
         }
-        // (with one piece each they fit: kMaxParts states for every row)
-        if (used <= slots) return (int)items;
-    }
+        return items;
+    };
+    const int64_t share = std::max<int64_t>(kLeastTiles, (all * n_kv + kTargetPieces - 1) / kTargetPieces);
+    int64_t tiles = share;
+    while (tiles < 2 * share && pieces(tiles) * n_kv > kTargetPieces) tiles++;
+    int64_t items = pieces(tiles);
+    if (items * n_kv > kTargetPieces) items = pieces(tiles = share);
+    // (with one piece each the states fit: kMaxParts for every row)
+    while (used > slots) items = pieces(tiles *= 2);
+    return (int)items;
 }
 
 }  // namespace
@@ -570,7 +581,9 @@ sllm_status sllm_page_batch_create(sllm_page_cache *pc, int n_heads, int max_seq
     const PageCache &c = *pc->c;
     if (n_heads <= 0 || n_heads % c.n_kv != 0 || n_heads / c.n_kv > 8)
         return set_error(SLLM_ERR_SHAPE, "n_heads must be a multiple of n_kv_heads, at most 8 times it");
-    if ((int64_t)max_rows * n_heads > (1 << 26)) return set_error(SLLM_ERR_SHAPE, "max_rows x n_heads must stay below 2^26");
+    // the kernels address a row's q, output and states with 32 bits
+    if ((int64_t)max_rows * n_heads * c.d_k > (1 << 28))
+        return set_error(SLLM_ERR_SHAPE, "max_rows x n_heads x d_k must be at most 2^28");
     return guarded([&]() -> sllm_status {
         sllm_status st = on_device(c.device);
         if (st != SLLM_OK) return st;
@@ -584,7 +597,7 @@ sllm_status sllm_page_batch_create(sllm_page_cache *pc, int n_heads, int max_seq
         const int rep = n_heads / c.n_kv;
         b->b.slots = (kMaxParts + 1) * max_rows * rep + kSpareStates;
         const size_t states = (size_t)b->b.slots * c.n_kv;
-        if (hipMalloc(&b->b.qrot, (size_t)max_rows * n_heads * c.d_k * sizeof(float)) != hipSuccess ||
+        if (hipMalloc(&b->b.qrot, (size_t)max_rows * n_heads * (c.d_k + 1) * sizeof(float)) != hipSuccess ||
             hipMalloc(&b->b.part, states * c.d_k * sizeof(float)) != hipSuccess ||
             hipMalloc(&b->b.ml, states * 2 * sizeof(float)) != hipSuccess) {
             (void)hipGetLastError();
@@ -665,7 +678,7 @@ sllm_status sllm_page_batch_begin(sllm_page_batch *batch, const int *seqs, const
         }
         if ((st = append(c, seqs, rows, count, &copies)) != SLLM_OK) return st;
         share(c, seqs, rows, row0, std::move(who), 0, 0, &plan);
-        const int n_items = cut(&plan, (int)rep, c.n_kv, b.slots);
+        const int n_items = cut(&plan, (int)rep, c.n_kv, kShapeRows[shape_class(c.d_k, c.type == SLLM_CACHE_F16)], b.slots);
         int *h = (int *)b.host[slot];
         int at = kStepHeader;
         auto place = [&](int64_t ints) {
@@ -732,6 +745,8 @@ sllm_status sllm_page_batch_begin(sllm_page_batch *batch, const int *seqs, const
                 }
         }
         b.items = n_items;
+        b.wide = false;
+        for (const Segment &s : plan.segs) b.wide |= s.shape == 0 && s.ntok * rep > 16;
         b.seqs.assign(seqs, seqs + count);
         b.versions.resize((size_t)count);
         for (int i = 0; i < count; i++) b.versions[(size_t)i] = c.seqs[(size_t)seqs[i]].version;
@@ -801,11 +816,13 @@ sllm_status sllm_page_attention_dev(sllm_page_batch *batch, int layer, const sll
     a.pool_v = c.v + loff;
     a.step = b.dev;
     a.qrot = b.qrot;
+    a.qscale = b.qrot + (size_t)b.max_rows * b.n_heads * c.d_k;
     a.part = b.part;
     a.ml = b.ml;
     a.slots = b.slots;
     // a captured launch serves later steps of the batch too
     a.grid_rows = capture ? b.max_rows : b.rows;
+    a.wide = capture || b.wide;
     a.items = capture ? -1 : b.items * c.n_kv;
     a.grid_items = capture ? 2 * kTargetPieces : b.items * c.n_kv;
     a.combine = capture ? INT32_MAX : b.combine;

@@ -76,8 +76,13 @@ struct StepItem {
     int flags;
     int pages[8];  // the first page ids from p0 on: enough for every wave's first rows
 };
-enum { kItemShape = 3, kItemCausal = 4, kItemDirect = 8, kItemRun = 16 };  // shape: rows of 16, 32 or 128 to a block
-constexpr int kShapeRows[3] = {16, 32, 128};
+enum { kItemShape = 3, kItemCausal = 4, kItemDirect = 8, kItemRun = 16 };  // shape: kShapeRows
+// The rows of a block of each shape (0: not there), as far as a wave's registers go: rows that all waves take
+// together, 16 and 32 rows of each wave's own. By d_k: up to 128, the same with f16 runs that are not whole, up to 192, above.
+constexpr int kShapeRows[4][3] = {{32, 64, 128}, {16, 64, 128}, {16, 64, 0}, {0, 64, 0}};
+constexpr int shape_class(int d_k, bool f16) {
+    return d_k > 192 ? 3 : d_k > 128 ? 2 : f16 && d_k > 64 && d_k != 128 ? 1 : 0;
+}
 
 struct PageBatch {
     std::shared_ptr<PageCache> c;
@@ -89,10 +94,11 @@ struct PageBatch {
     int *dev = nullptr;              // the step: header, rows, tables (device)
     size_t dev_cap = 0;              // bytes
     std::vector<void *> retired;
-    float *qrot = nullptr;           // max_rows x n_heads x d_k
+    float *qrot = nullptr;           // max_rows x n_heads x d_k, then a scale for every head
     float *part = nullptr, *ml = nullptr;  // the pieces' states, slots for every kv head
     int slots = 0;
     int items = 0;
+    bool wide = false;               // some block of the first shape has more than 16 rows
     int combine = 0;                 // most pieces that a row's states are merged of (0: none has several)
     // staging of a step on the host: a slot is written again when its upload is done
     static constexpr int kSlots = 4;
@@ -119,8 +125,9 @@ struct PageAttnArgs {
     float scale_log2;       // log2(e) / sqrt(d_k)
     char *pool_k, *pool_v;  // this layer
     const int *step;
-    float *qrot, *part, *ml;
+    float *qrot, *qscale, *part, *ml;
     int slots;
+    bool wide;                  // blocks of the first shape may have more than 16 rows
     int items;                  // pieces over all kv heads; -1: as the step says
     int grid_rows, grid_items;  // the step's, or under capture what later ones may have
     int combine;                // most pieces of a row, 0 where none has several
