@@ -2,8 +2,8 @@
 //   dst[r] = y[r] + scale_a B_a (A_a x[r]),  a = ids[r]
 // for the rows of a batch, each with its own adapter or none.
 //
-// Rows of one adapter are worked on together: 64 rows' ids fit one wave, which splits them into units of up to 16 rows
-// with one adapter by ballots (no sort, no launch of its own, and rows in any order read each adapter once per unit).
+// Rows of one adapter are worked on together: 64 rows' ids fit one wave, which splits them into units of up to 16
+// (prompts: 64) rows with one adapter (no sort, no launch of its own; rows in any order read an adapter once per unit).
 // Two launches: `down` (t = A x, the columns split over workgroups and their waves) and `up` (adds the parts of t in
 // order, dst = y + scale B t). Products are float32 matrix instructions (16 ranks or outputs x 16 rows x 4), exact in
 // x for every type of adapter; a unit of a single row wastes 15 of their 16 columns and is bound by the loads all the
@@ -35,10 +35,12 @@ struct LoraArgs {
     const int *ids;
     const float *x, *y;
     float *t, *dst;  // t: parts of A x, [split][x_rows][stride]
-    int rows, cols, slots, max_rank, stride, x_rows, splits, chunks;
+    int *groups;     // of every 64 rows: how many groups of 16 with one adapter, then their records
+    int rows, cols, slots, max_rank, stride, x_rows, tiles, splits, chunks, most;
+    int steps, more;  // every wave's steps of columns; the first `more` waves' have one more
 };
 
-constexpr int kWaves = 4;
+constexpr int kWaves = 8;  // of a `down` workgroup
 constexpr int kStep = 32;  // columns of a load: 128 bytes of x for every row
 
 typedef float v4f __attribute__((ext_vector_type(4)));
@@ -56,21 +58,25 @@ __device__ __forceinline__ float bf16_at(uint32_t w, int j) {
 template <class T>
 struct Eight {
     v4f v[2];
-    __device__ __forceinline__ void load(const T *p) {
+    // lane / 16 = g4: its columns of a step (each instruction reads 64 bytes in a row)
+    static constexpr int kLane = 4, kSecond = 16;
+    __device__ __forceinline__ void load(const T *p, int second = kSecond) {
         v[0] = *(const v4f *)p;
-        v[1] = *(const v4f *)(p + 4);
+        v[1] = *(const v4f *)(p + second);
     }
     __device__ __forceinline__ float at(int j) const { return v[j >> 2][j & 3]; }
 };
 template <>
 struct Eight<_Float16> {
     v8h v;
+    static constexpr int kLane = 8, kSecond = 4;
     __device__ __forceinline__ void load(const _Float16 *p) { v = *(const v8h *)p; }
     __device__ __forceinline__ float at(int j) const { return (float)v[j]; }
 };
 template <>
 struct Eight<uint16_t> {  // bf16
     v4u v;
+    static constexpr int kLane = 8, kSecond = 4;
     __device__ __forceinline__ void load(const uint16_t *p) { v = *(const v4u *)p; }
     __device__ __forceinline__ float at(int j) const { return bf16_at(v[j >> 1], j); }
 };
@@ -85,86 +91,128 @@ __device__ __forceinline__ v4f four(const uint16_t *p) {
     return v4f{bf16_at(w[0], 0), bf16_at(w[0], 1), bf16_at(w[1], 0), bf16_at(w[1], 1)};
 }
 
-// Up to 16 rows with one adapter (rank 0: with none).
+// Up to 16 MT rows with one adapter (rank 0: with none).
+template <int MT>
 struct Unit {
-    int slot, rank, count, row;  // row: of lane % 16 (behind the count: the first one's)
+    int slot, rank, count, row[MT];  // row: of lane % 16 of a tile of 16 (behind the count: the first one's)
     float scale;
 };
 
-// The ids of 64 rows, a lane each, and their adapters.
+// The ids of 64 rows, a lane each, their adapters, and the units of up to 16 MT rows with one adapter: in the order of
+// their first rows, whatever the others are.
+template <int MT>
 struct Rows64 {
-    int id, rank;
+    int id, rank, nth;  // nth: of the rows with this id
     float scale;
-    uint64_t in;
+    uint64_t in, first, first16;  // rows; those that begin a unit, a group of 16 of a unit
 
-    __device__ __forceinline__ void load(const LoraArgs &g, int tile, int lane) {
-        const int64_t r = (int64_t)tile * 64 + lane;
-        in = __ballot(r < g.x_rows);
-        id = g.ids[min(r, (int64_t)g.x_rows - 1)];
+    __device__ __forceinline__ int load(const LoraArgs &g, int tile, int lane) {
+        const int count = min(64, g.x_rows - tile * 64);
+        in = count == 64 ? ~0ull : (1ull << count) - 1;
+        id = g.ids[(int64_t)tile * 64 + min(lane, count - 1)];
         const bool valid = id >= 0 && id < g.slots;
-        const Adapter ad = g.adapters[valid ? id : 0];
-        rank = valid ? ad.rank : 0;
-        scale = ad.scale;
+        if (g.slots <= 64) {  // all of them, under way beside the ids
+            const Adapter ad = g.adapters[min(lane, g.slots - 1)];
+            rank = __builtin_amdgcn_ds_bpermute(4 * (valid ? id : 0), ad.rank);
+            scale = __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute(4 * (valid ? id : 0), __builtin_bit_cast(int, ad.scale)));
+        } else {
+            const Adapter ad = g.adapters[valid ? id : 0];
+            rank = ad.rank;
+            scale = ad.scale;
+        }
+        if (!valid) rank = 0;
         if (rank == 0) id = -1;
+        nth = 0;
+        for (int j0 = 0; j0 < count; j0 += 8) {
+#pragma unroll
+            for (int j = j0; j < j0 + 8; j++) nth += __builtin_amdgcn_readlane(id, j) == id && j < lane ? 1 : 0;
+        }
+        first = __ballot(nth % (16 * MT) == 0) & in;
+        first16 = __ballot(nth % 16 == 0) & in;
+        return __builtin_popcountll(first);
     }
 
-    // The u-th unit (in the order of the adapters' first rows); false: there is none.
-    __device__ __forceinline__ bool unit(int tile, int lane, int u, Unit *out) const {
-        uint64_t left = in;
-        while (left) {
-            const int first = __builtin_ctzll(left);
-            out->slot = __builtin_amdgcn_readlane(id, first);
-            const uint64_t same = __ballot(id == out->slot) & in;
-            const int n = __builtin_popcountll(same);
-            if (u * 16 < n) {
-                const uint64_t below = (1ull << lane) - 1;
-                const int at = __builtin_popcountll(same & below);
-                const uint64_t mine = __ballot((same >> lane & 1) && at >> 4 == u);
-                out->count = __builtin_popcountll(mine);
-                out->rank = __builtin_amdgcn_readlane(rank, first);
-                out->scale = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, scale), first));
-                // every lane sends its number: the unit's to the front, in order
-                const int to = mine >> lane & 1 ? __builtin_popcountll(mine & below)
-                                                : out->count + __builtin_popcountll(~mine & below);
-                const int lanes = __builtin_amdgcn_ds_permute(4 * to, lane);
-                const int k = lane & 15;
-                out->row = tile * 64 + __builtin_amdgcn_ds_bpermute(4 * (k < out->count ? k : 0), lanes);
-                return true;
-            }
-            u -= (n + 15) / 16;
-            left &= ~same;
+    // the u-th
+    __device__ __forceinline__ void unit(int tile, int lane, int u, Unit<MT> *out) const {
+        const uint64_t below = (1ull << lane) - 1;
+        const int lead = __builtin_ctzll(__ballot((first >> lane & 1) && __builtin_popcountll(first & below) == u));
+        out->slot = __builtin_amdgcn_readlane(id, lead);
+        out->rank = __builtin_amdgcn_readlane(rank, lead);
+        out->scale = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, scale), lead));
+        const int group = __builtin_amdgcn_readlane(nth, lead) / (16 * MT);
+        const uint64_t mine = __ballot(id == out->slot && nth / (16 * MT) == group) & in;
+        out->count = __builtin_popcountll(mine);
+        // every lane sends its number: the unit's to the front, in order
+        const int to = mine >> lane & 1 ? __builtin_popcountll(mine & below)
+                                        : out->count + __builtin_popcountll(~mine & below);
+        const int lanes = __builtin_amdgcn_ds_permute(4 * to, lane);
+#pragma unroll
+        for (int m = 0; m < MT; m++) {
+            const int k = 16 * m + (lane & 15);
+            out->row[m] = tile * 64 + __builtin_amdgcn_ds_bpermute(4 * (k < out->count ? k : 0), lanes);
         }
-        return false;
     }
 };
+
+// What `up` needs to know of a group: ints [slot, rank, count, scale, rows].
+constexpr int kGroup = 4 + 16;
+
+// A workgroup's share of `parts` x `tiles`: every XCD (workgroups b, b + 8, ...) takes parts of its own for all tiles,
+// so that one L2 holds what they read of the adapters. False: none (the grid is a multiple of 8).
+__device__ __forceinline__ bool share(int parts, int tiles, int *tile, int *part) {
+    const int at = (blockIdx.x % 8) * (gridDim.x / 8) + blockIdx.x / 8;
+    *part = at / tiles;
+    *tile = at % tiles;
+    return *part < parts;
+}
 
 // Parts of t = A x of the units u, u + gridDim.y, ... of 64 rows: workgroup s takes every unit's s-th share of the
-// columns, its waves a quarter of that, and adds them up. RB: tiles of 16 ranks at a time.
-template <class T, int RB>
+// columns, its waves parts of that, and adds them up. RB: tiles of 16 ranks at a time.
+template <class T, int RB, int MT>
 __global__ void __launch_bounds__(64 * kWaves, 2) lora_down_kernel(LoraArgs g) {
     constexpr int kAhead = 2;  // steps whose loads are under way
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j16 = lane & 15, g4 = lane >> 4;
-    const int tile = blockIdx.x / g.splits, s = blockIdx.x % g.splits;
-    __shared__ v4f sums[kWaves][RB][64];
-    Rows64 rows;
-    rows.load(g, tile, lane);
-    const int steps = g.cols / kStep, parts = g.splits * kWaves, part = s * kWaves + wave;
-    const int from = (int)((int64_t)steps * part / parts), n = (int)((int64_t)steps * (part + 1) / parts) - from;
-    Unit u;
-    for (int at = blockIdx.y; rows.unit(tile, lane, at, &u); at += gridDim.y) {
+    int tile, s;
+    if (!share(g.splits, g.tiles, &tile, &s)) return;
+    __shared__ v4f sums[4][MT * RB][64];
+    Rows64<MT> rows;
+    const int units = rows.load(g, tile, lane);
+    if (s == 0 && blockIdx.y == 0 && threadIdx.x == 0) g.groups[tile] = __builtin_popcountll(rows.first16);
+    const int part = s * kWaves + wave, from = part * g.steps + min(part, g.more), n = g.steps + (part < g.more ? 1 : 0);
+    for (int at = blockIdx.y; at < units; at += gridDim.y) {
+        Unit<MT> u;
+        rows.unit(tile, lane, at, &u);
+        if (s == 0 && wave == 0) {
+#pragma unroll
+            for (int m = 0; m < MT; m++) {
+                if (16 * m >= u.count) break;
+                const int lead = __builtin_amdgcn_readfirstlane(u.row[m]) - tile * 64;
+                const int nr = __builtin_popcountll(rows.first16 & ((1ull << lead) - 1));
+                int *rec = g.groups + g.tiles + ((size_t)tile * g.most + nr) * kGroup;
+                if (lane < 4) {
+                    const int count = min(16, u.count - 16 * m);
+                    rec[lane] = lane == 0 ? u.slot : lane == 1 ? u.rank : lane == 2 ? count : __builtin_bit_cast(int, u.scale);
+                }
+                if (lane < 16) rec[4 + lane] = u.row[m];
+            }
+        }
         if (u.rank == 0) continue;
-        const T *a = (const T *)g.a + (size_t)u.slot * g.max_rank * g.cols + 8 * g4;
-        const float *x = g.x + (size_t)u.row * g.cols + 8 * g4;
+        constexpr int kLane = Eight<T>::kLane;
+        const T *a = (const T *)g.a + (size_t)u.slot * g.max_rank * g.cols + kLane * g4;
+        const float *x[MT];
+#pragma unroll
+        for (int m = 0; m < MT; m++) x[m] = g.x + (size_t)u.row[m] * g.cols + kLane * g4;
         for (int k0 = 0; k0 < u.rank; k0 += 16 * RB) {
             int arow[RB];
 #pragma unroll
             for (int t = 0; t < RB; t++) arow[t] = min(k0 + 16 * t + j16, u.rank - 1) * g.cols;
-            v4f acc[RB] = {};
+            v4f acc[MT][RB] = {};
             Eight<T> av[kAhead][RB];
-            Eight<float> xv[kAhead];
+            Eight<float> xv[kAhead][MT];
             auto load = [&](int b, int i) {
                 const int c = (from + min(i, n - 1)) * kStep;
-                xv[b].load(x + c);
+#pragma unroll
+                for (int m = 0; m < MT; m++) xv[b][m].load(x[m] + c, Eight<T>::kSecond);
 #pragma unroll
                 for (int t = 0; t < RB; t++) av[b][t].load(a + arow[t] + c);
             };
@@ -176,138 +224,199 @@ __global__ void __launch_bounds__(64 * kWaves, 2) lora_down_kernel(LoraArgs g) {
                     for (int b = 0; b < kAhead; b++) {
                         if (i + b < n) {
 #pragma unroll
-                            for (int j = 0; j < 8; j++)
+                            for (int m = 0; m < MT; m++)
+                                if (16 * m < u.count) {
 #pragma unroll
-                                for (int t = 0; t < RB; t++)
-                                    acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(av[b][t].at(j), xv[b].at(j), acc[t], 0, 0, 0);
+                                    for (int j = 0; j < 8; j++)
+#pragma unroll
+                                        for (int t = 0; t < RB; t++)
+                                            acc[m][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(av[b][t].at(j), xv[b][m].at(j),
+                                                                                             acc[m][t], 0, 0, 0);
+                                }
                         }
                         load(b, i + b + kAhead);
                     }
                 }
             }
-#pragma unroll
-            for (int t = 0; t < RB; t++) sums[wave][t][lane] = acc[t];
-            __syncthreads();
             // lane: its row's ranks 4 g4 .. + 3 of the tile
-            for (int t = wave; t < RB; t += kWaves) {
-                const int k = k0 + 16 * t + 4 * g4;
-                v4f v = sums[0][t][lane];
 #pragma unroll
-                for (int w = 1; w < kWaves; w++) v += sums[w][t][lane];
-                if (j16 < u.count && k < u.rank) *(v4f *)(g.t + ((size_t)s * g.x_rows + u.row) * g.stride + k) = v;
+            for (int w = kWaves - 4; w >= 0; w -= 4) {
+                if (wave >= w && wave < w + 4) {
+#pragma unroll
+                    for (int m = 0; m < MT; m++)
+#pragma unroll
+                        for (int t = 0; t < RB; t++) {
+                            v4f v = acc[m][t];
+                            if (w < kWaves - 4) v += sums[wave - w][m * RB + t][lane];
+                            sums[wave - w][m * RB + t][lane] = v;
+                        }
+                }
+                __syncthreads();
+            }
+            for (int e = wave; e < MT * RB; e += kWaves) {
+                const int m = e / RB, k = k0 + 16 * (e % RB) + 4 * g4;
+                v4f v = sums[0][e][lane];
+#pragma unroll
+                for (int w = 1; w < 4; w++) v += sums[w][e][lane];
+                int row = u.row[0];
+#pragma unroll
+                for (int i = 1; i < MT; i++) row = m == i ? u.row[i] : row;
+                if (16 * m + j16 < u.count && k < u.rank) *(v4f *)(g.t + ((size_t)s * g.x_rows + row) * g.stride + k) = v;
             }
             __syncthreads();
         }
     }
 }
 
-// dst = y + scale B t of the units of 64 rows; a wave: NT tiles of 16 outputs.
-template <class T, int NT>
-__global__ void __launch_bounds__(64 * kWaves, 2) lora_up_kernel(LoraArgs g) {
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j16 = lane & 15, g4 = lane >> 4;
-    const int tile = blockIdx.x / g.chunks, n0 = ((blockIdx.x % g.chunks) * kWaves + wave) * 16 * NT;
-    extern __shared__ float tl[];  // [16][pitch]: the unit's scale t, zeros behind its rank
-    const int pitch = ((g.max_rank + 15) & ~15) + 4;
-    __shared__ int list[16];
-    Rows64 rows;
-    rows.load(g, tile, lane);
-    Unit u;
-    for (int at = blockIdx.y; rows.unit(tile, lane, at, &u); at += gridDim.y) {
-        if (u.rank == 0 && g.dst == g.y) continue;
-        const bool mine = j16 < u.count;
-        const size_t row = (size_t)u.row * g.rows;
-        v4f y[NT], acc[NT] = {};
-#pragma unroll
-        for (int t = 0; t < NT; t++) {
-            const int n = n0 + 16 * t + 4 * g4;
-            if (mine && n + 4 <= g.rows) {
-                y[t] = *(const v4fu *)(g.y + row + n);
-            } else {
-                for (int j = 0; j < 4; j++) y[t][j] = mine && n + j < g.rows ? g.y[row + n + j] : 0.0f;
-            }
-        }
-        if (u.rank > 0) {
-            if (threadIdx.x < 16) list[lane] = u.row;
-            __syncthreads();
-            const int k16 = (u.rank + 15) / 16, groups = 4 * k16;
-            for (int e = threadIdx.x; e < u.count * groups; e += 64 * kWaves) {
-                const int r = e / groups, k = 4 * (e - r * groups);
-                v4f v = {};
-                if (k < u.rank) {
-                    const float *p = g.t + (size_t)list[r] * g.stride + k;
-                    const size_t split = (size_t)g.x_rows * g.stride;
+// The parts of t, added up into the first one.
+__global__ void __launch_bounds__(256) lora_sum_kernel(float *t, int64_t n4, int splits) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n4) return;
+    v4f *p = (v4f *)t + i;
+    v4f v = *p;
 #pragma unroll 8
-                    for (int s = 0; s < g.splits; s++) v += *(const v4f *)(p + s * split);
-                    v *= u.scale;
+    for (int s = 1; s < splits; s++) v += p[s * n4];
+    *p = v;
+}
+
+// dst = y + scale B t of the groups that `down` recorded; a wave: NT tiles of 16 outputs. PARTS: of t.
+template <class T, int NT, int PARTS>
+__global__ void __launch_bounds__(256, 2) lora_up_kernel(LoraArgs g) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j16 = lane & 15, g4 = lane >> 4;
+    int tile, chunk;
+    if (!share(g.chunks, g.tiles, &tile, &chunk)) return;
+    const int n0 = (chunk * 4 + wave) * 16 * NT, groups = g.groups[tile];
+    const bool whole = n0 + 16 * NT <= g.rows;
+    for (int at = blockIdx.y; at < groups; at += gridDim.y) {
+        const int *rec = g.groups + g.tiles + ((size_t)tile * g.most + at) * kGroup;
+        const int slot = rec[0], rank = rec[1];
+        const float scale = __builtin_bit_cast(float, rec[3]);
+        if (rank == 0 && g.dst == g.y) continue;
+        const bool mine = j16 < rec[2];
+        const int row = rec[4 + j16];
+        const float *yp = g.y + (size_t)row * g.rows + n0 + 4 * g4;
+        float *dp = g.dst + (size_t)row * g.rows + n0 + 4 * g4;
+        v4f y[NT], acc[NT] = {};
+        if (whole) {
 #pragma unroll
-                    for (int j = 0; j < 4; j++) v[j] = k + j < u.rank ? v[j] : 0.0f;
+            for (int t = 0; t < NT; t++) y[t] = *(const v4fu *)(yp + 16 * t);
+        } else {
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) y[t][j] = yp[max(0, min(16 * t + j, g.rows - 1 - n0 - 4 * g4))];
+        }
+        const T *b[NT];
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+            b[t] = (const T *)g.b + ((size_t)max(slot, 0) * g.rows + min(n0 + 16 * t + j16, g.rows - 1)) * g.stride;
+        const size_t split = (size_t)g.x_rows * g.stride;
+        const float *tp = g.t + (size_t)row * g.stride;
+        if (rank > 0) {
+            // (every load is in range and without a branch; what lies behind the rank is taken as zero)
+            v4f bv[2][NT], tv[2];
+            auto load = [&](int i, int k16) {
+                const int k = min(k16 + 4 * g4, g.stride - 4);
+#pragma unroll
+                for (int t = 0; t < NT; t++) bv[i][t] = four(b[t] + k);
+                v4f part[PARTS];
+#pragma unroll
+                for (int s = 0; s < PARTS; s++) part[s] = *(const v4f *)(tp + s * split + k);
+                tv[i] = part[0];
+#pragma unroll
+                for (int s = 1; s < PARTS; s++) tv[i] += part[s];
+            };
+            auto product = [&](int i, int k16) {
+                const int k = k16 + 4 * g4;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const float tj = k + j < rank ? tv[i][j] * scale : 0.0f;
+#pragma unroll
+                    for (int t = 0; t < NT; t++) {
+                        const float bj = k + j < rank ? bv[i][t][j] : 0.0f;
+                        acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(bj, tj, acc[t], 0, 0, 0);
+                    }
                 }
-                *(v4f *)(tl + r * pitch + k) = v;
+            };
+            load(0, 0);
+            for (int k = 0; k < rank; k += 32) {
+                load(1, min(k + 16, g.stride - 4));
+                product(0, k);
+                if (k + 16 < rank) {
+                    load(0, min(k + 32, g.stride - 4));
+                    product(1, k + 16);
+                }
             }
-            __syncthreads();
-            const T *b = (const T *)g.b + (size_t)u.slot * g.rows * g.stride;
-            for (int ks = 0; ks < k16; ks++) {
-                const int k = 16 * ks + 4 * g4;
-                v4f bv[NT];
 #pragma unroll
-                for (int t = 0; t < NT; t++)
-                    bv[t] = k < g.stride ? four(b + (size_t)min(n0 + 16 * t + j16, g.rows - 1) * g.stride + k) : v4f{};
-                const v4f tv = *(const v4f *)(tl + j16 * pitch + k);
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-#pragma unroll
-                    for (int t = 0; t < NT; t++)
-                        acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(bv[t][j], tv[j], acc[t], 0, 0, 0);
-            }
-            __syncthreads();  // before the next unit's t
+            for (int t = 0; t < NT; t++) y[t] += acc[t];
         }
         // lane: its row's outputs 4 g4 .. + 3 of the tile
+        if (whole) {
 #pragma unroll
-        for (int t = 0; t < NT; t++) {
-            const int n = n0 + 16 * t + 4 * g4;
-            const v4f v = u.rank > 0 ? y[t] + acc[t] : y[t];
-            if (mine && n + 4 <= g.rows) {
-                *(v4fu *)(g.dst + row + n) = v;
-            } else {
+            for (int t = 0; t < NT; t++)
+                if (mine) *(v4fu *)(dp + 16 * t) = y[t];
+        } else {
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
                 for (int j = 0; j < 4; j++)
-                    if (mine && n + j < g.rows) g.dst[row + n + j] = v[j];
-            }
+                    if (mine && n0 + 4 * g4 + 16 * t + j < g.rows) dp[16 * t + j] = y[t][j];
         }
     }
 }
 
-// Workgroups of 64 rows' units: as many as there can be, or fewer that loop where most would find none.
+// Groups of 16 rows with one adapter that 64 rows can have, splits of the columns, and the tiles of 16 rows in a unit.
 struct Plan {
-    int tiles, units, splits;
+    int tiles, most, splits, mt;
 };
 
-constexpr int kTarget = 1024;  // workgroups of `down`
+constexpr int kCUs = 256;
+constexpr int kParts = 8;  // of t, where `up` adds them up
+
+int eights(int n) { return (n + 7) / 8 * 8; }
 
 Plan plan(const LoraArgs &g) {
     Plan p;
+    p.mt = g.x_rows > 64 ? 4 : 1;
     p.tiles = (g.x_rows + 63) / 64;
     const int64_t rows = std::min(g.x_rows, 64);
-    const int most = (int)std::min<int64_t>(rows, (rows + 15) / 16 + (int64_t)g.slots);
-    p.units = std::min<int64_t>(most, std::max(8, kTarget / p.tiles));
-    p.splits = std::max(1, std::min({kTarget / std::max(1, p.tiles * p.units), g.cols / kStep / kWaves, 16}));
+    p.most = (int)std::min<int64_t>(rows, (rows + 15) / 16 + (int64_t)g.slots);
+    const int fit = std::max(1, g.cols / kStep / kWaves);
+    if (p.mt == 1) p.splits = kParts;  // (fewer columns: some of zeros)
+    else p.splits = std::max(1, std::min({kCUs / p.tiles, fit, 32}));  // a workgroup for every CU
     return p;
 }
 
-template <class T>
-sllm_status launch(LoraArgs g, const Plan &p, hipStream_t s) {
-    const dim3 down(p.tiles * p.splits, p.units), wg(64 * kWaves);
-    if (g.max_rank <= 16) hipLaunchKernelGGL((lora_down_kernel<T, 1>), down, wg, 0, s, g);
-    else if (g.max_rank <= 32) hipLaunchKernelGGL((lora_down_kernel<T, 2>), down, wg, 0, s, g);
-    else hipLaunchKernelGGL((lora_down_kernel<T, 4>), down, wg, 0, s, g);
+template <class T, int MT>
+sllm_status launch_rows(LoraArgs g, const Plan &p, hipStream_t s) {
+    // A workgroup for every unit there can be, or (prompts) one for all of 64 rows: they come together, so that 64 have
+    // little more than one unit, and two of 32 rows take no more products than one of 64. (Workgroups that may find
+    // nothing cost more than that: 700 rows of 3 adapters, f32, rank 64: 49 us with four for 64 rows.)
+    const dim3 down(eights(p.tiles * p.splits), MT == 1 ? p.most : 1), wg(64 * kWaves);
+    if (g.max_rank <= 16) hipLaunchKernelGGL((lora_down_kernel<T, 1, MT>), down, wg, 0, s, g);
+    else if (g.max_rank <= 32) hipLaunchKernelGGL((lora_down_kernel<T, 2, MT>), down, wg, 0, s, g);
+    else hipLaunchKernelGGL((lora_down_kernel<T, 4, MT>), down, wg, 0, s, g);
     SLLM_HIP(hipGetLastError());
-    const int wide = kWaves * 16 * 4, lds = 16 * (((g.max_rank + 15) & ~15) + 4) * 4;
-    const bool many = (int64_t)p.tiles * p.units * ((g.rows + wide - 1) / wide) >= 256;
-    g.chunks = many ? (g.rows + wide - 1) / wide : (g.rows + wide / 4 - 1) / (wide / 4);
-    const dim3 up(p.tiles * g.chunks, p.units);
-    if (many) hipLaunchKernelGGL((lora_up_kernel<T, 4>), up, wg, lds, s, g);
-    else hipLaunchKernelGGL((lora_up_kernel<T, 1>), up, wg, lds, s, g);
+    if (MT > 1 && g.splits > 1) {
+        const int64_t n4 = (int64_t)g.x_rows * g.stride / 4;
+        hipLaunchKernelGGL(lora_sum_kernel, dim3((unsigned)((n4 + 255) / 256)), dim3(256), 0, s, g.t, n4, g.splits);
+        SLLM_HIP(hipGetLastError());
+    }
+    constexpr int wide = 4 * 16 * 4, narrow = wide / 4;
+    const int groups = MT == 1 ? p.most : std::min(p.most, 4);
+    const bool many = (int64_t)p.tiles * groups * ((g.rows + wide - 1) / wide) >= kCUs;
+    g.chunks = many ? (g.rows + wide - 1) / wide : (g.rows + narrow - 1) / narrow;
+    const dim3 up(eights(p.tiles * g.chunks), groups);
+    constexpr int parts = MT == 1 ? kParts : 1;
+    if (many) hipLaunchKernelGGL((lora_up_kernel<T, 4, parts>), up, dim3(256), 0, s, g);
+    else hipLaunchKernelGGL((lora_up_kernel<T, 1, parts>), up, dim3(256), 0, s, g);
     SLLM_HIP(hipGetLastError());
     return SLLM_OK;
+}
+
+template <class T>
+sllm_status launch(const LoraArgs &g, const Plan &p, hipStream_t s) {
+    return p.mt > 1 ? launch_rows<T, 4>(g, p, s) : launch_rows<T, 1>(g, p, s);
 }
 
 }  // namespace
@@ -420,13 +529,20 @@ sllm_status sllm_lora_add_dev(const sllm_lora_set *set, const float *x, int x_ro
     g.stride = set->stride();
     g.x_rows = x_rows;
     const Plan p = plan(g);
+    g.tiles = p.tiles;
     g.splits = p.splits;
+    g.most = p.most;
+    g.steps = g.cols / kStep / (p.splits * kWaves);
+    g.more = g.cols / kStep % (p.splits * kWaves);
     void *ws = nullptr;
     size_t cap = 0;
     hipStream_t s = (hipStream_t)stream;
-    const sllm_status st = stream_workspace(s, (size_t)p.splits * x_rows * g.stride * sizeof(float), &ws, &cap);
+    const size_t parts = (size_t)p.splits * x_rows * g.stride * sizeof(float);
+    const size_t groups = (size_t)p.tiles * (1 + (size_t)p.most * kGroup) * sizeof(int);
+    const sllm_status st = stream_workspace(s, parts + groups, &ws, &cap);
     if (st != SLLM_OK) return st;
     g.t = (float *)ws;
+    g.groups = (int *)((char *)ws + parts);
     if (set->type == SLLM_LORA_F32) return launch<float>(g, p, s);
     if (set->type == SLLM_LORA_F16) return launch<_Float16>(g, p, s);
     return launch<uint16_t>(g, p, s);
