@@ -15,6 +15,7 @@
 #include <memory>
 #include <new>
 #include <string>
+#include <type_traits>
 
 #include "qmm_device.hpp"
 #include "qmm_pages.hpp"
@@ -41,12 +42,14 @@ struct LoraArgs {
 };
 
 constexpr int kWaves = 8;  // of a `down` workgroup
+constexpr int kGroup = 4 + 16;  // ints of a group's record: slot, rank, count, scale, rows (behind the count: the first)
 constexpr int kStep = 32;  // columns of a load: 128 bytes of x for every row
 
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef float v4fu __attribute__((ext_vector_type(4), aligned(4)));  // rows of any length
 typedef _Float16 v4h __attribute__((ext_vector_type(4)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef int v4i __attribute__((ext_vector_type(4)));
 typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 
@@ -92,10 +95,15 @@ __device__ __forceinline__ v4f four(const uint16_t *p) {
 }
 
 // Up to 16 MT rows with one adapter (rank 0: with none).
-template <int MT>
 struct Unit {
-    int slot, rank, count, row[MT];  // row: of lane % 16 of a tile of 16 (behind the count: the first one's)
+    int slot, rank, count;
     float scale;
+    int tile, order;  // lane: the number of its row among the 64
+
+    // Its k-th row (behind the count: the first one).
+    __device__ __forceinline__ int row(int k) const {
+        return tile * 64 + __builtin_amdgcn_ds_bpermute(4 * (k < count ? k : 0), order);
+    }
 };
 
 // The ids of 64 rows, a lane each, their adapters, and the units of up to 16 MT rows with one adapter: in the order of
@@ -133,7 +141,7 @@ struct Rows64 {
     }
 
     // the u-th
-    __device__ __forceinline__ void unit(int tile, int lane, int u, Unit<MT> *out) const {
+    __device__ __forceinline__ void unit(int tile, int lane, int u, Unit *out) const {
         const uint64_t below = (1ull << lane) - 1;
         const int lead = __builtin_ctzll(__ballot((first >> lane & 1) && __builtin_popcountll(first & below) == u));
         out->slot = __builtin_amdgcn_readlane(id, lead);
@@ -145,17 +153,25 @@ struct Rows64 {
         // every lane sends its number: the unit's to the front, in order
         const int to = mine >> lane & 1 ? __builtin_popcountll(mine & below)
                                         : out->count + __builtin_popcountll(~mine & below);
-        const int lanes = __builtin_amdgcn_ds_permute(4 * to, lane);
-#pragma unroll
-        for (int m = 0; m < MT; m++) {
-            const int k = 16 * m + (lane & 15);
-            out->row[m] = tile * 64 + __builtin_amdgcn_ds_bpermute(4 * (k < out->count ? k : 0), lanes);
+        out->order = __builtin_amdgcn_ds_permute(4 * to, lane);
+        out->tile = tile;
+    }
+
+    // What `up` needs to know of the unit's groups; by one wave.
+    __device__ __forceinline__ void record(const LoraArgs &g, int lane, const Unit &u) const {
+        for (int k = 0; k < u.count; k += 16) {
+            const int row = u.row(k + (lane & 15));
+            const int lead = __builtin_amdgcn_readfirstlane(row) - u.tile * 64;
+            const int nr = __builtin_popcountll(first16 & ((1ull << lead) - 1));
+            int *rec = g.groups + ((g.tiles + 3) & ~3) + ((size_t)u.tile * g.most + nr) * kGroup;
+            if (lane < 4) {
+                const int count = min(16, u.count - k);
+                rec[lane] = lane == 0 ? u.slot : lane == 1 ? u.rank : lane == 2 ? count : __builtin_bit_cast(int, u.scale);
+            }
+            if (lane < 16) rec[4 + lane] = row;
         }
     }
 };
-
-// What `up` needs to know of a group: ints [slot, rank, count, scale, rows].
-constexpr int kGroup = 4 + 16;
 
 // A workgroup's share of `parts` x `tiles`: every XCD (workgroups b, b + 8, ...) takes parts of its own for all tiles,
 // so that one L2 holds what they read of the adapters. False: none (the grid is a multiple of 8).
@@ -166,53 +182,38 @@ __device__ __forceinline__ bool share(int parts, int tiles, int *tile, int *part
     return *part < parts;
 }
 
-// Parts of t = A x of the units u, u + gridDim.y, ... of 64 rows: workgroup s takes every unit's s-th share of the
-// columns, its waves parts of that, and adds them up. RB: tiles of 16 ranks at a time.
-template <class T, int RB, int MT>
+// Parts of t = A x of the units u, u + gridDim.y, ... of up to 16 of 64 rows: workgroup s takes every unit's s-th share
+// of the columns, its waves parts of that, and adds them up. RB: tiles of 16 ranks at a time.
+template <class T, int RB>
 __global__ void __launch_bounds__(64 * kWaves, 2) lora_down_kernel(LoraArgs g) {
     constexpr int kAhead = 2;  // steps whose loads are under way
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j16 = lane & 15, g4 = lane >> 4;
     int tile, s;
     if (!share(g.splits, g.tiles, &tile, &s)) return;
-    __shared__ v4f sums[4][MT * RB][64];
-    Rows64<MT> rows;
+    __shared__ v4f sums[kWaves][RB][64];
+    Rows64<1> rows;
     const int units = rows.load(g, tile, lane);
-    if (s == 0 && blockIdx.y == 0 && threadIdx.x == 0) g.groups[tile] = __builtin_popcountll(rows.first16);
+    if (s == 0 && blockIdx.y == 0 && threadIdx.x == 0) g.groups[tile] = units;
     const int part = s * kWaves + wave, from = part * g.steps + min(part, g.more), n = g.steps + (part < g.more ? 1 : 0);
     for (int at = blockIdx.y; at < units; at += gridDim.y) {
-        Unit<MT> u;
+        Unit u;
         rows.unit(tile, lane, at, &u);
-        if (s == 0 && wave == 0) {
-#pragma unroll
-            for (int m = 0; m < MT; m++) {
-                if (16 * m >= u.count) break;
-                const int lead = __builtin_amdgcn_readfirstlane(u.row[m]) - tile * 64;
-                const int nr = __builtin_popcountll(rows.first16 & ((1ull << lead) - 1));
-                int *rec = g.groups + g.tiles + ((size_t)tile * g.most + nr) * kGroup;
-                if (lane < 4) {
-                    const int count = min(16, u.count - 16 * m);
-                    rec[lane] = lane == 0 ? u.slot : lane == 1 ? u.rank : lane == 2 ? count : __builtin_bit_cast(int, u.scale);
-                }
-                if (lane < 16) rec[4 + lane] = u.row[m];
-            }
-        }
+        if (s == 0 && wave == 0) rows.record(g, lane, u);
         if (u.rank == 0) continue;
         constexpr int kLane = Eight<T>::kLane;
+        const int row = u.row(j16);
         const T *a = (const T *)g.a + (size_t)u.slot * g.max_rank * g.cols + kLane * g4;
-        const float *x[MT];
-#pragma unroll
-        for (int m = 0; m < MT; m++) x[m] = g.x + (size_t)u.row[m] * g.cols + kLane * g4;
+        const float *x = g.x + (size_t)row * g.cols + kLane * g4;
         for (int k0 = 0; k0 < u.rank; k0 += 16 * RB) {
             int arow[RB];
 #pragma unroll
             for (int t = 0; t < RB; t++) arow[t] = min(k0 + 16 * t + j16, u.rank - 1) * g.cols;
-            v4f acc[MT][RB] = {};
+            v4f acc[RB] = {};
             Eight<T> av[kAhead][RB];
-            Eight<float> xv[kAhead][MT];
+            Eight<float> xv[kAhead];
             auto load = [&](int b, int i) {
                 const int c = (from + min(i, n - 1)) * kStep;
-#pragma unroll
-                for (int m = 0; m < MT; m++) xv[b][m].load(x[m] + c, Eight<T>::kSecond);
+                xv[b].load(x + c, Eight<T>::kSecond);
 #pragma unroll
                 for (int t = 0; t < RB; t++) av[b][t].load(a + arow[t] + c);
             };
@@ -224,15 +225,10 @@ __global__ void __launch_bounds__(64 * kWaves, 2) lora_down_kernel(LoraArgs g) {
                     for (int b = 0; b < kAhead; b++) {
                         if (i + b < n) {
 #pragma unroll
-                            for (int m = 0; m < MT; m++)
-                                if (16 * m < u.count) {
+                            for (int j = 0; j < 8; j++)
 #pragma unroll
-                                    for (int j = 0; j < 8; j++)
-#pragma unroll
-                                        for (int t = 0; t < RB; t++)
-                                            acc[m][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(av[b][t].at(j), xv[b][m].at(j),
-                                                                                             acc[m][t], 0, 0, 0);
-                                }
+                                for (int t = 0; t < RB; t++)
+                                    acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(av[b][t].at(j), xv[b].at(j), acc[t], 0, 0, 0);
                         }
                         load(b, i + b + kAhead);
                     }
@@ -240,27 +236,171 @@ __global__ void __launch_bounds__(64 * kWaves, 2) lora_down_kernel(LoraArgs g) {
             }
             // lane: its row's ranks 4 g4 .. + 3 of the tile
 #pragma unroll
-            for (int w = kWaves - 4; w >= 0; w -= 4) {
-                if (wave >= w && wave < w + 4) {
+            for (int t = 0; t < RB; t++) sums[wave][t][lane] = acc[t];
+            __syncthreads();
+            for (int t = wave; t < RB; t += kWaves) {
+                const int k = k0 + 16 * t + 4 * g4;
+                v4f v = sums[0][t][lane];
 #pragma unroll
-                    for (int m = 0; m < MT; m++)
-#pragma unroll
-                        for (int t = 0; t < RB; t++) {
-                            v4f v = acc[m][t];
-                            if (w < kWaves - 4) v += sums[wave - w][m * RB + t][lane];
-                            sums[wave - w][m * RB + t][lane] = v;
-                        }
-                }
-                __syncthreads();
+                for (int w = 1; w < kWaves; w++) v += sums[w][t][lane];
+                if (j16 < u.count && k < u.rank) *(v4f *)(g.t + ((size_t)s * g.x_rows + row) * g.stride + k) = v;
             }
-            for (int e = wave; e < MT * RB; e += kWaves) {
-                const int m = e / RB, k = k0 + 16 * (e % RB) + 4 * g4;
-                v4f v = sums[0][e][lane];
+            __syncthreads();
+        }
+    }
+}
+
+// Reads of LDS and the wait for them in one block: the compiler, which cannot tell the two stages of a ring apart, would
+// wait for all loads into LDS before any read of it.
+__device__ __forceinline__ void lds_read(v4u (&d)[8], unsigned a0, unsigned a1) {  // every 2048 bytes (rows of 128)
+    asm volatile("ds_read_b128 %0, %8\n\tds_read_b128 %1, %9\n\tds_read_b128 %2, %8 offset:2048\n\t"
+                 "ds_read_b128 %3, %9 offset:2048\n\tds_read_b128 %4, %8 offset:4096\n\tds_read_b128 %5, %9 offset:4096\n\t"
+                 "ds_read_b128 %6, %8 offset:6144\n\tds_read_b128 %7, %9 offset:6144\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(d[0]), "=&v"(d[1]), "=&v"(d[2]), "=&v"(d[3]), "=&v"(d[4]), "=&v"(d[5]), "=&v"(d[6]), "=&v"(d[7])
+                 : "v"(a0), "v"(a1)
+                 : "memory");
+}
+__device__ __forceinline__ void lds_read(v4u (&d)[4], unsigned a0, unsigned a1) {
+    asm volatile("ds_read_b128 %0, %4\n\tds_read_b128 %1, %5\n\tds_read_b128 %2, %4 offset:2048\n\t"
+                 "ds_read_b128 %3, %5 offset:2048\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(d[0]), "=&v"(d[1]), "=&v"(d[2]), "=&v"(d[3])
+                 : "v"(a0), "v"(a1)
+                 : "memory");
+}
+__device__ __forceinline__ void lds_read(v4u (&d)[2], unsigned a0, unsigned a1) {
+    asm volatile("ds_read_b128 %0, %2\n\tds_read_b128 %1, %3\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(d[0]), "=&v"(d[1])
+                 : "v"(a0), "v"(a1)
+                 : "memory");
+}
+__device__ __forceinline__ void lds_read(v4u (&d)[4], unsigned a0) {  // every 1024 bytes (rows of 64)
+    asm volatile("ds_read_b128 %0, %4\n\tds_read_b128 %1, %4 offset:1024\n\tds_read_b128 %2, %4 offset:2048\n\t"
+                 "ds_read_b128 %3, %4 offset:3072\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(d[0]), "=&v"(d[1]), "=&v"(d[2]), "=&v"(d[3])
+                 : "v"(a0)
+                 : "memory");
+}
+__device__ __forceinline__ void lds_read(v4u (&d)[2], unsigned a0) {
+    asm volatile("ds_read_b128 %0, %2\n\tds_read_b128 %1, %2 offset:1024\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(d[0]), "=&v"(d[1])
+                 : "v"(a0)
+                 : "memory");
+}
+__device__ __forceinline__ void lds_read(v4u (&d)[1], unsigned a0) {
+    asm volatile("ds_read_b128 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=&v"(d[0]) : "v"(a0) : "memory");
+}
+
+typedef const __attribute__((address_space(1))) void *GlobalPtr;
+typedef __attribute__((address_space(3))) void *LdsPtr;
+
+// LDS of the kernel below for one wave's step: 64 rows of x, 16 RB of A.
+template <class T, int RB>
+constexpr int stage_bytes() {
+    return (64 * 4 + 16 * RB * (int)sizeof(T)) * kStep;
+}
+
+// The same of units of up to 64 rows of a prompt: 16 bytes of x or A then bring 4 .. 16 matrix instructions, and read
+// straight into their operands (16 rows x 64 bytes an instruction) they were what bounded them (700 rows, 14336 columns,
+// rank 64, f32: 41 us). So every wave brings whole lines into two stages of LDS of its own, one on its way while the
+// other is used; a row's pieces of 16 bytes are kept in an order (exclusive or with the row) that lets 16 rows' be
+// read without conflicts.
+template <class T, int RB>
+__global__ void __launch_bounds__(256, 1) lora_down_rows_kernel(LoraArgs g) {
+    constexpr int XB = 64 * 4 * kStep, stage = stage_bytes<T, RB>();
+    constexpr int AL = kStep * (int)sizeof(T) / 16;   // pieces of a row of A: 8 or 4
+    constexpr int AN = 16 * RB * AL / 64, NL = 8 + AN;  // loads of a step: of A, of both
+    extern __shared__ v4f lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j16 = lane & 15, g4 = lane >> 4;
+    int tile, s;
+    if (!share(g.splits, g.tiles, &tile, &s)) return;
+    char *ring = (char *)lds + wave * 2 * stage;
+    const unsigned ring_at = (unsigned)(uintptr_t)(LdsPtr)ring;
+    // operands in a stage: lane j16, g4 takes a row's columns as Eight has them
+    const unsigned px = j16 * 128 + ((AL == 8 ? g4 : 2 * g4) ^ (j16 >> 1)) * 16;
+    const unsigned px2 = j16 * 128 + ((AL == 8 ? 4 + g4 : 2 * g4 + 1) ^ (j16 >> 1)) * 16;
+    const unsigned pa = XB + j16 * 64 + (g4 ^ (j16 >> 2)) * 16;  // (AL == 8: as x)
+    Rows64<4> rows;
+    const int units = rows.load(g, tile, lane);
+    if (s == 0 && threadIdx.x == 0) g.groups[tile] = __builtin_popcountll(rows.first16);
+    const int part = s * 4 + wave, from = part * g.steps + min(part, g.more), n = g.steps + (part < g.more ? 1 : 0);
+    for (int at = 0; at < units; at++) {
+        Unit u;
+        rows.unit(tile, lane, at, &u);
+        if (s == 0 && wave == 0) rows.record(g, lane, u);
+        if (u.rank == 0) continue;
+        const float *x[8];
 #pragma unroll
-                for (int w = 1; w < 4; w++) v += sums[w][e][lane];
-                int row = u.row[0];
+        for (int q = 0; q < 8; q++)
+            x[q] = g.x + (size_t)u.row(8 * q + (lane >> 3)) * g.cols + (size_t)from * kStep + ((lane & 7) ^ ((4 * q + g4) & 7)) * 4;
+        const T *a = (const T *)g.a + (size_t)u.slot * g.max_rank * g.cols + (size_t)from * kStep;
+        int out[4];
 #pragma unroll
-                for (int i = 1; i < MT; i++) row = m == i ? u.row[i] : row;
+        for (int m = 0; m < 4; m++) out[m] = u.row(16 * m + j16);
+        for (int k0 = 0; k0 < u.rank; k0 += 16 * RB) {
+            int arow[AN];
+#pragma unroll
+            for (int q = 0; q < AN; q++) {
+                const int r = AL == 8 ? 8 * q + (lane >> 3) : 16 * q + (lane >> 2);
+                const int piece = AL == 8 ? (lane & 7) ^ ((4 * q + g4) & 7) : (lane & 3) ^ g4;
+                arow[q] = min(k0 + r, u.rank - 1) * g.cols + piece * (16 / (int)sizeof(T));
+            }
+            auto fill = [&](int i) {
+                char *to = ring + (i & 1) * stage;
+#pragma unroll
+                for (int q = 0; q < 8; q++)
+                    __builtin_amdgcn_global_load_lds((GlobalPtr)(x[q] + i * kStep), (LdsPtr)(to + q * 1024), 16, 0, 0);
+#pragma unroll
+                for (int q = 0; q < AN; q++)
+                    __builtin_amdgcn_global_load_lds((GlobalPtr)(a + arow[q] + i * kStep), (LdsPtr)(to + XB + q * 1024), 16, 0, 0);
+            };
+            v4f acc[4][RB] = {};
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // earlier loads and stores don't count below
+            if (n > 0) fill(0);
+            if (n > 1) fill(1);
+            for (int i = 0; i < n; i++) {
+                if (i + 1 < n) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");
+                else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                const unsigned st = ring_at + (i & 1) * stage;
+                v4u xr[8], ar[AL == 8 ? 2 * RB : RB];
+                lds_read(xr, st + px, st + px2);
+                if constexpr (AL == 8) lds_read(ar, st + XB + px, st + XB + px2);
+                else lds_read(ar, st + pa);
+                if (i + 2 < n) fill(i + 2);
+                auto av = [&](int t, int j) {
+                    if constexpr (AL == 8) return __builtin_bit_cast(v4f, ar[2 * t + (j >> 2)])[j & 3];
+                    else if constexpr (std::is_same_v<T, _Float16>) return (float)__builtin_bit_cast(v8h, ar[t])[j];
+                    else return bf16_at(ar[t][j >> 1], j);
+                };
+                float af[RB][8];
+#pragma unroll
+                for (int t = 0; t < RB; t++)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) af[t][j] = av(t, j);
+#pragma unroll
+                for (int m = 0; m < 4; m++)
+                    if (16 * m < u.count) {
+#pragma unroll
+                        for (int j = 0; j < 8; j++)
+#pragma unroll
+                            for (int t = 0; t < RB; t++)
+                                acc[m][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                                    af[t][j], __builtin_bit_cast(v4f, xr[2 * m + (j >> 2)])[j & 3], acc[m][t], 0, 0, 0);
+                    }
+            }
+            // the waves' sums, in stages that none reads or fills any more; lane: its row's ranks 4 g4 .. + 3 of the tile
+            v4f *own = (v4f *)ring;
+#pragma unroll
+            for (int m = 0; m < 4; m++)
+#pragma unroll
+                for (int t = 0; t < RB; t++) own[(m * RB + t) * 64 + lane] = acc[m][t];
+            __syncthreads();
+#pragma unroll
+            for (int t = 0; t < RB; t++) {
+                const int k = k0 + 16 * t + 4 * g4, m = wave;
+                v4f v = lds[(m * RB + t) * 64 + lane];
+#pragma unroll
+                for (int w = 1; w < 4; w++) v += lds[w * 2 * stage / 16 + (m * RB + t) * 64 + lane];
+                const int row = m == 0 ? out[0] : m == 1 ? out[1] : m == 2 ? out[2] : out[3];
                 if (16 * m + j16 < u.count && k < u.rank) *(v4f *)(g.t + ((size_t)s * g.x_rows + row) * g.stride + k) = v;
             }
             __syncthreads();
@@ -288,31 +428,32 @@ __global__ void __launch_bounds__(256, 2) lora_up_kernel(LoraArgs g) {
     const int n0 = (chunk * 4 + wave) * 16 * NT, groups = g.groups[tile];
     const bool whole = n0 + 16 * NT <= g.rows;
     for (int at = blockIdx.y; at < groups; at += gridDim.y) {
-        const int *rec = g.groups + g.tiles + ((size_t)tile * g.most + at) * kGroup;
-        const int slot = rec[0], rank = rec[1];
+        const int *rec = g.groups + ((g.tiles + 3) & ~3) + ((size_t)tile * g.most + at) * kGroup;
+        const int slot = rec[0], rank = rec[1], count = rec[2];
         const float scale = __builtin_bit_cast(float, rec[3]);
         if (rank == 0 && g.dst == g.y) continue;
-        const bool mine = j16 < rec[2];
-        const int row = rec[4 + j16];
-        const float *yp = g.y + (size_t)row * g.rows + n0 + 4 * g4;
-        float *dp = g.dst + (size_t)row * g.rows + n0 + 4 * g4;
-        v4f y[NT], acc[NT] = {};
-        if (whole) {
+        // lane: NT outputs in a row, n0 + NT j16 .., of the rows 4 g4 .. + 3 (NT 4: whole lines of four rows at a time)
+        const v4i r4 = *(const v4i *)(rec + 4 + 4 * g4);
+        const int n = n0 + NT * j16;
+        float y[4][NT];
+        v4f acc[NT] = {};
 #pragma unroll
-            for (int t = 0; t < NT; t++) y[t] = *(const v4fu *)(yp + 16 * t);
-        } else {
+        for (int r = 0; r < 4; r++) {
+            const float *p = g.y + (size_t)r4[r] * g.rows;
+            if (whole) {
+                if constexpr (NT == 4) *(v4f *)y[r] = *(const v4fu *)(p + n);
+                else y[r][0] = p[n];
+            } else {
 #pragma unroll
-            for (int t = 0; t < NT; t++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) y[t][j] = yp[max(0, min(16 * t + j, g.rows - 1 - n0 - 4 * g4))];
+                for (int t = 0; t < NT; t++) y[r][t] = p[min(n + t, g.rows - 1)];
+            }
         }
-        const T *b[NT];
-#pragma unroll
-        for (int t = 0; t < NT; t++)
-            b[t] = (const T *)g.b + ((size_t)max(slot, 0) * g.rows + min(n0 + 16 * t + j16, g.rows - 1)) * g.stride;
-        const size_t split = (size_t)g.x_rows * g.stride;
-        const float *tp = g.t + (size_t)row * g.stride;
         if (rank > 0) {
+            const T *b[NT];
+#pragma unroll
+            for (int t = 0; t < NT; t++) b[t] = (const T *)g.b + ((size_t)slot * g.rows + min(n + t, g.rows - 1)) * g.stride;
+            const size_t split = (size_t)g.x_rows * g.stride;
+            const float *tp = g.t + (size_t)rec[4 + j16] * g.stride;
             // (every load is in range and without a branch; what lies behind the rank is taken as zero)
             v4f bv[2][NT], tv[2];
             auto load = [&](int i, int k16) {
@@ -334,40 +475,44 @@ __global__ void __launch_bounds__(256, 2) lora_up_kernel(LoraArgs g) {
 #pragma unroll
                     for (int t = 0; t < NT; t++) {
                         const float bj = k + j < rank ? bv[i][t][j] : 0.0f;
-                        acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(bj, tj, acc[t], 0, 0, 0);
+                        acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(tj, bj, acc[t], 0, 0, 0);
                     }
                 }
             };
             load(0, 0);
             for (int k = 0; k < rank; k += 32) {
-                load(1, min(k + 16, g.stride - 4));
+                load(1, k + 16);
                 product(0, k);
                 if (k + 16 < rank) {
-                    load(0, min(k + 32, g.stride - 4));
+                    load(0, k + 32);
                     product(1, k + 16);
                 }
             }
 #pragma unroll
-            for (int t = 0; t < NT; t++) y[t] += acc[t];
+            for (int r = 0; r < 4; r++)
+#pragma unroll
+                for (int t = 0; t < NT; t++) y[r][t] += acc[t][r];
         }
-        // lane: its row's outputs 4 g4 .. + 3 of the tile
-        if (whole) {
 #pragma unroll
-            for (int t = 0; t < NT; t++)
-                if (mine) *(v4fu *)(dp + 16 * t) = y[t];
-        } else {
+        for (int r = 0; r < 4; r++) {
+            float *p = g.dst + (size_t)r4[r] * g.rows;
+            if (4 * g4 + r < count) {
+                if (whole) {
+                    if constexpr (NT == 4) *(v4fu *)(p + n) = *(v4f *)y[r];
+                    else p[n] = y[r][0];
+                } else {
 #pragma unroll
-            for (int t = 0; t < NT; t++)
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    if (mine && n0 + 4 * g4 + 16 * t + j < g.rows) dp[16 * t + j] = y[t][j];
+                    for (int t = 0; t < NT; t++)
+                        if (n + t < g.rows) p[n + t] = y[r][t];
+                }
+            }
         }
     }
 }
 
 // Groups of 16 rows with one adapter that 64 rows can have, splits of the columns, and the tiles of 16 rows in a unit.
 struct Plan {
-    int tiles, most, splits, mt;
+    int tiles, most, splits, mt, waves;
 };
 
 constexpr int kCUs = 256;
@@ -381,7 +526,8 @@ Plan plan(const LoraArgs &g) {
     p.tiles = (g.x_rows + 63) / 64;
     const int64_t rows = std::min(g.x_rows, 64);
     p.most = (int)std::min<int64_t>(rows, (rows + 15) / 16 + (int64_t)g.slots);
-    const int fit = std::max(1, g.cols / kStep / kWaves);
+    p.waves = p.mt == 1 ? kWaves : 4;  // of a `down` workgroup
+    const int fit = std::max(1, g.cols / kStep / p.waves);
     if (p.mt == 1) p.splits = kParts;  // (fewer columns: some of zeros)
     else p.splits = std::max(1, std::min({kCUs / p.tiles, fit, 32}));  // a workgroup for every CU
     return p;
@@ -392,10 +538,18 @@ sllm_status launch_rows(LoraArgs g, const Plan &p, hipStream_t s) {
     // A workgroup for every unit there can be, or (prompts) one for all of 64 rows: they come together, so that 64 have
     // little more than one unit, and two of 32 rows take no more products than one of 64. (Workgroups that may find
     // nothing cost more than that: 700 rows of 3 adapters, f32, rank 64: 49 us with four for 64 rows.)
-    const dim3 down(eights(p.tiles * p.splits), MT == 1 ? p.most : 1), wg(64 * kWaves);
-    if (g.max_rank <= 16) hipLaunchKernelGGL((lora_down_kernel<T, 1, MT>), down, wg, 0, s, g);
-    else if (g.max_rank <= 32) hipLaunchKernelGGL((lora_down_kernel<T, 2, MT>), down, wg, 0, s, g);
-    else hipLaunchKernelGGL((lora_down_kernel<T, 4, MT>), down, wg, 0, s, g);
+    const int grid = eights(p.tiles * p.splits);
+    if constexpr (MT == 1) {
+        const dim3 down(grid, p.most), wg(64 * kWaves);
+        if (g.max_rank <= 16) hipLaunchKernelGGL((lora_down_kernel<T, 1>), down, wg, 0, s, g);
+        else if (g.max_rank <= 32) hipLaunchKernelGGL((lora_down_kernel<T, 2>), down, wg, 0, s, g);
+        else hipLaunchKernelGGL((lora_down_kernel<T, 4>), down, wg, 0, s, g);
+    } else {
+        const dim3 down(grid), wg(256);
+        if (g.max_rank <= 16) hipLaunchKernelGGL((lora_down_rows_kernel<T, 1>), down, wg, (8 * stage_bytes<T, 1>()), s, g);
+        else if (g.max_rank <= 32) hipLaunchKernelGGL((lora_down_rows_kernel<T, 2>), down, wg, (8 * stage_bytes<T, 2>()), s, g);
+        else hipLaunchKernelGGL((lora_down_rows_kernel<T, 4>), down, wg, (8 * stage_bytes<T, 4>()), s, g);
+    }
     SLLM_HIP(hipGetLastError());
     if (MT > 1 && g.splits > 1) {
         const int64_t n4 = (int64_t)g.x_rows * g.stride / 4;
@@ -532,13 +686,13 @@ sllm_status sllm_lora_add_dev(const sllm_lora_set *set, const float *x, int x_ro
     g.tiles = p.tiles;
     g.splits = p.splits;
     g.most = p.most;
-    g.steps = g.cols / kStep / (p.splits * kWaves);
-    g.more = g.cols / kStep % (p.splits * kWaves);
+    g.steps = g.cols / kStep / (p.splits * p.waves);
+    g.more = g.cols / kStep % (p.splits * p.waves);
     void *ws = nullptr;
     size_t cap = 0;
     hipStream_t s = (hipStream_t)stream;
     const size_t parts = (size_t)p.splits * x_rows * g.stride * sizeof(float);
-    const size_t groups = (size_t)p.tiles * (1 + (size_t)p.most * kGroup) * sizeof(int);
+    const size_t groups = (((size_t)p.tiles + 3) / 4 * 4 + (size_t)p.tiles * p.most * kGroup) * sizeof(int);
     const sllm_status st = stream_workspace(s, parts + groups, &ws, &cap);
     if (st != SLLM_OK) return st;
     g.t = (float *)ws;
