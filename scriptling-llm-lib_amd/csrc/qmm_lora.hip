@@ -24,6 +24,14 @@ namespace sllm {
 
 namespace {
 
+// Where B[n][k] lies in its adapter: 64 outputs by 16 ranks together (fewer at the end of the stride), four operands of a
+// matrix instruction (outputs 4 j + t, j < 16) whose lanes' four ranks follow each other, so that a load of `up` reads
+// 512 or 1024 bytes in a row (as rows of B, 64 bytes of 16 rows: 17.6 us instead of 14.3 for 700 rows of rank 64, f32).
+__host__ __device__ __forceinline__ int b_at(int n, int k, int stride) {
+    const int k16 = k & ~15, groups = stride - k16 < 16 ? (stride - k16) / 4 : 4;
+    return (n / 64 * stride + k16) * 64 + ((n % 4 * groups + (k - k16) / 4) * 16 + n % 64 / 4) * 4 + k % 4;
+}
+
 // What the kernels read of one adapter; rank 0: none loaded.
 struct Adapter {
     int rank = 0;
@@ -31,7 +39,7 @@ struct Adapter {
 };
 
 struct LoraArgs {
-    const void *a, *b;  // [slot][max_rank][cols], [slot][rows][stride], zeros behind an adapter's rank in b
+    const void *a, *b;  // [slot][max_rank][cols]; [slot], as b_at has it, zeros behind an adapter's rank
     const Adapter *adapters;
     const int *ids;
     const float *x, *y;
@@ -186,7 +194,6 @@ __device__ __forceinline__ bool share(int parts, int tiles, int *tile, int *part
 // of the columns, its waves parts of that, and adds them up. RB: tiles of 16 ranks at a time.
 template <class T, int RB>
 __global__ void __launch_bounds__(64 * kWaves, 2) lora_down_kernel(LoraArgs g) {
-    constexpr int kAhead = 2;  // steps whose loads are under way
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j16 = lane & 15, g4 = lane >> 4;
     int tile, s;
     if (!share(g.splits, g.tiles, &tile, &s)) return;
@@ -209,31 +216,33 @@ __global__ void __launch_bounds__(64 * kWaves, 2) lora_down_kernel(LoraArgs g) {
 #pragma unroll
             for (int t = 0; t < RB; t++) arow[t] = min(k0 + 16 * t + j16, u.rank - 1) * g.cols;
             v4f acc[RB] = {};
-            Eight<T> av[kAhead][RB];
-            Eight<float> xv[kAhead];
-            auto load = [&](int b, int i) {
-                const int c = (from + min(i, n - 1)) * kStep;
-                xv[b].load(x + c, Eight<T>::kSecond);
+            // some steps, their loads under way together
+            auto steps = [&](auto count, int i) {
+                constexpr int D = decltype(count)::value;
+                Eight<T> av[D][RB];
+                Eight<float> xv[D];
 #pragma unroll
-                for (int t = 0; t < RB; t++) av[b][t].load(a + arow[t] + c);
-            };
-            if (n > 0) {
+                for (int d = 0; d < D; d++) {
+                    const int c = (from + i + d) * kStep;
+                    xv[d].load(x + c, Eight<T>::kSecond);
 #pragma unroll
-                for (int b = 0; b < kAhead; b++) load(b, b);
-                for (int i = 0; i < n; i += kAhead) {
-#pragma unroll
-                    for (int b = 0; b < kAhead; b++) {
-                        if (i + b < n) {
-#pragma unroll
-                            for (int j = 0; j < 8; j++)
-#pragma unroll
-                                for (int t = 0; t < RB; t++)
-                                    acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(av[b][t].at(j), xv[b].at(j), acc[t], 0, 0, 0);
-                        }
-                        load(b, i + b + kAhead);
-                    }
+                    for (int t = 0; t < RB; t++) av[d][t].load(a + arow[t] + c);
                 }
+#pragma unroll
+                for (int d = 0; d < D; d++)
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+#pragma unroll
+                        for (int t = 0; t < RB; t++)
+                            acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(av[d][t].at(j), xv[d].at(j), acc[t], 0, 0, 0);
+            };
+            int i = 0;
+            for (; i + 4 <= n; i += 4) steps(std::integral_constant<int, 4>(), i);
+            if (i + 2 <= n) {
+                steps(std::integral_constant<int, 2>(), i);
+                i += 2;
             }
+            if (i < n) steps(std::integral_constant<int, 1>(), i);
             // lane: its row's ranks 4 g4 .. + 3 of the tile
 #pragma unroll
             for (int t = 0; t < RB; t++) sums[wave][t][lane] = acc[t];
@@ -449,9 +458,8 @@ __global__ void __launch_bounds__(256, 2) lora_up_kernel(LoraArgs g) {
             }
         }
         if (rank > 0) {
-            const T *b[NT];
-#pragma unroll
-            for (int t = 0; t < NT; t++) b[t] = (const T *)g.b + ((size_t)slot * g.rows + min(n + t, g.rows - 1)) * g.stride;
+            const int rows64 = (g.rows + 63) & ~63, nb = min(n, rows64 - 64 + n % 64);  // (behind the rows: not stored)
+            const T *b = (const T *)g.b + (size_t)slot * rows64 * g.stride;
             const size_t split = (size_t)g.x_rows * g.stride;
             const float *tp = g.t + (size_t)rec[4 + j16] * g.stride;
             // (every load is in range and without a branch; what lies behind the rank is taken as zero)
@@ -459,7 +467,7 @@ __global__ void __launch_bounds__(256, 2) lora_up_kernel(LoraArgs g) {
             auto load = [&](int i, int k16) {
                 const int k = min(k16 + 4 * g4, g.stride - 4);
 #pragma unroll
-                for (int t = 0; t < NT; t++) bv[i][t] = four(b[t] + k);
+                for (int t = 0; t < NT; t++) bv[i][t] = four(b + b_at(nb + t, k, g.stride));
                 v4f part[PARTS];
 #pragma unroll
                 for (int s = 0; s < PARTS; s++) part[s] = *(const v4f *)(tp + s * split + k);
@@ -516,7 +524,7 @@ struct Plan {
 };
 
 constexpr int kCUs = 256;
-constexpr int kParts = 8;  // of t, where `up` adds them up
+constexpr int kParts = 8, kManyParts = 32;  // of t; `up` adds 8 up
 
 int eights(int n) { return (n + 7) / 8 * 8; }
 
@@ -528,7 +536,9 @@ Plan plan(const LoraArgs &g) {
     p.most = (int)std::min<int64_t>(rows, (rows + 15) / 16 + (int64_t)g.slots);
     p.waves = p.mt == 1 ? kWaves : 4;  // of a `down` workgroup
     const int fit = std::max(1, g.cols / kStep / p.waves);
-    if (p.mt == 1) p.splits = kParts;  // (fewer columns: some of zeros)
+    // Few units of many rows: more parts, added up by a launch of their own (64 rows, one adapter, 14336 columns, rank 64,
+    // f32: 20.6 us in 8 parts, 9.4 in 32; as many added up by `up` cost it 14 us, the launch 3).
+    if (p.mt == 1) p.splits = g.x_rows > 16 && p.most <= 8 && g.cols / kStep >= kManyParts * kWaves ? kManyParts : kParts;
     else p.splits = std::max(1, std::min({kCUs / p.tiles, fit, 32}));  // a workgroup for every CU
     return p;
 }
@@ -551,7 +561,7 @@ sllm_status launch_rows(LoraArgs g, const Plan &p, hipStream_t s) {
         else hipLaunchKernelGGL((lora_down_rows_kernel<T, 4>), down, wg, (8 * stage_bytes<T, 4>()), s, g);
     }
     SLLM_HIP(hipGetLastError());
-    if (MT > 1 && g.splits > 1) {
+    if (g.splits > 1 && g.splits != (MT == 1 ? kParts : 1)) {
         const int64_t n4 = (int64_t)g.x_rows * g.stride / 4;
         hipLaunchKernelGGL(lora_sum_kernel, dim3((unsigned)((n4 + 255) / 256)), dim3(256), 0, s, g.t, n4, g.splits);
         SLLM_HIP(hipGetLastError());
@@ -561,9 +571,13 @@ sllm_status launch_rows(LoraArgs g, const Plan &p, hipStream_t s) {
     const bool many = (int64_t)p.tiles * groups * ((g.rows + wide - 1) / wide) >= kCUs;
     g.chunks = many ? (g.rows + wide - 1) / wide : (g.rows + narrow - 1) / narrow;
     const dim3 up(eights(p.tiles * g.chunks), groups);
-    constexpr int parts = MT == 1 ? kParts : 1;
-    if (many) hipLaunchKernelGGL((lora_up_kernel<T, 4, parts>), up, dim3(256), 0, s, g);
-    else hipLaunchKernelGGL((lora_up_kernel<T, 1, parts>), up, dim3(256), 0, s, g);
+    auto run = [&](auto parts) {
+        constexpr int P = decltype(parts)::value;
+        if (many) hipLaunchKernelGGL((lora_up_kernel<T, 4, P>), up, dim3(256), 0, s, g);
+        else hipLaunchKernelGGL((lora_up_kernel<T, 1, P>), up, dim3(256), 0, s, g);
+    };
+    if (MT == 1 && p.splits == kParts) run(std::integral_constant<int, kParts>());
+    else run(std::integral_constant<int, 1>());
     SLLM_HIP(hipGetLastError());
     return SLLM_OK;
 }
@@ -581,7 +595,8 @@ struct sllm_lora_set {
     int rows = 0, cols = 0, slots = 0, max_rank = 0, type = 0, device = 0;
     char *a = nullptr, *b = nullptr;
     sllm::Adapter *adapters = nullptr;
-    int stride() const { return (max_rank + 3) & ~3; }  // of B's rows, zeros behind an adapter's rank
+    int stride() const { return (max_rank + 3) & ~3; }  // of t's and B's rows
+    int rows64() const { return (rows + 63) & ~63; }
     int elem() const { return type == SLLM_LORA_F32 ? 4 : 2; }
     ~sllm_lora_set() {
         (void)hipFree(a);
@@ -604,7 +619,7 @@ sllm_status sllm_lora_set_create(int rows, int cols, int max_adapters, int max_r
     if (type != SLLM_LORA_F32 && type != SLLM_LORA_F16 && type != SLLM_LORA_BF16)
         return set_error(SLLM_ERR_ARG, "unknown adapter type");
     // one adapter's matrices: below 2 GiB each, so that the kernels' offsets in one fit 32 bits
-    if (((int64_t)max_rank + 3) * (rows > cols ? rows : cols) * 4 >= ((int64_t)1 << 31))
+    if (((int64_t)max_rank + 3) * ((int64_t)(rows > cols ? rows : cols) + 63) * 4 >= ((int64_t)1 << 31))
         return set_error(SLLM_ERR_SHAPE, "max_rank x rows (cols) x 4 bytes must stay below 2 GiB");
     sllm_status st = library_init();
     if (st != SLLM_OK) return st;
@@ -619,7 +634,7 @@ sllm_status sllm_lora_set_create(int rows, int cols, int max_adapters, int max_r
     const size_t per = (size_t)max_adapters * w->stride() * w->elem();
     if ((double)per * (rows > cols ? rows : cols) > 1e15 ||
         hipMalloc(&w->a, (size_t)max_adapters * max_rank * w->elem() * cols) != hipSuccess ||
-        hipMalloc(&w->b, per * rows) != hipSuccess ||
+        hipMalloc(&w->b, per * w->rows64()) != hipSuccess ||
         hipMalloc(&w->adapters, (size_t)max_adapters * sizeof(Adapter)) != hipSuccess) {
         (void)hipGetLastError();
         return set_error(SLLM_ERR_OOM, "adapter allocation failed");
@@ -641,14 +656,13 @@ sllm_status sllm_lora_set_load(sllm_lora_set *set, int slot, int rank, const voi
     if (dev != set->device) return set_error(SLLM_ERR_ARG, "the adapter set is another device's");
     const Adapter ad{rank, scale};
     const size_t e = (size_t)set->elem();
-    // B with its rows at the set's stride (one copy: row by row, 4096 rows of 16 ranks took 40 ms)
-    const size_t pitch = set->stride() * e, bytes = rank > 0 ? set->rows * pitch : 0;
-    std::unique_ptr<char[]> packed(new (std::nothrow) char[bytes]);
+    const int stride = set->stride();
+    const size_t bytes = rank > 0 ? (size_t)set->rows64() * stride * e : 0;
+    std::unique_ptr<char[]> packed(new (std::nothrow) char[bytes]());
     if (!packed) return set_error(SLLM_ERR_OOM, "out of memory");
-    for (size_t r = 0; r * pitch < bytes; r++) {
-        std::memcpy(packed.get() + r * pitch, (const char *)b + r * rank * e, rank * e);
-        std::memset(packed.get() + r * pitch + rank * e, 0, pitch - rank * e);
-    }
+    for (int r = 0; rank > 0 && r < set->rows; r++)
+        for (int k = 0; k < rank; k++)
+            std::memcpy(packed.get() + (size_t)b_at(r, k, stride) * e, (const char *)b + ((size_t)r * rank + k) * e, e);
     // calls in flight on any stream may still read the slot
     SLLM_HIP(hipDeviceSynchronize());
     if (rank > 0) {
