@@ -436,8 +436,9 @@ sllm_status sllm_page_cache_compact(sllm_page_cache *pc, int *used, void *stream
 
 /*
  * The steps of up to max_seqs sequences at a time, max_rows rows in all, for
- * a model of n_heads query heads (n_kv_heads x 1..8). A batch owns the device
- * memory that its attention calls need, so those allocate nothing.
+ * a model of n_heads query heads (n_kv_heads x 1..8); max_rows x n_heads x d_k
+ * at most 2^28 (SLLM_ERR_SHAPE). A batch owns the device memory that its
+ * attention calls need, so those allocate nothing.
  * sllm_page_batch_begin begins a step: rows[i] (0: none) rows are appended to
  * sequence seqs[i] (each named once), pages taken and shared tail pages copied;
  * then one sllm_page_attention_dev per layer fills and reads them. SLLM_ERR_OOM
@@ -490,7 +491,9 @@ sllm_status sllm_lora_set_load(sllm_lora_set *set, int slot, int rank, const voi
  * names no loaded adapter (-1, say) get dst[r] = y[r]. dst may be y: the
  * output of the shared projection (sllm_matmul_dev and its kin) then gets the
  * adapters' part in place. Products and sums in fp32. x must be 16-byte aligned.
- * Asynchronous on `stream`; uses the stream's workspace (sllm_workspace_reserve).
+ * Asynchronous on `stream`; uses the stream's workspace (sllm_workspace_reserve;
+ * x_rows x (128 x max_rank + 1024) bytes are enough). A captured call reads ids
+ * and adapters as they are at each replay.
  */
 sllm_status sllm_lora_add_dev(const sllm_lora_set *set, const float *x_dev, int x_rows, const int *ids_dev,
                               const float *y_dev, float *dst_dev, void *stream);
