@@ -445,7 +445,9 @@ sllm_status sllm_page_cache_compact(sllm_page_cache *pc, int *used, void *stream
  * (and nothing changed) where there are too few vacant pages. A step ends with
  * the next begin; freeing, cutting or moving (compaction, a tail page copied for
  * another step) one of its sequences ends it too: attention calls are refused
- * (SLLM_ERR_ARG) until the next begin.
+ * (SLLM_ERR_ARG) until the next begin. Rows that a step appends exist once the
+ * attention calls of all layers are enqueued: sequences that are to have them are
+ * forked or copied behind these.
  */
 typedef struct sllm_page_batch sllm_page_batch;
 sllm_status sllm_page_batch_create(sllm_page_cache *pc, int n_heads, int max_seqs, int max_rows,

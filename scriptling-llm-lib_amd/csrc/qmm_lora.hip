@@ -531,7 +531,7 @@ int eights(int n) { return (n + 7) / 8 * 8; }
 Plan plan(const LoraArgs &g) {
     Plan p;
     p.mt = g.x_rows > 64 ? 4 : 1;
-    p.tiles = (g.x_rows + 63) / 64;
+    p.tiles = (g.x_rows - 1) / 64 + 1;
     const int64_t rows = std::min(g.x_rows, 64);
     p.most = (int)std::min<int64_t>(rows, (rows + 15) / 16 + (int64_t)g.slots);
     p.waves = p.mt == 1 ? kWaves : 4;  // of a `down` workgroup

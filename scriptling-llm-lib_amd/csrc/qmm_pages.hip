@@ -677,6 +677,9 @@ sllm_status sllm_page_batch_begin(sllm_page_batch *batch, const int *seqs, const
             b.host_cap[slot] = b.dev_cap;
         }
         if ((st = append(c, seqs, rows, count, &copies)) != SLLM_OK) return st;
+        b.begun = false;
+        // (at once: the tables name the copies from here on, whatever becomes of the rest)
+        if ((st = launch_page_copies(c, copies.data(), copies.size(), s)) != SLLM_OK) return st;
         share(c, seqs, rows, row0, std::move(who), 0, 0, &plan);
         const int n_items = cut(&plan, (int)rep, c.n_kv, kShapeRows[shape_class(c.d_k, c.type == SLLM_CACHE_F16)], b.slots);
         int *h = (int *)b.host[slot];
@@ -751,11 +754,10 @@ sllm_status sllm_page_batch_begin(sllm_page_batch *batch, const int *seqs, const
         b.versions.resize((size_t)count);
         for (int i = 0; i < count; i++) b.versions[(size_t)i] = c.seqs[(size_t)seqs[i]].version;
         b.rows = (int)total;
-        b.begun = true;
-        if ((st = launch_page_copies(c, copies.data(), copies.size(), s)) != SLLM_OK) return st;
         SLLM_HIP(hipMemcpyAsync(b.dev, h, (size_t)at * sizeof(int), hipMemcpyHostToDevice, s));
         SLLM_HIP(hipEventRecord(b.done[slot], s));
         b.slot = (slot + 1) % PageBatch::kSlots;
+        b.begun = true;
         return SLLM_OK;
     });
 }
