@@ -5,7 +5,8 @@
 // Rows of one adapter are worked on together: 64 rows' ids fit one wave, which splits them into units of up to 16
 // (prompts: 64) rows with one adapter (no sort, no launch of its own; rows in any order read an adapter once per unit).
 // Two launches: `down` (t = A x, the columns split over workgroups and their waves) and `up` (adds the parts of t in
-// order, dst = y + scale B t). Products are float32 matrix instructions (16 ranks or outputs x 16 rows x 4), exact in
+// order, dst = y + scale B t); prompts a third one between them that adds up more parts, small projections one
+// launch for all. Products are float32 matrix instructions (16 ranks or outputs x 16 rows x 4), exact in
 // x for every type of adapter; a unit of a single row wastes 15 of their 16 columns and is bound by the loads all the
 // same.
 #include <hip/hip_runtime.h>
@@ -190,6 +191,38 @@ __device__ __forceinline__ bool share(int parts, int tiles, int *tile, int *part
     return *part < parts;
 }
 
+// acc += A x over n steps of the columns; x, a: the lane's row of either operand (arow: of A's tiles).
+template <class T, int RB>
+__device__ __forceinline__ void columns(const float *x, const T *a, const int (&arow)[RB], int from, int n, v4f (&acc)[RB]) {
+    // some steps, their loads under way together
+    auto steps = [&](auto count, int i) {
+        constexpr int D = decltype(count)::value;
+        Eight<T> av[D][RB];
+        Eight<float> xv[D];
+#pragma unroll
+        for (int d = 0; d < D; d++) {
+            const int c = (from + i + d) * kStep;
+            xv[d].load(x + c, Eight<T>::kSecond);
+#pragma unroll
+            for (int t = 0; t < RB; t++) av[d][t].load(a + arow[t] + c);
+        }
+#pragma unroll
+        for (int d = 0; d < D; d++)
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+#pragma unroll
+                for (int t = 0; t < RB; t++)
+                    acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(av[d][t].at(j), xv[d].at(j), acc[t], 0, 0, 0);
+    };
+    int i = 0;
+    for (; i + 4 <= n; i += 4) steps(std::integral_constant<int, 4>(), i);
+    if (i + 2 <= n) {
+        steps(std::integral_constant<int, 2>(), i);
+        i += 2;
+    }
+    if (i < n) steps(std::integral_constant<int, 1>(), i);
+}
+
 // Parts of t = A x of the units u, u + gridDim.y, ... of up to 16 of 64 rows: workgroup s takes every unit's s-th share
 // of the columns, its waves parts of that, and adds them up. RB: tiles of 16 ranks at a time.
 template <class T, int RB>
@@ -216,33 +249,7 @@ __global__ void __launch_bounds__(64 * kWaves, 2) lora_down_kernel(LoraArgs g) {
 #pragma unroll
             for (int t = 0; t < RB; t++) arow[t] = min(k0 + 16 * t + j16, u.rank - 1) * g.cols;
             v4f acc[RB] = {};
-            // some steps, their loads under way together
-            auto steps = [&](auto count, int i) {
-                constexpr int D = decltype(count)::value;
-                Eight<T> av[D][RB];
-                Eight<float> xv[D];
-#pragma unroll
-                for (int d = 0; d < D; d++) {
-                    const int c = (from + i + d) * kStep;
-                    xv[d].load(x + c, Eight<T>::kSecond);
-#pragma unroll
-                    for (int t = 0; t < RB; t++) av[d][t].load(a + arow[t] + c);
-                }
-#pragma unroll
-                for (int d = 0; d < D; d++)
-#pragma unroll
-                    for (int j = 0; j < 8; j++)
-#pragma unroll
-                        for (int t = 0; t < RB; t++)
-                            acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(av[d][t].at(j), xv[d].at(j), acc[t], 0, 0, 0);
-            };
-            int i = 0;
-            for (; i + 4 <= n; i += 4) steps(std::integral_constant<int, 4>(), i);
-            if (i + 2 <= n) {
-                steps(std::integral_constant<int, 2>(), i);
-                i += 2;
-            }
-            if (i < n) steps(std::integral_constant<int, 1>(), i);
+            columns<T, RB>(x, a, arow, from, n, acc);
             // lane: its row's ranks 4 g4 .. + 3 of the tile
 #pragma unroll
             for (int t = 0; t < RB; t++) sums[wave][t][lane] = acc[t];
@@ -417,6 +424,69 @@ __global__ void __launch_bounds__(256, 1) lora_down_rows_kernel(LoraArgs g) {
     }
 }
 
+// Small projections: both products in one launch. A workgroup takes 128 outputs of a unit, 16 a wave, and forms all of
+// the unit's t for itself: the waves' shares of the columns meet in LDS as the second product's operands. y and B are on their way
+// beside A. Bound by latency (one row, 576 x 576, rank 8, f16: 4.6 us, in two launches 8.1).
+template <class T, int RB>
+__global__ void __launch_bounds__(64 * kWaves) lora_small_kernel(LoraArgs g) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j16 = lane & 15, g4 = lane >> 4;
+    __shared__ v4f sums[kWaves][RB][64];
+    Rows64<1> rows;
+    const int units = rows.load(g, 0, lane);
+    const int from = wave * g.steps + min(wave, g.more), n = g.steps + (wave < g.more ? 1 : 0);
+    // lane: output n of the rows 4 g4 .. + 3 (behind the rows: the last one's, not stored)
+    const int out = (blockIdx.x * kWaves + wave) * 16 + j16, nb = min(out, g.rows - 1);
+    for (int at = blockIdx.y; at < units; at += gridDim.y) {
+        Unit u;
+        rows.unit(0, lane, at, &u);
+        if (u.rank == 0 && g.dst == g.y) continue;
+        size_t to[4];
+        float y[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            to[r] = (size_t)u.row(4 * g4 + r) * g.rows + nb;
+            y[r] = g.y[to[r]];
+        }
+        if (u.rank > 0) {
+            constexpr int kLane = Eight<T>::kLane;
+            const int rows64 = (g.rows + 63) & ~63;
+            const T *b = (const T *)g.b + (size_t)u.slot * rows64 * g.stride;
+            v4f bv[RB], acc[RB] = {};
+            int arow[RB];
+#pragma unroll
+            for (int t = 0; t < RB; t++) {
+                bv[t] = four(b + b_at(nb, min(16 * t + 4 * g4, g.stride - 4), g.stride));
+                arow[t] = min(16 * t + j16, u.rank - 1) * g.cols;
+            }
+            columns<T, RB>(g.x + (size_t)u.row(j16) * g.cols + kLane * g4,
+                           (const T *)g.a + (size_t)u.slot * g.max_rank * g.cols + kLane * g4, arow, from, n, acc);
+#pragma unroll
+            for (int t = 0; t < RB; t++) sums[wave][t][lane] = acc[t];
+            __syncthreads();
+            v4f d = {};
+#pragma unroll
+            for (int t = 0; t < RB; t++) {
+                // lane: its row's ranks k .. + 3, as the product takes them
+                v4f tv = sums[0][t][lane];
+#pragma unroll
+                for (int w = 1; w < kWaves; w++) tv += sums[w][t][lane];
+                const int k = 16 * t + 4 * g4;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const bool in = k + j < u.rank;
+                    d = __builtin_amdgcn_mfma_f32_16x16x4f32(in ? tv[j] * u.scale : 0.0f, in ? bv[t][j] : 0.0f, d, 0, 0, 0);
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 4; r++) y[r] += d[r];
+            __syncthreads();  // before the next unit's sums
+        }
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+            if (4 * g4 + r < u.count && out < g.rows) g.dst[to[r]] = y[r];
+    }
+}
+
 // The parts of t, added up into the first one.
 __global__ void __launch_bounds__(256) lora_sum_kernel(float *t, int64_t n4, int splits) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -543,6 +613,26 @@ Plan plan(const LoraArgs &g) {
     return p;
 }
 
+// Both products in one launch: as long as few columns make every workgroup's own t cheap (its columns are a few steps of
+// eight waves) and all of them together read little of the adapters from the caches (2048 x 2048, rank 16, f16, us: one
+// row 6.6, in two launches 4.0 + 3.6; 32 rows on 8 adapters 8.3, 4.5 + 4.3).
+bool small(const LoraArgs &g, const Plan &p, int elem) {
+    return p.mt == 1 && g.max_rank <= 64 && g.cols <= 2048 &&
+           (int64_t)p.most * ((g.rows + 127) / 128) * g.max_rank * g.cols * elem <= (32 << 20);
+}
+
+template <class T>
+sllm_status launch_small(LoraArgs g, const Plan &p, hipStream_t s) {
+    g.steps = g.cols / kStep / kWaves;
+    g.more = g.cols / kStep % kWaves;
+    const dim3 grid((g.rows + 16 * kWaves - 1) / (16 * kWaves), p.most), wg(64 * kWaves);
+    if (g.max_rank <= 16) hipLaunchKernelGGL((lora_small_kernel<T, 1>), grid, wg, 0, s, g);
+    else if (g.max_rank <= 32) hipLaunchKernelGGL((lora_small_kernel<T, 2>), grid, wg, 0, s, g);
+    else hipLaunchKernelGGL((lora_small_kernel<T, 4>), grid, wg, 0, s, g);
+    SLLM_HIP(hipGetLastError());
+    return SLLM_OK;
+}
+
 template <class T, int MT>
 sllm_status launch_rows(LoraArgs g, const Plan &p, hipStream_t s) {
     // A workgroup for every unit there can be, or (prompts) one for all of 64 rows: they come together, so that 64 have
@@ -584,6 +674,7 @@ sllm_status launch_rows(LoraArgs g, const Plan &p, hipStream_t s) {
 
 template <class T>
 sllm_status launch(const LoraArgs &g, const Plan &p, hipStream_t s) {
+    if (small(g, p, sizeof(T))) return launch_small<T>(g, p, s);
     return p.mt > 1 ? launch_rows<T, 4>(g, p, s) : launch_rows<T, 1>(g, p, s);
 }
 
@@ -707,8 +798,10 @@ sllm_status sllm_lora_add_dev(const sllm_lora_set *set, const float *x, int x_ro
     hipStream_t s = (hipStream_t)stream;
     const size_t parts = (size_t)p.splits * x_rows * g.stride * sizeof(float);
     const size_t groups = (((size_t)p.tiles + 3) / 4 * 4 + (size_t)p.tiles * p.most * kGroup) * sizeof(int);
-    const sllm_status st = stream_workspace(s, parts + groups, &ws, &cap);
-    if (st != SLLM_OK) return st;
+    if (!small(g, p, set->elem())) {
+        const sllm_status st = stream_workspace(s, parts + groups, &ws, &cap);
+        if (st != SLLM_OK) return st;
+    }
     g.t = (float *)ws;
     g.groups = (int *)((char *)ws + parts);
     if (set->type == SLLM_LORA_F32) return launch<float>(g, p, s);
