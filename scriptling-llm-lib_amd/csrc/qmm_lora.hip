@@ -487,14 +487,28 @@ __global__ void __launch_bounds__(64 * kWaves) lora_small_kernel(LoraArgs g) {
     }
 }
 
-// The parts of t, added up into the first one.
-__global__ void __launch_bounds__(256) lora_sum_kernel(float *t, int64_t n4, int splits) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+// The parts of t, added up into the first one. Bound by latency: a wave a workgroup, 16 parts' loads under way.
+__global__ void __launch_bounds__(64) lora_sum_kernel(float *t, int64_t n4, int splits) {
+    const int64_t i = (int64_t)blockIdx.x * 64 + threadIdx.x;
     if (i >= n4) return;
     v4f *p = (v4f *)t + i;
-    v4f v = *p;
-#pragma unroll 8
-    for (int s = 1; s < splits; s++) v += p[s * n4];
+    v4f v = {};
+    int s = 0;
+    for (; s + 16 <= splits; s += 16) {
+        v4f x[16];
+#pragma unroll
+        for (int j = 0; j < 16; j++) x[j] = p[(s + j) * n4];
+#pragma unroll
+        for (int j = 0; j < 16; j++) v += x[j];
+    }
+    if (s < splits) {
+        v4f x[16];
+#pragma unroll
+        for (int j = 0; j < 16; j++) x[j] = p[min(s + j, splits - 1) * n4];
+#pragma unroll
+        for (int j = 0; j < 16; j++)
+            if (s + j < splits) v += x[j];
+    }
     *p = v;
 }
 
@@ -653,7 +667,7 @@ sllm_status launch_rows(LoraArgs g, const Plan &p, hipStream_t s) {
     SLLM_HIP(hipGetLastError());
     if (g.splits > 1 && g.splits != (MT == 1 ? kParts : 1)) {
         const int64_t n4 = (int64_t)g.x_rows * g.stride / 4;
-        hipLaunchKernelGGL(lora_sum_kernel, dim3((unsigned)((n4 + 255) / 256)), dim3(256), 0, s, g.t, n4, g.splits);
+        hipLaunchKernelGGL(lora_sum_kernel, dim3((unsigned)((n4 + 63) / 64)), dim3(64), 0, s, g.t, n4, g.splits);
         SLLM_HIP(hipGetLastError());
     }
     constexpr int wide = 4 * 16 * 4, narrow = wide / 4;
