@@ -651,7 +651,7 @@ template <class T, int MT>
 sllm_status launch_rows(LoraArgs g, const Plan &p, hipStream_t s) {
     // A workgroup for every unit there can be, or (prompts) one for all of 64 rows: they come together, so that 64 have
     // little more than one unit, and two of 32 rows take no more products than one of 64. (Workgroups that may find
-    // nothing cost more than that: 700 rows of 3 adapters, f32, rank 64: 49 us with four for 64 rows.)
+    // nothing cost more than that: 700 rows of 3 adapters, f32, rank 64, us: 49 with four for 64 rows, 41 with one, in a kernel of this kind.)
     const int grid = eights(p.tiles * p.splits);
     if constexpr (MT == 1) {
         const dim3 down(grid, p.most), wg(64 * kWaves);
@@ -671,7 +671,7 @@ sllm_status launch_rows(LoraArgs g, const Plan &p, hipStream_t s) {
         SLLM_HIP(hipGetLastError());
     }
     constexpr int wide = 4 * 16 * 4, narrow = wide / 4;
-    const int groups = MT == 1 ? p.most : std::min(p.most, 4);
+    const int groups = MT == 1 ? p.most : std::min(p.most, 8);  // (that case in all, us: 46.9 with 2, 43.9 with 4, 43.0)
     const bool many = (int64_t)p.tiles * groups * ((g.rows + wide - 1) / wide) >= kCUs;
     g.chunks = many ? (g.rows + wide - 1) / wide : (g.rows + narrow - 1) / narrow;
     const dim3 up(eights(p.tiles * g.chunks), groups);

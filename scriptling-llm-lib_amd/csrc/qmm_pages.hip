@@ -57,7 +57,7 @@ __global__ void __launch_bounds__(256) page_copy_kernel(CopyJobs jobs, char *poo
 }
 
 // A small step, by value: a copy from staging memory and the event that guards it cost the host more (4 beams' fork,
-// rows and end: 22.4 us with it, @ with this).
+// rows and end: 22.4 us with it, 20.1 with this; 53 and 30 when each is waited for).
 constexpr int kSmallStep = 960;  // ints
 struct SmallStep {
     int v[kSmallStep];
