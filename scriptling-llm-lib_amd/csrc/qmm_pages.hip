@@ -10,6 +10,7 @@
 
 #include <algorithm>
 #include <cstring>
+#include <functional>
 #include <new>
 #include <string>
 #include <unordered_map>
@@ -234,11 +235,29 @@ constexpr int kLeastTiles = 4;     // of a piece: one for every wave
 
 constexpr int kSpareStates = 8192; // of a kv head, beyond what a step's rows need in one piece each
 
-// The segments' blocks and pieces: every piece about as many tiles as a share of all the step's, or a little more where
-// that lets all workgroups run at a time (16 ragged sequences, f32: 35.0 us with 560 workgroups, 32.4 with the fewer
-// ones; 5 prompts: 60.6, 56.2), and no more states than the batch has room for. Returns the number of pieces (for one
-// kv head).
-int cut(Plan *plan, int rep, int n_kv, const int *most, int slots) {
+// How long a piece takes (us), roughly: a tile's bytes or products at a workgroup's share of what the card reaches
+// when all workgroups run, and what a piece costs beside its tiles.
+struct PieceCost {
+    double tile[3];  // by shape
+    double piece = 4.5;
+    double state;    // one row's state of all kv heads, written and read
+    PieceCost(const PageCache &c, const int *most) {
+        const double read = 6.0e6, f16 = 0.4e9, f32 = 0.1e9;  // bytes, operations in a us
+        for (int i = 0; i < 3; i++) {
+            const double bytes = 2.0 * kPieceTile * c.d_k * c.elem(), ops = 4.0 * kPieceTile * c.d_k * most[i];
+            tile[i] = std::max(i ? 0.0 : bytes / read, ops / (c.elem() == 2 ? f16 : f32)) * kTargetPieces;
+        }
+        state = 8.0 * (c.d_k + 2) * c.n_kv / read;
+    }
+};
+
+// The segments' blocks and pieces: of a few lengths around a share of all the step's tiles the one whose pieces, taken by
+// workgroups one after the other, are estimated to end first; and no more states than the batch has room for. Returns
+// the number of pieces (for one kv head). (32 / 8 heads of 128; the longest share that all workgroups take at once, and
+// so chosen, us: f32, 64 sequences on a prefix of 4000 85.7, 70.8; 16 on 8000 48.8, 44.9; 5 prompts of 211 rows 161,
+// 147; f16, the 64 39.3, 35.2; others within 1. The estimates take the host 4 us for 16 sequences.)
+int cut(const PageCache &c, Plan *plan, int rep, int slots) {
+    const int *most = kShapeRows[shape_class(c.d_k, c.type == SLLM_CACHE_F16)], n_kv = c.n_kv;
     int64_t all = 0;
     for (Segment &s : plan->segs) {
         const int64_t nv = (int64_t)s.ntok * rep;
@@ -263,10 +282,35 @@ int cut(Plan *plan, int rep, int n_kv, const int *most, int slots) {
         return items;
     };
     const int64_t share = std::max<int64_t>(kLeastTiles, (all * n_kv + kTargetPieces - 1) / kTargetPieces);
+    const PieceCost cost(c, most);
+    std::vector<double> busy;
+    auto estimate = [&] {
+        busy.assign((size_t)std::max(1, kTargetPieces / n_kv), 0.0);  // a heap, the first to be free on top
+        double end = 0.0;
+        for (const Segment &s : plan->segs)
+            for (int i = 0; i < s.pieces; i++) {
+                const int n = (std::min(s.p1, s.p0 + (i + 1) * s.piece) - s.p0 - i * s.piece + kPieceTile - 1) / kPieceTile;
+                const double t = cost.piece + n * cost.tile[s.shape];
+                for (int k = 0; k < s.ntok; k += s.block) {
+                    std::pop_heap(busy.begin(), busy.end(), std::greater<>());
+                    end = std::max(end, busy.back() += t);
+                    std::push_heap(busy.begin(), busy.end(), std::greater<>());
+                }
+            }
+        return end + (double)used * cost.state;
+    };
     int64_t tiles = share;
-    while (tiles < 2 * share && pieces(tiles) * n_kv > kTargetPieces) tiles++;
+    double best = -1.0;
+    for (const int64_t eighths : {4, 5, 6, 7, 8, 9, 10, 11, 12, 14, 16, 20}) {
+        const int64_t t = std::max<int64_t>(kLeastTiles, share * eighths / 8);
+        pieces(t);
+        if (used > slots) continue;
+        const double e = estimate();
+        if (best >= 0.0 && e >= best) continue;
+        best = e;
+        tiles = t;
+    }
     int64_t items = pieces(tiles);
-    if (items * n_kv > kTargetPieces) items = pieces(tiles = share);
     // (with one piece each the states fit: kMaxParts for every row)
     while (used > slots) items = pieces(tiles *= 2);
     return (int)items;
@@ -658,7 +702,7 @@ sllm_status sllm_page_batch_begin(sllm_page_batch *batch, const int *seqs, const
         // room for the step on the device and in the next staging slot: header, rows, rows of segments,
         // pieces, tables
         const int64_t most_segs = 2 * (int64_t)count, rep = b.n_heads / c.n_kv;
-        const int64_t most_items = most_segs + kMaxParts * total + 2 * kTargetPieces;
+        const int64_t most_items = most_segs + kMaxParts * total + 3 * kTargetPieces;
         const size_t bytes = (size_t)(kStepHeader + total * (int64_t)(sizeof(StepRow) / 4 + kMaxParts) + 16 * most_items + pages + 32) *
                              sizeof(int);
         if (b.dev_cap < bytes) {
@@ -691,7 +735,7 @@ sllm_status sllm_page_batch_begin(sllm_page_batch *batch, const int *seqs, const
         // (at once: the tables name the copies from here on, whatever becomes of the rest)
         if ((st = launch_page_copies(c, copies.data(), copies.size(), s)) != SLLM_OK) return st;
         share(c, seqs, rows, row0, std::move(who), 0, 0, &plan);
-        const int n_items = cut(&plan, (int)rep, c.n_kv, kShapeRows[shape_class(c.d_k, c.type == SLLM_CACHE_F16)], b.slots);
+        const int n_items = cut(c, &plan, (int)rep, b.slots);
         int *h = (int *)b.host[slot];
         int at = kStepHeader;
         auto place = [&](int64_t ints) {

@@ -66,7 +66,7 @@ __device__ __forceinline__ void put_q(const PageAttnArgs &a, size_t pair, int d,
 // A workgroup takes heads of one row, LP lanes of four dimensions to a head; the rotation (the same for
 // every head: float32 angle, sine and cosine in 64 bits, as the reference) is formed once in LDS, the first
 // heads' elements loaded before it. Bound by latency: few rows have a workgroup for every 256 / LP heads.
-// (16 rows of 32 + 8 heads of 128, us: one workgroup of eight waves per row, a wave per head 8.2; this 2.7.)
+// (16 rows of 32 + 8 heads of 128, us: one workgroup of eight waves per row, a wave per head 8.2; this 4.0.)
 constexpr int kPrepThreads = 256;
 template <class T, int LP>
 __global__ void __launch_bounds__(kPrepThreads) page_prep_kernel(PageAttnArgs a) {

@@ -159,6 +159,34 @@ def test_on_another_stream_and_in_a_graph(m):
         run(s, ad, ids, rep)
 
 
+@pytest.mark.parametrize("rows,cols,rank", [(130, 544, 12), (300, 4096, 20)])
+def test_more_adapters_than_a_wave_has_lanes(rows, cols, rank):
+    s, ad = make(rows, cols, [rank if i % 5 else 0 for i in range(90)], "f16", 4)
+    rng = np.random.default_rng(rows)
+    for m in (1, 30, 64):
+        run(s, ad, [int(i) for i in rng.permutation(90)[:m]], m)                     # every row another one
+    run(s, ad, [int(i) for i in rng.integers(-2, 92, size=200)], 2, in_place=True)   # up to 64 units of 64 rows
+
+
+def test_calls_on_two_streams_at_once():
+    sets = [make(700, 2176, [16, 24, 3], "bf16", 2), make(130, 512, [9, 40], "f32", 3)]
+    st = [torch.cuda.Stream() for _ in range(2)]
+    g = torch.Generator().manual_seed(1)
+    jobs = []
+    for i in range(24):
+        s, ad = sets[i // 2 % 2]
+        m = (1, 33, 90)[i % 3]
+        ids = [(i + r) % 5 - 1 for r in range(m)]
+        x, y = torch.randn(m, s.cols, generator=g).cuda(), torch.randn(m, s.rows, generator=g).cuda()
+        jobs.append((s, ad, ids, x, y, torch.empty_like(y), torch.tensor(ids, dtype=torch.int32, device="cuda")))
+    torch.cuda.synchronize()
+    for i, (s, ad, ids, x, y, dst, di) in enumerate(jobs):
+        sq.lora_add_dev(s, x.data_ptr(), len(ids), di.data_ptr(), y.data_ptr(), dst.data_ptr(), st[i % 2].cuda_stream)
+    torch.cuda.synchronize()
+    for s, ad, ids, x, y, dst, di in jobs:
+        check(ad, x, y, ids, dst)
+
+
 def test_refusals():
     s, _ = make(64, 128, [4], "f16", 1)
     x = torch.zeros(4096, device="cuda")

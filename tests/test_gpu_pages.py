@@ -527,6 +527,40 @@ def test_bookkeeping_follows_its_rules(page, dt, seed):
                 assert (K == m).all() and (V == m + 1).all()
 
 
+@pytest.mark.parametrize("dt", ["f32", "f16"])
+def test_steps_one_after_the_other_without_waiting(dt):
+    """Steps of one row and of hundreds in turn (more than the batch has staging memory for), nothing waited for between
+    them: the same bits as step by step."""
+    outs = []
+    for wait in (True, False):
+        rng = np.random.default_rng(3)
+        m = Model(8, 2, 64, 32, rng)
+        cache = sq.PageCache(1, 2, 64, 16, 400, dt)
+        batch = sq.PageBatch(cache, 8, 40, 400)
+        st = torch.cuda.Stream()
+        seqs = [cache.add() for _ in range(40)]
+        got, keep = [], []
+        torch.cuda.synchronize()
+        for i in range(14):
+            rows = [1] if i % 3 == 0 else [1] * 40 if i % 3 == 1 else [9 + j % 3 for j in range(30)]
+            n = sum(rows)
+            d = [torch.from_numpy(rng.normal(size=(n, k * 64)).astype(np.float32)).cuda() for k in (8, 2, 2)]
+            out = torch.empty(n, 8 * 64, device="cuda")
+            if wait:
+                torch.cuda.synchronize()
+            else:
+                st.wait_stream(torch.cuda.current_stream())
+            batch.begin(seqs[:len(rows)], rows, st.cuda_stream)
+            sq.page_attention_dev(batch, 0, m.params, *(t.data_ptr() for t in d), out.data_ptr(), st.cuda_stream)
+            got.append(out)
+            keep.append(d)
+        torch.cuda.synchronize()
+        outs.append([o.cpu().numpy() for o in got])
+        assert all(np.isfinite(o).all() for o in outs[-1])
+    for a, b in zip(*outs):
+        assert np.array_equal(a.view(np.uint32), b.view(np.uint32))
+
+
 def test_refused_steps_change_nothing():
     cache = sq.PageCache(1, 2, 64, 16, 4, "f32")
     a, b = cache.add(), cache.add()
