@@ -495,7 +495,8 @@ sllm_status sllm_lora_set_load(sllm_lora_set *set, int slot, int rank, const voi
  * adapters' part in place. Products and sums in fp32. x must be 16-byte aligned.
  * Asynchronous on `stream`; uses the stream's workspace (sllm_workspace_reserve;
  * x_rows x (128 x max_rank + 1024) bytes are enough). A captured call reads ids
- * and adapters as they are at each replay.
+ * and adapters as they are at each replay; replays of graphs that were captured on
+ * one stream share its workspace and must not overlap.
  */
 sllm_status sllm_lora_add_dev(const sllm_lora_set *set, const float *x_dev, int x_rows, const int *ids_dev,
                               const float *y_dev, float *dst_dev, void *stream);

@@ -290,10 +290,10 @@ __device__ __forceinline__ void lds_read(v4u (&d)[2], unsigned a0, unsigned a1) 
                  : "memory");
 }
 __device__ __forceinline__ void lds_read(v4u (&d)[4], unsigned a0) {  // every 1024 bytes (rows of 64)
-    asm volatile("ds_read_b128 %0, %4\n\tds_read_b128 %1, %4 offset:1024\n\tds_read_b128 %2, %4 offset:2048\n\t"
-                 "ds_read_b128 %3, %4 offset:3072\n\ts_waitcnt lgkmcnt(0)"
+    asm volatile("ds_read_b128 %0, %4\n\tds_read_b128 %1, %4 offset:1024\n\tds_read_b128 %2, %5\n\t"
+                 "ds_read_b128 %3, %5 offset:1024\n\ts_waitcnt lgkmcnt(0)"
                  : "=&v"(d[0]), "=&v"(d[1]), "=&v"(d[2]), "=&v"(d[3])
-                 : "v"(a0)
+                 : "v"(a0), "v"(a0 + 2048)
                  : "memory");
 }
 __device__ __forceinline__ void lds_read(v4u (&d)[2], unsigned a0) {
@@ -651,7 +651,8 @@ template <class T, int MT>
 sllm_status launch_rows(LoraArgs g, const Plan &p, hipStream_t s) {
     // A workgroup for every unit there can be, or (prompts) one for all of 64 rows: they come together, so that 64 have
     // little more than one unit, and two of 32 rows take no more products than one of 64. (Workgroups that may find
-    // nothing cost more than that: 700 rows of 3 adapters, f32, rank 64, us: 49 with four for 64 rows, 41 with one, in a kernel of this kind.)
+    // nothing cost more than that: 700 rows of 3 adapters, f32, rank 64, in an earlier form of the kernel, us: 49 with
+    // four for 64 rows, 41 with one.)
     const int grid = eights(p.tiles * p.splits);
     if constexpr (MT == 1) {
         const dim3 down(grid, p.most), wg(64 * kWaves);
