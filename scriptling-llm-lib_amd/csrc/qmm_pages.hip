@@ -239,7 +239,7 @@ constexpr int kSpareStates = 8192; // of a kv head, beyond what a step's rows ne
 // when all workgroups run, and what a piece costs beside its tiles.
 struct PieceCost {
     double tile[3];  // by shape
-    double piece = 4.5;
+    double piece = 4.5, merge = 2.5;
     double state;    // one row's state of all kv heads, written and read
     PieceCost(const PageCache &c, const int *most) {
         const double read = 6.0e6, f16 = 0.4e9, f32 = 0.1e9;  // bytes, operations in a us
@@ -284,28 +284,31 @@ int cut(const PageCache &c, Plan *plan, int rep, int slots) {
     const int64_t share = std::max<int64_t>(kLeastTiles, (all * n_kv + kTargetPieces - 1) / kTargetPieces);
     const PieceCost cost(c, most);
     std::vector<double> busy;
-    auto estimate = [&] {
+    auto estimate = [&](int64_t items) {
+        // fewer workgroups than CUs have more of the card each; a launch merges states where there are any (one row, 130
+        // positions of 9 / 3 heads of 64: 10.0 us in two pieces, 7.9 in one)
+        const double x = (double)items * n_kv / kTargetPieces, load = x >= 0.5 ? 1.0 : std::max(0.27, x);
         busy.assign((size_t)std::max(1, kTargetPieces / n_kv), 0.0);  // a heap, the first to be free on top
         double end = 0.0;
         for (const Segment &s : plan->segs)
             for (int i = 0; i < s.pieces; i++) {
                 const int n = (std::min(s.p1, s.p0 + (i + 1) * s.piece) - s.p0 - i * s.piece + kPieceTile - 1) / kPieceTile;
-                const double t = cost.piece + n * cost.tile[s.shape];
+                const double t = cost.piece + n * load * cost.tile[s.shape];
                 for (int k = 0; k < s.ntok; k += s.block) {
                     std::pop_heap(busy.begin(), busy.end(), std::greater<>());
                     end = std::max(end, busy.back() += t);
                     std::push_heap(busy.begin(), busy.end(), std::greater<>());
                 }
             }
-        return end + (double)used * cost.state;
+        return end + (used ? cost.merge : 0.0) + (double)used * cost.state;
     };
     int64_t tiles = share;
     double best = -1.0;
     for (const int64_t eighths : {4, 5, 6, 7, 8, 9, 10, 11, 12, 14, 16, 20}) {
         const int64_t t = std::max<int64_t>(kLeastTiles, share * eighths / 8);
-        pieces(t);
+        const int64_t n = pieces(t);
         if (used > slots) continue;
-        const double e = estimate();
+        const double e = estimate(n);
         if (best >= 0.0 && e >= best) continue;
         best = e;
         tiles = t;
