@@ -79,6 +79,10 @@ sllm_status guarded(F f) {
     }
 }
 
+struct DeviceFree {
+    void operator()(void *p) const { (void)hipFree(p); }
+};
+
 sllm_status on_device(int device) {
     int dev = 0;
     SLLM_HIP(hipGetDevice(&dev));
@@ -708,18 +712,21 @@ sllm_status sllm_page_batch_begin(sllm_page_batch *batch, const int *seqs, const
         const int64_t most_items = most_segs + kMaxParts * total + 3 * kTargetPieces;
         const size_t bytes = (size_t)(kStepHeader + total * (int64_t)(sizeof(StepRow) / 4 + kMaxParts) + 16 * most_items + pages + 32) *
                              sizeof(int);
-        if (b.dev_cap < bytes) {
+        // (a larger buffer takes the old one's place once nothing refuses the step any more: until then the step before
+        // it is the batch's, and the old buffer holds it)
+        std::unique_ptr<void, DeviceFree> grown;
+        size_t dev_cap = b.dev_cap;
+        if (dev_cap < bytes) {
             if (b.captured)
                 return set_error(SLLM_ERR_SHAPE, "the step has more pages than the batch held when it was captured");
+            b.retired.reserve(b.retired.size() + 1);
             void *p = nullptr;
-            const size_t want = 2 * bytes + 65536;
-            if (hipMalloc(&p, want) != hipSuccess) {
+            dev_cap = 2 * bytes + 65536;
+            if (hipMalloc(&p, dev_cap) != hipSuccess) {
                 (void)hipGetLastError();
                 return set_error(SLLM_ERR_OOM, "page batch allocation failed");
             }
-            if (b.dev) b.retired.push_back(b.dev);
-            b.dev = (int *)p;
-            b.dev_cap = want;
+            grown.reset(p);
         }
         const int slot = b.slot;
         SLLM_HIP(hipEventSynchronize(b.done[slot]));
@@ -727,14 +734,19 @@ sllm_status sllm_page_batch_begin(sllm_page_batch *batch, const int *seqs, const
             if (b.host[slot]) (void)hipHostFree(b.host[slot]);
             b.host[slot] = nullptr;
             b.host_cap[slot] = 0;
-            if (hipHostMalloc((void **)&b.host[slot], b.dev_cap, hipHostMallocDefault) != hipSuccess) {
+            if (hipHostMalloc((void **)&b.host[slot], dev_cap, hipHostMallocDefault) != hipSuccess) {
                 (void)hipGetLastError();
                 return set_error(SLLM_ERR_OOM, "page batch staging allocation failed");
             }
-            b.host_cap[slot] = b.dev_cap;
+            b.host_cap[slot] = dev_cap;
         }
         if ((st = append(c, seqs, rows, count, &copies)) != SLLM_OK) return st;
         b.begun = false;
+        if (grown) {
+            if (b.dev) b.retired.push_back(b.dev);
+            b.dev = (int *)grown.release();
+            b.dev_cap = dev_cap;
+        }
         // (at once: the tables name the copies from here on, whatever becomes of the rest)
         if ((st = launch_page_copies(c, copies.data(), copies.size(), s)) != SLLM_OK) return st;
         share(c, seqs, rows, row0, std::move(who), 0, 0, &plan);
