@@ -91,9 +91,8 @@ sllm_status on_device(int device) {
 }
 
 // The pages that appending rows[i] rows to each sequence takes, and whether there are so
-// many; then the appending: the sequences' tables and lengths, and the copies of shared
-// tail pages.
-sllm_status append(PageCache &c, const int *seqs, const int *rows, int n, std::vector<PageCopy> *copies) {
+// many; all the memory that `append` needs is taken here.
+sllm_status prepare_append(PageCache &c, const int *seqs, const int *rows, int n, std::vector<PageCopy> *copies) {
     std::unordered_map<int, int> lost;  // holders that tail pages lose to copies
     int64_t need = 0;
     for (int i = 0; i < n; i++) {
@@ -117,7 +116,11 @@ sllm_status append(PageCache &c, const int *seqs, const int *rows, int n, std::v
         PageSeq &q = c.seqs[(size_t)seqs[i]];
         if (rows[i]) q.pages.reserve((size_t)(((int64_t)q.len + rows[i] + c.page_rows - 1) >> c.shift));
     }
-    // nothing below allocates
+    return SLLM_OK;
+}
+
+// The appending: the sequences' tables and lengths, and the copies of shared tail pages.
+void append(PageCache &c, const int *seqs, const int *rows, int n, std::vector<PageCopy> *copies) noexcept {
     for (int i = 0; i < n; i++) {
         PageSeq &q = c.seqs[(size_t)seqs[i]];
         if (!rows[i]) continue;
@@ -132,7 +135,6 @@ sllm_status append(PageCache &c, const int *seqs, const int *rows, int n, std::v
         q.len += rows[i];
         while ((int64_t)q.pages.size() < (((int64_t)q.len + c.page_rows - 1) >> c.shift)) q.pages.push_back(c.take());
     }
-    return SLLM_OK;
 }
 
 int new_seq(PageCache &c) {
@@ -179,6 +181,7 @@ struct Plan {
 // reading them once more costs less than another state to merge.
 constexpr int kWorthSharing = 128;
 
+// (The plan is made before the step's rows are appended: they change no full page before them.)
 // Sequences `who` (of the step) have page p in common for p < from (their segments up to there
 // are made); what follows is cut into segments: a run of pages that several hold once for all of these, and so
 // on behind it, at most kMaxParts to a sequence.
@@ -186,12 +189,12 @@ void share(const PageCache &c, const int *seqs, const int *rows, const std::vect
            int depth, Plan *plan) {
     auto table = [&](int i) -> const std::vector<int> & { return c.seqs[(size_t)seqs[i]].pages; };
     // full pages before the sequence's first new row: every new row sees all of them
-    auto full = [&](int i) { return (c.seqs[(size_t)seqs[i]].len - rows[i]) >> c.shift; };
+    auto full = [&](int i) { return c.seqs[(size_t)seqs[i]].len >> c.shift; };
     auto own = [&](int i) {
         Segment s;
         s.first = i;
         s.p0 = from << c.shift;
-        s.p1 = c.seqs[(size_t)seqs[i]].len;
+        s.p1 = c.seqs[(size_t)seqs[i]].len + rows[i];
         s.tok0 = (int)plan->tok.size();
         s.ntok = rows[i];
         s.causal = rows[i] > 1;
@@ -524,7 +527,8 @@ sllm_status sllm_page_seq_extend(sllm_page_cache *pc, int seq, int rows, void *s
         if (stream_capturing((hipStream_t)stream))
             return set_error(SLLM_ERR_ARG, "a page cache's sequences cannot change under capture");
         std::vector<PageCopy> copies;
-        if ((st = append(c, &seq, &rows, 1, &copies)) != SLLM_OK) return st;
+        if ((st = prepare_append(c, &seq, &rows, 1, &copies)) != SLLM_OK) return st;
+        append(c, &seq, &rows, 1, &copies);
         return launch_page_copies(c, copies.data(), copies.size(), (hipStream_t)stream);
     });
 }
@@ -696,6 +700,7 @@ sllm_status sllm_page_batch_begin(sllm_page_batch *batch, const int *seqs, const
         if (st != SLLM_OK) return st;
         if (stream_capturing(s)) return set_error(SLLM_ERR_ARG, "a batch's step cannot begin under capture");
         std::vector<PageCopy> copies;
+        if ((st = prepare_append(c, seqs, rows, count, &copies)) != SLLM_OK) return st;
         Plan plan;
         plan.parts.resize((size_t)count);
         plan.tok.reserve((size_t)total * kMaxParts);
@@ -706,9 +711,13 @@ sllm_status sllm_page_batch_begin(sllm_page_batch *batch, const int *seqs, const
             r0 += rows[i];
             if (rows[i]) who.push_back(i);
         }
+        const int64_t rep = b.n_heads / c.n_kv;
+        share(c, seqs, rows, row0, std::move(who), 0, 0, &plan);
+        const int n_items = cut(c, &plan, (int)rep, b.slots);
+        std::vector<int> table((size_t)count, -1);  // of the sequences that segments read
         // room for the step on the device and in the next staging slot: header, rows, rows of segments,
         // pieces, tables
-        const int64_t most_segs = 2 * (int64_t)count, rep = b.n_heads / c.n_kv;
+        const int64_t most_segs = 2 * (int64_t)count;
         const int64_t most_items = most_segs + kMaxParts * total + 3 * kTargetPieces;
         const size_t bytes = (size_t)(kStepHeader + total * (int64_t)(sizeof(StepRow) / 4 + kMaxParts) + 16 * most_items + pages + 32) *
                              sizeof(int);
@@ -740,7 +749,8 @@ sllm_status sllm_page_batch_begin(sllm_page_batch *batch, const int *seqs, const
             }
             b.host_cap[slot] = dev_cap;
         }
-        if ((st = append(c, seqs, rows, count, &copies)) != SLLM_OK) return st;
+        // nothing below allocates memory or refuses the step
+        append(c, seqs, rows, count, &copies);
         b.begun = false;
         if (grown) {
             if (b.dev) b.retired.push_back(b.dev);
@@ -749,8 +759,6 @@ sllm_status sllm_page_batch_begin(sllm_page_batch *batch, const int *seqs, const
         }
         // (at once: the tables name the copies from here on, whatever becomes of the rest)
         if ((st = launch_page_copies(c, copies.data(), copies.size(), s)) != SLLM_OK) return st;
-        share(c, seqs, rows, row0, std::move(who), 0, 0, &plan);
-        const int n_items = cut(c, &plan, (int)rep, b.slots);
         int *h = (int *)b.host[slot];
         int at = kStepHeader;
         auto place = [&](int64_t ints) {
@@ -763,7 +771,6 @@ sllm_status sllm_page_batch_begin(sllm_page_batch *batch, const int *seqs, const
         StepItem *hi = (StepItem *)(h + place(16 * (int64_t)n_items));
         const int tok_at = place((int64_t)plan.tok.size());
         h[kStepRowsAt] = place((int64_t)(sizeof(StepRow) / 4) * total);
-        std::vector<int> table((size_t)count, -1);  // of the sequences that segments read
         StepRow *hr = (StepRow *)(h + h[kStepRowsAt]);
         b.combine = 0;
         for (int i = 0; i < count; i++) {

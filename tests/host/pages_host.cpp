@@ -7,6 +7,23 @@
 #include "qmm_pages.hip"
 
 static std::string error;
+
+// The library's allocations fail one after the other while `news_left` counts down to 0.
+static long news_left = -1;
+static bool news_failed;
+void *operator new(size_t n) {
+    if (news_left == 0) {
+        news_failed = true;
+        throw std::bad_alloc();
+    }
+    if (news_left > 0) news_left--;
+    if (void *p = std::malloc(n ? n : 1)) return p;
+    throw std::bad_alloc();
+}
+void *operator new(size_t n, const std::nothrow_t &) noexcept { return std::malloc(n ? n : 1); }
+void operator delete(void *p) noexcept { std::free(p); }
+void operator delete(void *p, size_t) noexcept { std::free(p); }
+
 static PageAttnArgs last;
 static int launches;
 
@@ -217,10 +234,58 @@ static void refused_begin() {
     }
 }
 
+// Host memory that runs out anywhere in a call: it says so, and nothing has changed.
+template <class Call, class State>
+static void every_allocation_fails(Call call, State state) {
+    const auto before = state();
+    for (long n = 0;; n++) {
+        CHECK(n < 1000);
+        news_failed = false;
+        news_left = n;
+        const sllm_status st = call();
+        news_left = -1;
+        if (!news_failed) {
+            CHECK(st == SLLM_OK);
+            return;
+        }
+        CHECK(st == SLLM_ERR_OOM && state() == before);
+    }
+}
+
+static void out_of_memory() {
+    Cache c(1, 2, 64, 16, 400, 1);
+    Batch b(c, 4, 8, 64);
+    std::vector<int> seqs = {c.add(700)};
+    for (int s : c.fork(seqs[0], 650, 5)) seqs.push_back(s);
+    const std::vector<int> first = {1, 0, 2, 1, 1, 3};
+    run(c, b, seqs, first);
+    auto whole = [&] { return c.state(seqs); };
+    auto step_too = [&] {
+        CHECK(b.attend() == SLLM_OK);
+        check_step(c, seqs, first);
+        return c.state(seqs);
+    };
+    int out[3];
+    every_allocation_fails([&] { return sllm_page_seq_fork(c.c, seqs[1], 333, 3, out); }, whole);
+    every_allocation_fails([&] { return sllm_page_seq_copy(c.c, seqs[1], 333, 3, out, nullptr); }, whole);
+    every_allocation_fails([&] { return sllm_page_seq_extend(c.c, out[0], 99, nullptr); }, whole);
+    std::vector<int> grown;
+    for (int s : seqs) grown.push_back(s);
+    const std::vector<int> rows = {1, 3, 2, 20, 1, 3};
+    every_allocation_fails([&] { return sllm_page_batch_begin(b.b, grown.data(), rows.data(), 6, nullptr); }, step_too);
+    CHECK(b.attend() == SLLM_OK);
+    check_step(c, seqs, rows);
+    every_allocation_fails([&] { return sllm_page_seq_free(c.c, seqs.data() + 1, 2); }, whole);
+    seqs = {seqs[0], seqs[3], seqs[4], seqs[5]};
+    every_allocation_fails([&] { return sllm_page_cache_compact(c.c, nullptr, nullptr); }, whole);
+    run(c, b, seqs, {1, 1, 1, 1});
+}
+
 int main(int argc, char **argv) {
     const std::string what = argc > 1 ? argv[1] : "";
     if (what == "steps") steps();
     else if (what == "refused_begin") refused_begin();
+    else if (what == "out_of_memory") out_of_memory();
     else return 2;
     std::puts("ok");
     return 0;
