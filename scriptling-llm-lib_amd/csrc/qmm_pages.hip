@@ -137,6 +137,22 @@ void append(PageCache &c, const int *seqs, const int *rows, int n, std::vector<P
     }
 }
 
+// `append` undone, with the copies that it asked for: pages that it took are vacant again, shared tail pages held again.
+void take_back(PageCache &c, const int *seqs, const int *rows, int n, std::vector<PageCopy> *copies) noexcept {
+    for (int i = n - 1; i >= 0; i--) {
+        if (!rows[i]) continue;
+        PageSeq &q = c.seqs[(size_t)seqs[i]];
+        q.len -= rows[i];
+        for (; (int64_t)q.pages.size() > (((int64_t)q.len + c.page_rows - 1) >> c.shift); q.pages.pop_back()) c.drop(q.pages.back());
+        if (copies->empty() || q.pages.empty() || q.pages.back() != copies->back().dst) continue;
+        c.drop(q.pages.back());
+        q.pages.back() = copies->back().src;
+        c.refs[(size_t)q.pages.back()]++;
+        q.version--;
+        copies->pop_back();
+    }
+}
+
 int new_seq(PageCache &c) {
     if (!c.spare.empty()) {
         const int s = c.spare.back();
@@ -511,7 +527,9 @@ sllm_status sllm_page_seq_copy(sllm_page_cache *pc, int seq, int rows, int count
             return set_error(SLLM_ERR_ARG, "a page cache's sequences cannot change under capture");
         std::vector<PageCopy> copies;
         if ((st = duplicate(c, seq, rows, count, out, &copies)) != SLLM_OK) return st;
-        return launch_page_copies(c, copies.data(), copies.size(), (hipStream_t)stream);
+        if ((st = launch_page_copies(c, copies.data(), copies.size(), (hipStream_t)stream)) != SLLM_OK)
+            for (int i = count - 1; i >= 0; i--) end_seq(c, out[i]);
+        return st;
     });
 }
 
@@ -529,7 +547,9 @@ sllm_status sllm_page_seq_extend(sllm_page_cache *pc, int seq, int rows, void *s
         std::vector<PageCopy> copies;
         if ((st = prepare_append(c, &seq, &rows, 1, &copies)) != SLLM_OK) return st;
         append(c, &seq, &rows, 1, &copies);
-        return launch_page_copies(c, copies.data(), copies.size(), (hipStream_t)stream);
+        if ((st = launch_page_copies(c, copies.data(), copies.size(), (hipStream_t)stream)) != SLLM_OK)
+            take_back(c, &seq, &rows, 1, &copies);
+        return st;
     });
 }
 
@@ -751,14 +771,16 @@ sllm_status sllm_page_batch_begin(sllm_page_batch *batch, const int *seqs, const
         }
         // nothing below allocates memory or refuses the step
         append(c, seqs, rows, count, &copies);
+        if ((st = launch_page_copies(c, copies.data(), copies.size(), s)) != SLLM_OK) {
+            take_back(c, seqs, rows, count, &copies);
+            return st;
+        }
         b.begun = false;
         if (grown) {
             if (b.dev) b.retired.push_back(b.dev);
             b.dev = (int *)grown.release();
             b.dev_cap = dev_cap;
         }
-        // (at once: the tables name the copies from here on, whatever becomes of the rest)
-        if ((st = launch_page_copies(c, copies.data(), copies.size(), s)) != SLLM_OK) return st;
         int *h = (int *)b.host[slot];
         int at = kStepHeader;
         auto place = [&](int64_t ints) {

@@ -281,11 +281,48 @@ static void out_of_memory() {
     run(c, b, seqs, {1, 1, 1, 1});
 }
 
+// Copies that can't be launched: the call says so, and its sequences, their pages and the step before it are as they were.
+static void failed_copies() {
+    Cache c(1, 2, 64, 16, 900, 1);
+    Batch b(c, 4, 8, 64);
+    std::vector<int> seqs = {c.add(700)};
+    for (int s : c.fork(seqs[0], 650, 5)) seqs.push_back(s);
+    for (int s : c.fork(seqs[1], 645, 1)) seqs.push_back(s);
+    const std::vector<int> first = {1, 0, 2, 0, 0, 0, 0};
+    run(c, b, seqs, first);
+    const auto before = c.state(seqs);
+    auto refused = [&](sllm_status st) {
+        stub::launches_left = -1;
+        CHECK(st == SLLM_ERR_DEVICE && c.state(seqs) == before);
+        CHECK(b.attend() == SLLM_OK);
+        check_step(c, seqs, first);
+    };
+    int out[9];
+    stub::launches_left = 1;  // (the second of two)
+    refused(sllm_page_seq_copy(c.c, seqs[1], 650, 9, out, nullptr));
+    stub::launches_left = 0;
+    refused(sllm_page_seq_extend(c.c, seqs[3], 50, nullptr));
+    stub::launches_left = 0;
+    refused(b.begin(seqs, {1, 1, 1, 20, 1, 1, 30}));
+    stub::launches_left = 0;
+    refused(sllm_page_seq_extend(c.c, seqs[6], 50, nullptr));
+    stub::launches_left = 0;
+    CHECK(sllm_page_seq_free(c.c, seqs.data() + 3, 1) == SLLM_OK);
+    seqs.erase(seqs.begin() + 3);
+    const auto gap = c.state(seqs);
+    CHECK(sllm_page_cache_compact(c.c, nullptr, nullptr) == SLLM_OK);  // (nothing to move)
+    stub::launches_left = -1;
+    CHECK(c.state(seqs) == gap);
+    run(c, b, seqs, {1, 1, 1, 1, 1, 30});
+    CHECK(c.add() == 3 && c.add() == 7);  // numbers of sequences that were not made are free
+}
+
 int main(int argc, char **argv) {
     const std::string what = argc > 1 ? argv[1] : "";
     if (what == "steps") steps();
     else if (what == "refused_begin") refused_begin();
     else if (what == "out_of_memory") out_of_memory();
+    else if (what == "failed_copies") failed_copies();
     else return 2;
     std::puts("ok");
     return 0;
