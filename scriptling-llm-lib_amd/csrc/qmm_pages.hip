@@ -297,7 +297,7 @@ int cut(const PageCache &c, Plan *plan, int rep, int slots) {
             const int64_t n = (s.p1 - s.p0 + kPieceTile - 1) / kPieceTile;
             s.pieces = (int)((n + tiles - 1) / tiles);
             s.piece = (int)((n + s.pieces - 1) / s.pieces) * kPieceTile;
-            s.pieces = (s.p1 - s.p0 + s.piece - 1) / s.piece;
+            s.pieces = (int)(((int64_t)s.p1 - s.p0 + s.piece - 1) / s.piece);
             s.slot = (int)used;
             if (!(s.lone && s.pieces == 1)) used += (int64_t)s.pieces * s.ntok * rep;
             items += (int64_t)s.pieces * ((s.ntok + s.block - 1) / s.block);
@@ -315,7 +315,7 @@ int cut(const PageCache &c, Plan *plan, int rep, int slots) {
         double end = 0.0;
         for (const Segment &s : plan->segs)
             for (int i = 0; i < s.pieces; i++) {
-                const int n = (std::min(s.p1, s.p0 + (i + 1) * s.piece) - s.p0 - i * s.piece + kPieceTile - 1) / kPieceTile;
+                const int at = s.p0 + i * s.piece, n = (std::min(s.p1 - at, s.piece) + kPieceTile - 1) / kPieceTile;
                 const double t = cost.piece + n * load * cost.tile[s.shape];
                 for (int k = 0; k < s.ntok; k += s.block) {
                     std::pop_heap(busy.begin(), busy.end(), std::greater<>());
@@ -716,6 +716,13 @@ sllm_status sllm_page_batch_begin(sllm_page_batch *batch, const int *seqs, const
             pages += ((int64_t)c.seqs[(size_t)seqs[i]].len + rows[i] + c.page_rows - 1) >> c.shift;
         }
         if (total > b.max_rows) return set_error(SLLM_ERR_SHAPE, "more rows than max_rows");
+        // room for the step on the device and in the next staging slot: header, rows, rows of segments,
+        // pieces, tables
+        const int64_t most_segs = 2 * (int64_t)count;
+        const int64_t most_items = most_segs + kMaxParts * total + 3 * kTargetPieces;
+        const int64_t ints = kStepHeader + total * (int64_t)(sizeof(StepRow) / 4 + kMaxParts) + 16 * most_items + pages + 32;
+        if (ints > INT32_MAX) return set_error(SLLM_ERR_SHAPE, "the step has too many rows and pages (offsets of 32 bits)");
+        const size_t bytes = (size_t)ints * sizeof(int);
         sllm_status st = on_device(c.device);
         if (st != SLLM_OK) return st;
         if (stream_capturing(s)) return set_error(SLLM_ERR_ARG, "a batch's step cannot begin under capture");
@@ -735,12 +742,6 @@ sllm_status sllm_page_batch_begin(sllm_page_batch *batch, const int *seqs, const
         share(c, seqs, rows, row0, std::move(who), 0, 0, &plan);
         const int n_items = cut(c, &plan, (int)rep, b.slots);
         std::vector<int> table((size_t)count, -1);  // of the sequences that segments read
-        // room for the step on the device and in the next staging slot: header, rows, rows of segments,
-        // pieces, tables
-        const int64_t most_segs = 2 * (int64_t)count;
-        const int64_t most_items = most_segs + kMaxParts * total + 3 * kTargetPieces;
-        const size_t bytes = (size_t)(kStepHeader + total * (int64_t)(sizeof(StepRow) / 4 + kMaxParts) + 16 * most_items + pages + 32) *
-                             sizeof(int);
         // (a larger buffer takes the old one's place once nothing refuses the step any more: until then the step before
         // it is the batch's, and the old buffer holds it)
         std::unique_ptr<void, DeviceFree> grown;
@@ -827,7 +828,7 @@ sllm_status sllm_page_batch_begin(sllm_page_batch *batch, const int *seqs, const
                     StepItem x;
                     x.table = t;
                     x.p0 = s.p0 + i * s.piece;
-                    x.p1 = std::min(s.p1, x.p0 + s.piece);
+                    x.p1 = x.p0 + std::min(s.p1 - x.p0, s.piece);
                     x.ntok = std::min(s.block, s.ntok - k);
                     const int *tk = plan.tok.data() + s.tok0 + k;
                     bool run = true;

@@ -317,12 +317,28 @@ static void failed_copies() {
     CHECK(c.add() == 3 && c.add() == 7);  // numbers of sequences that were not made are free
 }
 
+// Sequences up to the longest, whose pieces end next to what 32 bits hold.
+static void long_sequences() {
+    const int longest = INT32_MAX - 512;
+    for (int rows : {longest - 40, longest - 4000000, longest / 2 + 77})
+        for (int type = 0; type < 2; type++) {
+            Cache c(1, 1, 8, 256, 1 << 23, type);
+            Batch b(c, 1, 2, 64);
+            const int s = c.add(rows);
+            run(c, b, {s}, {1});
+            run(c, b, {s}, {30});
+            run(c, b, c.fork(s, rows, 2), {1, 2});
+            CHECK(sllm_page_seq_extend(c.c, s, longest - rows, nullptr) == SLLM_ERR_SHAPE);
+        }
+}
+
 int main(int argc, char **argv) {
     const std::string what = argc > 1 ? argv[1] : "";
     if (what == "steps") steps();
     else if (what == "refused_begin") refused_begin();
     else if (what == "out_of_memory") out_of_memory();
     else if (what == "failed_copies") failed_copies();
+    else if (what == "long_sequences") long_sequences();
     else return 2;
     std::puts("ok");
     return 0;
