@@ -437,7 +437,7 @@ sllm_status sllm_page_cache_compact(sllm_page_cache *pc, int *used, void *stream
 /*
  * The steps of up to max_seqs sequences at a time, max_rows rows in all, for
  * a model of n_heads query heads (n_kv_heads x 1..8); max_rows x n_heads x d_k
- * at most 2^28 (SLLM_ERR_SHAPE). A batch owns the device memory that its
+ * at most 2^28, max_rows x n_heads below 2^24 (SLLM_ERR_SHAPE). A batch owns the device memory that its
  * attention calls need, so those allocate nothing.
  * sllm_page_batch_begin begins a step: rows[i] (0: none) rows are appended to
  * sequence seqs[i] (each named once), pages taken and shared tail pages copied;

@@ -669,6 +669,8 @@ sllm_status sllm_page_batch_create(sllm_page_cache *pc, int n_heads, int max_seq
     // the kernels address a row's q, output and states with 32 bits
     if ((int64_t)max_rows * n_heads * c.d_k > (1 << 28))
         return set_error(SLLM_ERR_SHAPE, "max_rows x n_heads x d_k must be at most 2^28");
+    // a launch has fewer than 2^32 threads: the merge 256 for every row and head
+    if ((int64_t)max_rows * n_heads >= 1 << 24) return set_error(SLLM_ERR_SHAPE, "max_rows x n_heads must be below 2^24");
     return guarded([&]() -> sllm_status {
         sllm_status st = on_device(c.device);
         if (st != SLLM_OK) return st;
@@ -932,7 +934,8 @@ sllm_status sllm_page_attention_dev(sllm_page_batch *batch, int layer, const sll
     a.grid_rows = capture ? b.max_rows : b.rows;
     a.wide = capture || b.wide;
     a.items = capture ? -1 : b.items * c.n_kv;
-    a.grid_items = capture ? 2 * kTargetPieces : b.items * c.n_kv;
+    // (workgroups take pieces one after the other where there are more than those of a launch of 2^31 threads)
+    a.grid_items = capture ? 2 * kTargetPieces : std::min(b.items * c.n_kv, 1 << 23);
     a.combine = capture ? INT32_MAX : b.combine;
     a.type = c.type;
     b.captured |= capture;

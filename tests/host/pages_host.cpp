@@ -332,6 +332,27 @@ static void long_sequences() {
         }
 }
 
+// Batches of more rows and heads than a launch can have threads for are refused; the largest are made.
+static void many_rows() {
+    for (int dk : {8, 16, 24}) {
+        Cache c(1, 1, dk, 16, 4, 1);
+        sllm_page_batch *b = nullptr;
+        for (int heads : {1, 8}) {
+            CHECK(sllm_page_batch_create(c.c, heads, 1, (1 << 24) / heads, &b) == SLLM_ERR_SHAPE && !b);
+            const int most = std::min((1 << 24) / heads - 1, (1 << 28) / heads / dk);
+            CHECK(sllm_page_batch_create(c.c, heads, 1, most, &b) == SLLM_OK);
+            sllm_page_batch_destroy(b);
+        }
+    }
+    // more pieces than workgroups: a row each of many sequences, for many kv heads
+    Cache c(1, 3000, 8, 16, 4000, 1);
+    Batch b(c, 3000, 3000, 3000);
+    std::vector<int> seqs, rows(3000, 1);
+    for (int i = 0; i < 3000; i++) seqs.push_back(c.add(0));
+    run(c, b, seqs, rows);
+    CHECK((uint64_t)last.grid_items * 256 >> 32 == 0 && last.items == 3000 * 3000);
+}
+
 int main(int argc, char **argv) {
     const std::string what = argc > 1 ? argv[1] : "";
     if (what == "steps") steps();
@@ -339,6 +360,7 @@ int main(int argc, char **argv) {
     else if (what == "out_of_memory") out_of_memory();
     else if (what == "failed_copies") failed_copies();
     else if (what == "long_sequences") long_sequences();
+    else if (what == "many_rows") many_rows();
     else return 2;
     std::puts("ok");
     return 0;

@@ -49,7 +49,7 @@ def test_a_refused_step_leaves_the_one_before_it():
 def test_a_sequence_next_to_the_longest():
     """2^31 - 1000 rows, a page table of 8 million entries: every score is 0, so each output is the mean of V. V is 1, and 2
     in the last 3 million rows (a part of the last piece): the waves' sums are whole numbers below 2^24 and exact; the
-    merge of up to 640 pieces rounds twice for each, the sums of values and of weights, and a few times behind it."""
+    merge of 205 pieces rounds twice for each, the sums of values and of weights, and a few times behind it."""
     rows, more = 2 ** 31 - 1000, 3_000_000
     cache = sq.PageCache(1, 1, 8, 256, (2 ** 31 - 512) // 256 + 1, "f16")
     pools = Pools(cache, fill=0.0)
@@ -66,4 +66,4 @@ def test_a_sequence_next_to_the_longest():
     for r in range(3):
         n = rows + r + 1
         want = (n + more + r + 1) / n
-        assert (np.abs(out[r] - want) <= want * (2 * 640 + 16) * 2.0 ** -24).all(), (r, out[r] - want)
+        assert (np.abs(out[r] - want) <= want * (2 * 205 + 16) * 2.0 ** -24).all(), (r, out[r] - want)

@@ -22,7 +22,7 @@ def program(tmp_path_factory):
     return out
 
 
-@pytest.mark.parametrize("what", ["steps", "refused_begin", "out_of_memory", "failed_copies", "long_sequences"])
+@pytest.mark.parametrize("what", ["steps", "refused_begin", "out_of_memory", "failed_copies", "long_sequences", "many_rows"])
 def test_host_code(program, what):
     res = subprocess.run([program, what], capture_output=True, text=True, timeout=300)
     assert res.returncode == 0, res.stderr[-2000:]
