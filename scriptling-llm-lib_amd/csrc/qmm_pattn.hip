@@ -21,6 +21,7 @@ namespace {
 constexpr int kMaxDk = 256;
 typedef float v2f __attribute__((ext_vector_type(2)));
 typedef float v4f __attribute__((ext_vector_type(4)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef _Float16 v4h __attribute__((ext_vector_type(4)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef unsigned v2u __attribute__((ext_vector_type(2)));
@@ -36,8 +37,9 @@ __device__ __forceinline__ void put4(_Float16 *dst, v4f x) {
 }
 
 // A rotated q head (row pair of a.qrot: d_k floats) as the attention takes it. f32: as it is. f16 caches: two f16
-// values for each element, d_k leading parts, then d_k rests (together 22 bits or more of it), of the head times a power of two that
-// puts its largest element between 2^10 and 2^11, so that no float32 leaves f16's range; a.qscale undoes it.
+// values for each element, d_k leading parts, then d_k rests (together within 2^-23 of it or 2^-35 of the head's largest
+// element, whichever is more), of the head times a power of two that puts its largest element between 2^10 and 2^11, so
+// that no float32 leaves f16's range; a.qscale undoes it.
 // LP lanes hold the head, zeros beyond d_k.
 template <class T, int LP>
 __device__ __forceinline__ void put_q(const PageAttnArgs &a, size_t pair, int d, int dk, v4f x) {
@@ -147,17 +149,26 @@ __global__ void __launch_bounds__(kPrepThreads) page_prep_kernel(PageAttnArgs a)
 //   S^T = K Q^T: lane l holds K[position l % 16], dimensions of its quarter q = l / 16;
 //   the result leaves positions 4 q + i in lane quarter q: as B operand of O^T = V^T P^T it
 //     stays where it is, and the quarter reads V rows 4 q + i, every lane a run of dimensions.
-// f16: 32 positions a step; K and V are exact operands, q and the weights go in as two f16 each (22 bits of
-//   them: 2^-22 of the value; the row's q scaled by a power of two, so no float32 leaves f16's range).
+// f16: 32 positions a step; K and V are exact operands, q and the weights go in as two f16 each (the row's q scaled by a
+//   power of two, so no float32 leaves f16's range: put_q).
 // f32: 16 positions a step, fp32 matrix instructions.
-// Softmax weights are 2^(s - m) with m the largest score at the last time that one exceeded it by
-// more than 2^8: while none does, neither the row's lanes have to agree on a maximum nor the
-// sums to be scaled again. Weights stay below 2^8, sums in fp32.
+// Softmax weights are 2^(s - m); m follows the largest score when one exceeds it by more than kTop: while none does,
+// neither the row's lanes have to agree on a maximum nor the sums to be scaled again. Sums are held in fp32.
+// A weight's f16 parts are its nearest f16 and the nearest to what is left: together within 2^-23 of the weight, or, as f16
+// ends, within 2^-25. So that small weights of f16 caches keep their bits too (many keys behind one of a large score), the
+// largest one lies between 2^13 and 2^15, near f16's other end: m is 13 below the largest score when it follows. Then
+// 2^-25 is 2^-38 of the largest weight so far: of a key 14 nats below another 2^-18 at worst (with the largest at 1 and
+// the parts cut off, 7 % were lost). Two binades before m follows again cost no time against eight (64 sequences on a
+// prefix of 4000 37.6 us either way, 5 prompts of 211 rows 58.4 and 58.0).
 // A result that is not finite (a non-finite K or V element, also one that only other rows of the block
 // see, where the matrix instruction forms 0 * inf) is computed again, row by row, as the formula says.
 constexpr int kWaves = 4;
 constexpr int kFewPieces = 8;    // of a row, up to which one group of lanes merges them
-constexpr float kGrow = 8.0f;  // log2 of how far weights may exceed 1
+// log2 of the largest weight when m follows it, and from which on it follows
+template <class T>
+constexpr float kLead = sizeof(T) == 2 ? 13.0f : 0.0f;
+template <class T>
+constexpr float kTop = sizeof(T) == 2 ? 15.0f : 8.0f;
 
 template <int... G, class F>
 __device__ __forceinline__ void each(std::integer_sequence<int, G...>, F f) {
@@ -384,9 +395,9 @@ struct Rows : Shape<T, NB, FULL, VM> {
 #pragma unroll
                 for (int i = 0; i < 4; i++) mx = fmaxf(mx, s[mt][h][i]);
             mx = mx * sc[mt];
-            if (__ballot(mx > m[mt] + kGrow)) {  // from -inf on: any score
+            if (__ballot(mx > m[mt] + kTop<T>)) {  // from -inf on: any score
                 float mn = fmaxf(mx, __shfl_xor(mx, 16, 64));
-                mn = fmaxf(m[mt], fmaxf(mn, __shfl_xor(mn, 32, 64)));
+                mn = fmaxf(m[mt], fmaxf(mn, __shfl_xor(mn, 32, 64)) - kLead<T>);
                 const float alpha = mn == m[mt] ? 1.0f : exp2_(m[mt] - mn);
                 m[mt] = mn;
                 l[mt] = l[mt] * alpha;
@@ -418,10 +429,10 @@ struct Rows : Shape<T, NB, FULL, VM> {
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const float x = s[mt][i / 2][2 * (i & 1)], y = s[mt][i / 2][2 * (i & 1) + 1];
-                    const auto hp = __builtin_amdgcn_cvt_pkrtz(x, y);
+                    const v2h hp = __builtin_convertvector((v2f{x, y}), v2h);
+                    const v2f left = {__builtin_fmaf((float)hp[0], -1.0f, x), __builtin_fmaf((float)hp[1], -1.0f, y)};
                     hi[i] = __builtin_bit_cast(unsigned, hp);
-                    lo[i] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)hp[0], -1.0f, x),
-                                                                                      __builtin_fmaf((float)hp[1], -1.0f, y)));
+                    lo[i] = __builtin_bit_cast(unsigned, __builtin_convertvector(left, v2h));
                 }
                 ph[mt] = __builtin_bit_cast(v8h, hi);
                 pl[mt] = __builtin_bit_cast(v8h, lo);

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import sllm_qmm as sq
-from test_gpu_pages import Model, Pools, batch_of, check_step
+from test_gpu_pages import NP, Model, Pools, attention64, batch_of, check_step
 
 pytestmark = pytest.mark.gpu
 
@@ -67,3 +67,55 @@ def test_a_sequence_next_to_the_longest():
         n = rows + r + 1
         want = (n + more + r + 1) / n
         assert (np.abs(out[r] - want) <= want * (2 * 205 + 16) * 2.0 ** -24).all(), (r, out[r] - want)
+
+
+@pytest.mark.parametrize("gap", [8, 11, 14, 17])
+@pytest.mark.parametrize("dt", ["f32", "f16"])
+@pytest.mark.parametrize("prefix,owns,news", [(0, [450, 300], [1, 1]), (330, [3] * 20, [1] * 20), (200, [1, 30], [70, 20])])
+def test_small_weights_behind_a_large_one(prefix, owns, news, dt, gap):
+    """Position 0's score is `gap` nats above hundreds of others, and its V is small: what those add is most of the
+    output, or a share of it that fp32 holds. Few rows (a workgroup's waves have tiles of their own), rows of 20
+    sequences on a prefix and rows of prompts (tiles for all waves). The values' weights of f16 caches are within 2^-23 of
+    themselves or 2^-38 of the largest: the latter, times |v|, is added to the bounds of test_gpu_pages."""
+    rng = np.random.default_rng(gap)
+    H, KV, dk = 8, 2, 64
+    m = Model(H, KV, dk, 0, rng)
+    cache = sq.PageCache(1, KV, dk, 16, 300, dt)
+    pools = Pools(cache)
+    base = cache.add()
+    seqs = []
+
+    def more(s, n):
+        at = cache.length(s)
+        cache.extend(s, n)
+        K, V = rng.normal(size=(1, n, KV, dk)) * 0.3, np.abs(rng.normal(size=(1, n, KV, dk))) + 0.5
+        K[..., 0] = 0
+        if at == 0 and n:
+            K[0, 0], V[0, 0] = 0, 1e-3 * V[0, 0]
+            K[0, 0, :, 0] = gap
+        if n:
+            pools.write(s, at, K.astype(NP[dt]), V.astype(NP[dt]))
+
+    more(base, prefix)
+    for o in owns:
+        seqs += cache.fork(base, prefix, 1)
+        more(seqs[-1], o)
+    n = sum(news)
+    batch = sq.PageBatch(cache, H, len(seqs), n)
+    batch.begin(seqs, news)
+    (q, k, v), _ = inputs(m, n, rng)
+    q, k, v = 0.5 * q, 0.3 * k, np.abs(v) + np.float32(0.5)
+    q[:, ::dk], k[:, ::dk] = dk ** 0.5, 0
+    out = attend(batch, m, [torch.from_numpy(a).cuda() for a in (q, k, v)], n)
+    host, at = pools.host(), 0
+    for s, c in zip(seqs, news):
+        pos = np.arange(cache.length(s) - c, cache.length(s))
+        K, V = (a[0].astype(np.float64) for a in pools.read(s, host))
+        qr, qs = m.row(q[at:at + c], H, None, None, pos)
+        for h in range(H):
+            o, b = attention64(qr[:, h], qs[:, h], K[:, h // 4], V[:, h // 4], pos, dk ** -0.5)
+            floor = np.stack([2.0 ** -38 * V[:p + 1, h // 4].sum(0) for p in pos])
+            got = out[at:at + c, h * dk:(h + 1) * dk]
+            worst = (np.abs(got - o) / (b + floor)).max()
+            assert worst <= 1, (s, h, worst, np.abs(got / o - 1).max())
+        at += c
