@@ -119,3 +119,44 @@ def test_small_weights_behind_a_large_one(prefix, owns, news, dt, gap):
             worst = (np.abs(got - o) / (b + floor)).max()
             assert worst <= 1, (s, h, worst, np.abs(got / o - 1).max())
         at += c
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16"])
+@pytest.mark.parametrize("dk", [64, 192])
+def test_workgroups_that_take_several_pieces(dk, dt):
+    """A captured launch has 1024 workgroups whatever the step: steps of more pieces, of blocks of one row, of up to 32
+    and of more, in one replay; each replayed twice, with the same bits."""
+    rng = np.random.default_rng(dk)
+    H = KV = 32
+    m = Model(H, KV, dk, dk // 2, rng)
+    cache = sq.PageCache(1, KV, dk, 16, 260, dt)
+    pools = Pools(cache)
+    seqs = batch_of(cache, pools, 150, [3, 40, 9, 170] * 8, rng)
+    batch = sq.PageBatch(cache, H, 32, 500)
+    st = torch.cuda.Stream()
+    d = [torch.zeros(500, h * dk, device="cuda") for h in (H, KV, KV)]
+    out = torch.zeros(500, H * dk, device="cuda")
+    batch.begin(seqs, [1] * 31 + [400], st.cuda_stream)  # (the buffer's size)
+    batch.begin(seqs[:1], [1], st.cuda_stream)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=st):
+        sq.page_attention_dev(batch, 0, m.params, *(t.data_ptr() for t in d), out.data_ptr(), st.cuda_stream)
+    for i, s in enumerate(seqs):  # (rows that no attention call wrote)
+        cache.truncate(s, 150 + [3, 40, 9, 170][i % 4])
+    for rows in ([1, 20, 1, 70, 2, 33, 1, 40] + [1] * 24, [1] * 32, [1, 1, 65, 1] * 4 + [1, 17, 1, 1] * 4):
+        n = sum(rows)
+        batch.begin(seqs, rows, st.cuda_stream)
+        before = pools.host()
+        host, dev = inputs(m, n, rng)
+        for t, a in zip(d, dev):
+            t[:n] = a
+        bits = []
+        for _ in range(2):
+            out.fill_(float("nan"))
+            torch.cuda.synchronize()
+            g.replay()
+            torch.cuda.synchronize()
+            bits.append(out.cpu().numpy())
+        check_step(cache, pools, m, seqs, rows, *host, bits[0], before, 0)
+        assert np.array_equal(bits[0].view(np.int32), bits[1].view(np.int32))
