@@ -855,18 +855,22 @@ sllm_status sllm_page_batch_begin(sllm_page_batch *batch, const int *seqs, const
         b.versions.resize((size_t)count);
         for (int i = 0; i < count; i++) b.versions[(size_t)i] = c.seqs[(size_t)seqs[i]].version;
         b.rows = (int)total;
-        if (at <= kSmallStep) {
-            SmallStep small;
-            std::memcpy(small.v, h, (size_t)at * sizeof(int));
-            hipLaunchKernelGGL(page_step_kernel, dim3(1), dim3(256), 0, s, small, b.dev, at);
-            SLLM_HIP(hipGetLastError());
-        } else {
-            SLLM_HIP(hipMemcpyAsync(b.dev, h, (size_t)at * sizeof(int), hipMemcpyHostToDevice, s));
-            SLLM_HIP(hipEventRecord(b.done[slot], s));
-            b.slot = (slot + 1) % PageBatch::kSlots;
-        }
-        b.begun = true;
-        return SLLM_OK;
+        st = [&]() -> sllm_status {
+            if (at <= kSmallStep) {
+                SmallStep small;
+                std::memcpy(small.v, h, (size_t)at * sizeof(int));
+                hipLaunchKernelGGL(page_step_kernel, dim3(1), dim3(256), 0, s, small, b.dev, at);
+                SLLM_HIP(hipGetLastError());
+            } else {
+                SLLM_HIP(hipMemcpyAsync(b.dev, h, (size_t)at * sizeof(int), hipMemcpyHostToDevice, s));
+                b.slot = (slot + 1) % PageBatch::kSlots;
+                SLLM_HIP(hipEventRecord(b.done[slot], s));
+            }
+            return SLLM_OK;
+        }();
+        if (st != SLLM_OK) take_back(c, seqs, rows, count, &copies);
+        b.begun = st == SLLM_OK;
+        return st;
     });
 }
 

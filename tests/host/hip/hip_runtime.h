@@ -35,7 +35,7 @@ typedef int *hipEvent_t;
 enum { hipMemcpyHostToDevice = 1, hipEventDisableTiming = 2, hipHostMallocDefault = 0 };
 
 namespace stub {
-inline int mallocs_left = -1, host_mallocs_left = -1, launches_left = -1;  // until one fails; -1: none does
+inline int mallocs_left = -1, host_mallocs_left = -1, launches_left = -1, memcpys_left = -1;  // until one fails; -1: none does
 inline int device = 0;
 inline hipError_t last = hipSuccess;
 inline bool capture = false;
@@ -103,6 +103,7 @@ inline hipError_t hipMemsetAsync(void *p, int v, size_t n, hipStream_t) {
     return hipSuccess;
 }
 inline hipError_t hipMemcpyAsync(void *to, const void *from, size_t n, int, hipStream_t) {
+    if (stub::fails(&stub::memcpys_left)) return hipErrorInvalidConfiguration;
     std::memcpy(to, from, n);
     return hipSuccess;
 }

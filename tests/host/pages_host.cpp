@@ -314,7 +314,19 @@ static void failed_copies() {
     stub::launches_left = -1;
     CHECK(c.state(seqs) == gap);
     run(c, b, seqs, {1, 1, 1, 1, 1, 30});
-    CHECK(c.add() == 3 && c.add() == 7);  // numbers of sequences that were not made are free
+    // neither can the step's description: no step, and no rows either
+    for (const auto &rows : {std::vector<int>{1, 1, 1, 1, 1, 1}, std::vector<int>{9, 9, 9, 9, 9, 9}}) {
+        seqs.push_back(c.fork(seqs[0], 701, 1)[0]);  // (and a tail page to copy)
+        const auto before = c.state(seqs);
+        std::vector<int> all = rows;
+        all.resize(seqs.size());
+        stub::launches_left = 1;
+        stub::memcpys_left = 0;
+        CHECK(b.begin(seqs, all) == SLLM_ERR_DEVICE && c.state(seqs) == before && b.attend() == SLLM_ERR_ARG);
+        stub::launches_left = stub::memcpys_left = -1;
+        run(c, b, seqs, all);
+    }
+    CHECK(seqs[6] == 3 && seqs[7] == 7 && c.add() == 8);  // numbers of sequences that were not made are free
 }
 
 // Sequences up to the longest, whose pieces end next to what 32 bits hold.
