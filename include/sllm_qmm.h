@@ -441,13 +441,14 @@ sllm_status sllm_page_cache_compact(sllm_page_cache *pc, int *used, void *stream
  * attention calls need, so those allocate nothing.
  * sllm_page_batch_begin begins a step: rows[i] (0: none) rows are appended to
  * sequence seqs[i] (each named once), pages taken and shared tail pages copied;
- * then one sllm_page_attention_dev per layer fills and reads them. SLLM_ERR_OOM
- * (and nothing changed) where there are too few vacant pages. A step ends with
- * the next begin; freeing, cutting or moving (compaction, a tail page copied for
- * another step) one of its sequences ends it too: attention calls are refused
- * (SLLM_ERR_ARG) until the next begin. Rows that a step appends exist once the
- * attention calls of all layers are enqueued: sequences that are to have them are
- * forked or copied behind these.
+ * then one sllm_page_attention_dev per layer fills and reads them. A begin that is
+ * refused (SLLM_ERR_OOM where there are too few vacant pages) changes nothing, and
+ * the step before it stays; one that fails on the device (SLLM_ERR_DEVICE) appends
+ * nothing and ends the step before it. A step ends with the next begin; freeing, cutting
+ * or moving (compaction, a tail page copied for another step) one of its sequences ends
+ * it too: attention calls are refused (SLLM_ERR_ARG) until the next begin. Rows that a
+ * step appends exist once the attention calls of all layers are enqueued: sequences that
+ * are to have them are forked or copied behind these.
  */
 typedef struct sllm_page_batch sllm_page_batch;
 sllm_status sllm_page_batch_create(sllm_page_cache *pc, int n_heads, int max_seqs, int max_rows,
@@ -465,10 +466,18 @@ sllm_status sllm_page_batch_begin(sllm_page_batch *batch, const int *seqs, const
  * then every row's causal attention over its sequence's rows (as the pages
  * hold them) to out (rows x n_heads*d_k). q, k, v and out must be 16-byte
  * aligned; q, k and v are not modified, rows of the pools beyond those appended
- * neither. Asynchronous on `stream`. A captured call follows the batch's
- * later steps when it is replayed (their begin calls stay outside the graph), as long as
- * they fit the buffers that it was captured with (begin says SLLM_ERR_SHAPE where not);
- * q, k, v and out must then hold max_rows rows.
+ * neither. Sums and softmax statistics are fp32, the weights the hardware's 32-bit
+ * exponentials (sllm_attention_dev forms them in 64 bits). Over f16 pages q and the
+ * weights enter the products as two f16 each: within 2^-23 of an element of q or 2^-35
+ * of its head's largest, within 2^-23 of a weight or 2^-38 of the row's largest.
+ * Asynchronous on `stream`.
+ * A captured call follows the batch's later steps when it is replayed (their begin
+ * calls stay outside the graph), as long as they fit the buffer that it was captured with:
+ * some twice the rows and page numbers of the step that last enlarged it (begin says
+ * SLLM_ERR_SHAPE where they don't; a new batch, captured again, takes them).
+ * q, k, v and out must then hold max_rows rows, and every replay launches for max_rows:
+ * captured decode steps want a batch of about their rows. The graph is replayed only while
+ * the call itself would be accepted: after a begin, before its sequences are freed or cut.
  */
 sllm_status sllm_page_attention_dev(sllm_page_batch *batch, int layer, const sllm_attn_params *p, const float *q_dev,
                                     const float *k_dev, const float *v_dev, float *out_dev, void *stream);
@@ -493,6 +502,8 @@ sllm_status sllm_lora_set_load(sllm_lora_set *set, int slot, int rank, const voi
  * names no loaded adapter (-1, say) get dst[r] = y[r]. dst may be y: the
  * output of the shared projection (sllm_matmul_dev and its kin) then gets the
  * adapters' part in place. Products and sums in fp32. x must be 16-byte aligned.
+ * Calls of more than 64 rows expect an adapter's rows to lie together (prompts); decode
+ * batches with many adapters in any order go faster in calls of 64 rows.
  * Asynchronous on `stream`; uses the stream's workspace (sllm_workspace_reserve;
  * x_rows x (128 x max_rank + 1024) bytes are enough). A captured call reads ids
  * and adapters as they are at each replay; replays of graphs that were captured on

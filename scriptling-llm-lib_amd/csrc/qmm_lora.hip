@@ -319,7 +319,9 @@ constexpr int stage_bytes() {
 // straight into their operands (16 rows x 64 bytes an instruction) they were what bounded them (700 rows, 14336 columns,
 // rank 64, f32: 41 us). So every wave brings whole lines into two stages of LDS of its own, one on its way while the
 // other is used; a row's pieces of 16 bytes are kept in an order (exclusive or with the row) that lets 16 rows' be
-// read without conflicts.
+// read without conflicts. A workgroup takes the units of its 64 rows one after the other: made for prompts, whose 64 rows
+// have one or two (4096 x 4096, rank 16, f16, 256 rows: 16.5 us on 8 adapters in order, 23 in any order; on 32 in any
+// order 58, four calls of 64 rows 43).
 template <class T, int RB>
 __global__ void __launch_bounds__(256, 1) lora_down_rows_kernel(LoraArgs g) {
     constexpr int XB = 64 * 4 * kStep, stage = stage_bytes<T, RB>();

@@ -200,7 +200,8 @@ constexpr int kWorthSharing = 128;
 // (The plan is made before the step's rows are appended: they change no full page before them.)
 // Sequences `who` (of the step) have page p in common for p < from (their segments up to there
 // are made); what follows is cut into segments: a run of pages that several hold once for all of these, and so
-// on behind it, at most kMaxParts to a sequence.
+// on behind it, at most kMaxParts to a sequence. Sequences that go on with the same page are one group; where the run that
+// all of it holds is shorter than kWorthSharing, each is on its own, also those that have more in common behind it.
 void share(const PageCache &c, const int *seqs, const int *rows, const std::vector<int> &row0, std::vector<int> who, int from,
            int depth, Plan *plan) {
     auto table = [&](int i) -> const std::vector<int> & { return c.seqs[(size_t)seqs[i]].pages; };
@@ -278,7 +279,8 @@ struct PieceCost {
 // workgroups one after the other, are estimated to end first; and no more states than the batch has room for. Returns
 // the number of pieces (for one kv head). (32 / 8 heads of 128; the longest share that all workgroups take at once, and
 // so chosen, us: f32, 64 sequences on a prefix of 4000 85.7, 70.8; 16 on 8000 48.8, 44.9; 5 prompts of 211 rows 161,
-// 147; f16, the 64 39.3, 35.2; others within 1. The estimates take the host 4 us for 16 sequences.)
+// 147; f16, the 64 39.3, 35.2; others within 1. A step's begin with all of this takes the host 12 us for 16 sequences, 30 for
+// 64 on a prefix of 4000 in pages of 64, 90 on one of 16000 in pages of 16, 105 for 256 on 4000.)
 int cut(const PageCache &c, Plan *plan, int rep, int slots) {
     const int *most = kShapeRows[shape_class(c.d_k, c.type == SLLM_CACHE_F16)], n_kv = c.n_kv;
     int64_t all = 0;
