@@ -72,7 +72,10 @@ const char *sllm_last_error(void);
  * call's; decided for each weight by itself, so a call of several weights still
  * gives the single calls' bits). A buffer that is outgrown is kept, not
  * freed, until the process ends, so graphs captured before a growth stay
- * valid. Growth at least doubles the buffer.
+ * valid. Growth at least doubles the buffer. A call's launches use the buffer one
+ * after the other: calls on one stream come from one thread at a time, and a graph's
+ * replay overlaps neither calls on the stream that it was captured on nor replays of
+ * other graphs captured there.
  */
 sllm_status sllm_workspace_reserve(void *stream, size_t bytes);
 
