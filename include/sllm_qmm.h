@@ -460,6 +460,18 @@ void sllm_page_batch_destroy(sllm_page_batch *batch);
 sllm_status sllm_page_batch_begin(sllm_page_batch *batch, const int *seqs, const int *rows, int count, void *stream);
 
 /*
+ * A step whose rows are drafted tokens, a tree (or several) for each sequence: parents holds, for the rows of all sequences
+ * one after the other, the number within its sequence of the row that a row continues: an earlier one, or -1 where that
+ * is the sequence's last row before the step (else SLLM_ERR_ARG). Rows are appended in their order; a row's position (its
+ * rotation) is that of its parent and one, it sees the sequence's rows before the step, its ancestors and itself.
+ * Sequences whose rows each follow the one before are steps of sllm_page_batch_begin; others have at most 1024 rows here
+ * (SLLM_ERR_SHAPE). Behind the attention of all layers sllm_page_accept_dev finds the path that the chosen tokens
+ * follow, sllm_page_keep_dev moves its rows together, and sllm_page_seq_truncate cuts the others off.
+ */
+sllm_status sllm_page_batch_begin_tree(sllm_page_batch *batch, const int *seqs, const int *rows, int count,
+                                       const int *parents, void *stream);
+
+/*
  * The attention section of `layer` for the batch's step (forwardBlock,
  * model_f32.go:398-466, as sllm_attention_dev for one sequence): q (rows x
  * n_heads*d_k), k and v (rows x n_kv_heads*d_k) hold the sequences' new rows
@@ -484,6 +496,73 @@ sllm_status sllm_page_batch_begin(sllm_page_batch *batch, const int *seqs, const
  */
 sllm_status sllm_page_attention_dev(sllm_page_batch *batch, int layer, const sllm_attn_params *p, const float *q_dev,
                                     const float *k_dev, const float *v_dev, float *out_dev, void *stream);
+
+/*
+ * Which of the step's rows the chosen tokens accept, for each sequence: its first row, then from row to row the first
+ * (lowest) one that continues it and holds the token chosen behind it. tokens[r] is the token of the step's row r, chosen[r] the
+ * one chosen from row r's logits (sllm_logits_rules_dev, or a sampler's). kept_dev (an int for each row): for a sequence with
+ * rows f .. f + n - 1 of the step, kept[f + j] is the j-th row of its path, -1 behind the path's end. counts_dev and
+ * next_dev (an int for each sequence of the step): the path's length, and the token chosen behind it, which is the
+ * first of the sequence's next step (0 and -1 for a sequence without rows). Also for steps of
+ * sllm_page_batch_begin, whose rows each continue the one before. Integers of any value are allowed in tokens and chosen.
+ * Asynchronous on `stream`; captured as sllm_page_attention_dev (tokens, chosen and kept then hold max_rows ints, counts
+ * and next max_seqs).
+ */
+sllm_status sllm_page_accept_dev(sllm_page_batch *batch, const int *tokens_dev, const int *chosen_dev, int *kept_dev,
+                                 int *counts_dev, int *next_dev, void *stream);
+
+/*
+ * Moves rows of the step to the front of their sequences' new rows, in every layer: kept_dev is as
+ * sllm_page_accept_dev leaves it; row kept[f + j] goes to the place of row f + j, up to a sequence's first entry that is not
+ * a row of the sequence from f + j on. Entries must ascend within a sequence. Rows keep their rotation: the j-th row of a
+ * path has the position of its place. The host's lengths stay: sllm_page_seq_truncate takes the rows behind the path (and
+ * ends the step). Other rows of the pools are not modified; the places behind the path keep their
+ * contents. A page with rows of the step that another sequence holds too (a fork
+ * since the step's begin) is refused (SLLM_ERR_ARG). Asynchronous on `stream`; captured as sllm_page_attention_dev.
+ */
+sllm_status sllm_page_keep_dev(sllm_page_batch *batch, const int *kept_dev, void *stream);
+
+/* What one request asks of its logits. 32 bytes; in device memory (sllm_logits_params). */
+typedef struct sllm_logits_rule {
+    float repeat;              /* 1: none */
+    float frequency, presence; /* 0: none */
+    int history_at, history;   /* the tokens history[history_at .. history_at + history - 1] */
+    int bias_at, biases;       /* the biases bias_at .. bias_at + biases - 1 */
+    int reserved;
+} sllm_logits_rule;
+
+/* What the rules refer to: counts by value, arrays in device memory (NULL where the count is 0). What lies outside
+ * an array (a history's or a list of biases' end, a mask's number, a token that the vocabulary has not) counts
+ * as not being there. */
+typedef struct sllm_logits_params {
+    const sllm_logits_rule *rules; /* by row; with a batch by sequence of its step. Rows beyond have no rule */
+    int n_rules;
+    const int *history;            /* tokens of all requests */
+    int n_history;
+    const int *bias_tokens;        /* of a token that a request names twice the later bias counts */
+    const float *bias_values;
+    int n_biases;
+    const uint32_t *masks;         /* n_masks rows of ceil(vocab / 32) words: token t allowed where bit t % 32 of word t / 32 is set */
+    int n_masks;
+    const int *mask_ids;           /* each row's mask, -1: none */
+    const int *tokens;             /* with a batch: the tokens of the step's rows; may be NULL */
+} sllm_logits_params;
+
+/*
+ * Logits (rows x vocab floats) after their requests' rules, and the token chosen from each row. With n(t) how often
+ * token t occurs in the request's history and, with a batch and tokens, among the tokens of the row and its
+ * ancestors in the step, a logit l of a token with n(t) > 0 becomes (l > 0 ? l / repeat : l * repeat) -
+ * (frequency * n(t) + presence); then the request's bias of t is added; then tokens that the row's mask does not allow
+ * become -inf. Each operation rounds once to float32, in this order. dst_dev (rows x vocab; may be logits_dev, else
+ * must not overlap it; NULL: not wanted) receives all logits, chosen_dev (rows ints; NULL: not wanted) the first token of
+ * the largest value as argmaxF32 (float32_ops.go:812-822) but for NaN values, which are never chosen, and -1 where no value is above -inf.
+ * batch (may be NULL): the rows are those of its step. Asynchronous on `stream`. Choosing
+ * uses the stream's workspace (sllm_workspace_reserve; rows x (vocab / 512 + 64) bytes are enough); graphs captured on one
+ * stream share it and must not overlap. A captured call with a batch follows its later steps as
+ * sllm_page_attention_dev: `rows` then are those that the buffers hold, max_rows say.
+ */
+sllm_status sllm_logits_rules_dev(const float *logits_dev, int rows, int vocab, const sllm_logits_params *params,
+                                  float *dst_dev, int *chosen_dev, const sllm_page_batch *batch, void *stream);
 
 typedef enum { SLLM_LORA_F32 = 0, SLLM_LORA_F16 = 1, SLLM_LORA_BF16 = 2 } sllm_lora_type;
 

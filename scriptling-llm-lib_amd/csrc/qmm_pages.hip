@@ -11,18 +11,10 @@
 #include <algorithm>
 #include <cstring>
 #include <functional>
-#include <new>
 #include <string>
 #include <unordered_map>
 
 #include "qmm_pages.hpp"
-
-struct sllm_page_cache {
-    std::shared_ptr<sllm::PageCache> c;
-};
-struct sllm_page_batch {
-    sllm::PageBatch b;
-};
 
 namespace sllm {
 
@@ -67,28 +59,9 @@ __global__ void __launch_bounds__(256) page_step_kernel(SmallStep step, int *dev
     for (int i = threadIdx.x; i < n; i += 256) dev[i] = step.v[i];
 }
 
-// A C entry ends with a status, whatever the host's allocations do.
-template <class F>
-sllm_status guarded(F f) {
-    try {
-        return f();
-    } catch (const std::bad_alloc &) {
-        return set_error(SLLM_ERR_OOM, "out of memory");
-    } catch (...) {
-        return set_error(SLLM_ERR_ARG, "internal error");
-    }
-}
-
 struct DeviceFree {
     void operator()(void *p) const { (void)hipFree(p); }
 };
-
-sllm_status on_device(int device) {
-    int dev = 0;
-    SLLM_HIP(hipGetDevice(&dev));
-    if (dev != device) return set_error(SLLM_ERR_ARG, "the page cache is another device's");
-    return SLLM_OK;
-}
 
 // The pages that appending rows[i] rows to each sequence takes, and whether there are so
 // many; all the memory that `append` needs is taken here.
@@ -184,10 +157,11 @@ struct Segment {
     int tok0, ntok;
     int shape = 0, block = 0;  // rows of a block (shape), query rows of a block
     int slot = 0, pieces = 1, piece = 0;
-    bool causal = false, lone = false;  // lone: its rows have no other segment
+    bool causal = false, tree = false, lone = false;  // lone: its rows have no other segment
 };
 
 struct Plan {
+    std::vector<char> tree;  // per sequence: its rows are a tree
     std::vector<Segment> segs;
     std::vector<int> tok;
     std::vector<std::vector<std::pair<int, int>>> parts;  // per sequence: (segment, number of its first row in it)
@@ -214,7 +188,8 @@ void share(const PageCache &c, const int *seqs, const int *rows, const std::vect
         s.p1 = c.seqs[(size_t)seqs[i]].len + rows[i];
         s.tok0 = (int)plan->tok.size();
         s.ntok = rows[i];
-        s.causal = rows[i] > 1;
+        s.tree = plan->tree[(size_t)i];
+        s.causal = rows[i] > 1 && !s.tree;
         s.lone = plan->parts[(size_t)i].empty();
         for (int r = 0; r < rows[i]; r++) plan->tok.push_back(row0[(size_t)i] + r);
         plan->parts[(size_t)i].push_back({(int)plan->segs.size(), 0});
@@ -683,6 +658,8 @@ sllm_status sllm_page_batch_create(sllm_page_cache *pc, int n_heads, int max_seq
         b->b.max_rows = max_rows;
         b->b.seqs.reserve((size_t)max_seqs);
         b->b.versions.reserve((size_t)max_seqs);
+        b->b.counts.reserve((size_t)max_seqs);
+        b->b.bases.reserve((size_t)max_seqs);
         const int rep = n_heads / c.n_kv;
         b->b.slots = (kMaxParts + 1) * max_rows * rep + kSpareStates;
         const size_t states = (size_t)b->b.slots * c.n_kv;
@@ -700,7 +677,10 @@ sllm_status sllm_page_batch_create(sllm_page_cache *pc, int n_heads, int max_seq
 
 void sllm_page_batch_destroy(sllm_page_batch *batch) { delete batch; }
 
-sllm_status sllm_page_batch_begin(sllm_page_batch *batch, const int *seqs, const int *rows, int count, void *stream) {
+// A step's begin; parents (may be null: every row follows the one before it) are those of all sequences' rows, numbered
+// within their sequence.
+static sllm_status begin_step(sllm_page_batch *batch, const int *seqs, const int *rows, int count, const int *parents,
+                              void *stream) {
     if (!batch || (count > 0 && (!seqs || !rows))) return set_error(SLLM_ERR_ARG, "null pointer");
     PageBatch &b = batch->b;
     if (count < 0 || count > b.max_seqs) return set_error(SLLM_ERR_ARG, "count outside 0 .. max_seqs");
@@ -709,22 +689,34 @@ sllm_status sllm_page_batch_begin(sllm_page_batch *batch, const int *seqs, const
         std::lock_guard<std::mutex> lb(b.mu);
         PageCache &c = *b.c;
         std::lock_guard<std::mutex> lk(c.mu);
-        int64_t total = 0, pages = 0;
+        int64_t total = 0, pages = 0, tree_ints = 0;
+        Plan plan;
+        plan.tree.assign((size_t)count, 0);
         std::vector<int> sorted(seqs, seqs + count);
         std::sort(sorted.begin(), sorted.end());
         for (int i = 0; i < count; i++) {
             if (!c.live(seqs[i])) return set_error(SLLM_ERR_ARG, "no such sequence");
             if (i && sorted[(size_t)i] == sorted[(size_t)i - 1]) return set_error(SLLM_ERR_ARG, "a sequence is named twice");
             if (rows[i] < 0) return set_error(SLLM_ERR_ARG, "rows must not be negative");
+            for (int r = 0; parents && r < rows[i]; r++) {
+                const int up = parents[total + r];
+                if (up < -1 || up >= r) return set_error(SLLM_ERR_ARG, "a row's parent must be an earlier row of its sequence, or -1");
+                plan.tree[(size_t)i] |= up != r - 1;
+            }
+            if (plan.tree[(size_t)i]) {
+                if (rows[i] > kTreeRows) return set_error(SLLM_ERR_SHAPE, "a sequence's tree has at most 1024 rows");
+                tree_ints += ((int64_t)rows[i] * tree_halves(c.seqs[(size_t)seqs[i]].len, rows[i]) + 1) / 2 + 3;
+            }
             total += rows[i];
             pages += ((int64_t)c.seqs[(size_t)seqs[i]].len + rows[i] + c.page_rows - 1) >> c.shift;
         }
         if (total > b.max_rows) return set_error(SLLM_ERR_SHAPE, "more rows than max_rows");
         // room for the step on the device and in the next staging slot: header, rows, rows of segments,
-        // pieces, tables
+        // pieces, tables, what trees see
         const int64_t most_segs = 2 * (int64_t)count;
         const int64_t most_items = most_segs + kMaxParts * total + 3 * kTargetPieces;
-        const int64_t ints = kStepHeader + total * (int64_t)(sizeof(StepRow) / 4 + kMaxParts) + 16 * most_items + pages + 32;
+        const int64_t ints = kStepHeader + total * (int64_t)(sizeof(StepRow) / 4 + kMaxParts + 1) + 16 * most_items + pages +
+                             count + tree_ints + 32;
         if (ints > INT32_MAX) return set_error(SLLM_ERR_SHAPE, "the step has too many rows and pages (offsets of 32 bits)");
         const size_t bytes = (size_t)ints * sizeof(int);
         sllm_status st = on_device(c.device);
@@ -732,7 +724,6 @@ sllm_status sllm_page_batch_begin(sllm_page_batch *batch, const int *seqs, const
         if (stream_capturing(s)) return set_error(SLLM_ERR_ARG, "a batch's step cannot begin under capture");
         std::vector<PageCopy> copies;
         if ((st = prepare_append(c, seqs, rows, count, &copies)) != SLLM_OK) return st;
-        Plan plan;
         plan.parts.resize((size_t)count);
         plan.tok.reserve((size_t)total * kMaxParts);
         std::vector<int> row0((size_t)count), who;
@@ -746,6 +737,7 @@ sllm_status sllm_page_batch_begin(sllm_page_batch *batch, const int *seqs, const
         share(c, seqs, rows, row0, std::move(who), 0, 0, &plan);
         const int n_items = cut(c, &plan, (int)rep, b.slots);
         std::vector<int> table((size_t)count, -1);  // of the sequences that segments read
+        std::vector<int> tree_at((size_t)count, 0);
         // (a larger buffer takes the old one's place once nothing refuses the step any more: until then the step before
         // it is the batch's, and the old buffer holds it)
         std::unique_ptr<void, DeviceFree> grown;
@@ -799,6 +791,28 @@ sllm_status sllm_page_batch_begin(sllm_page_batch *batch, const int *seqs, const
         const int tok_at = place((int64_t)plan.tok.size());
         h[kStepRowsAt] = place((int64_t)(sizeof(StepRow) / 4) * total);
         StepRow *hr = (StepRow *)(h + h[kStepRowsAt]);
+        h[kStepSeqs] = count;
+        h[kStepSeqsAt] = place((int64_t)count + 1);
+        h[kStepOfAt] = place(total);
+        std::copy(row0.begin(), row0.end(), h + h[kStepSeqsAt]);
+        h[h[kStepSeqsAt] + count] = (int)total;
+        for (int i = 0; i < count; i++) {
+            std::fill_n(h + h[kStepOfAt] + row0[(size_t)i], rows[i], i);
+            if (!plan.tree[(size_t)i]) continue;
+            const int base = c.seqs[(size_t)seqs[i]].len - rows[i], n = tree_halves(base, rows[i]);
+            const int *up = parents + row0[(size_t)i];
+            tree_at[(size_t)i] = place(((int64_t)rows[i] * n + 1) / 2);
+            uint16_t *sees = (uint16_t *)(h + tree_at[(size_t)i]);
+            for (int r = 0; r < rows[i]; r++) {
+                if (up[r] >= 0) {
+                    std::copy_n(sees + up[r] * n, n, sees + r * n);
+                } else {
+                    std::fill_n(sees + r * n, n, (uint16_t)0);
+                    sees[r * n] = (uint16_t)((1 << (base & 15)) - 1);
+                }
+                sees[r * n + ((base + r) >> 4) - (base >> 4)] |= (uint16_t)(1 << ((base + r) & 15));
+            }
+        }
         b.combine = 0;
         for (int i = 0; i < count; i++) {
             const PageSeq &q = c.seqs[(size_t)seqs[i]];
@@ -807,12 +821,19 @@ sllm_status sllm_page_batch_begin(sllm_page_batch *batch, const int *seqs, const
             for (const auto &m : mine) pieces += plan.segs[(size_t)m.first].pieces;
             if (pieces > 1) b.combine = std::max(b.combine, pieces);
             for (int r = 0; r < rows[i]; r++) {
-                const int pos = q.len - rows[i] + r;
-                StepRow x = {q.pages[(size_t)(pos >> c.shift)], pos & (c.page_rows - 1), pos, pieces == 1, {}};
+                const int base = q.len - rows[i], at_row = base + r;
+                StepRow x = {q.pages[(size_t)(at_row >> c.shift)], at_row & (c.page_rows - 1), at_row, pieces == 1, {}, at_row + 1, -1,
+                             r ? row0[(size_t)i] + r - 1 : -1};
+                if (plan.tree[(size_t)i]) {
+                    const int up = parents[row0[(size_t)i] + r];
+                    x.parent = up < 0 ? -1 : row0[(size_t)i] + up;
+                    x.pos = up < 0 ? base : hr[up - r].pos + 1;
+                    x.tree = 2 * tree_at[(size_t)i] + r * tree_halves(base, rows[i]);
+                }
                 for (size_t k = 0; k < mine.size(); k++) {
                     const Segment &s = plan.segs[(size_t)mine[k].first];
                     x.parts[k] = {s.slot + (mine[k].second + r) * (int)rep, s.ntok * (int)rep,
-                                  std::min(s.pieces, (pos - s.p0) / s.piece + 1), 0};
+                                  std::min(s.pieces, (at_row - s.p0) / s.piece + 1)};
                 }
                 *hr++ = x;
             }
@@ -840,8 +861,8 @@ sllm_status sllm_page_batch_begin(sllm_page_batch *batch, const int *seqs, const
                     x.tok = run ? tk[0] : tok_at + s.tok0 + k;
                     x.slot = s.slot + (i * s.ntok + k) * (int)rep;
                     // a sequence's own rows: row k of n sees n - 1 - k positions less than the last
-                    x.lim0 = s.causal ? std::min(x.p1, s.p1 - (s.ntok - 1 - k)) : x.p1;
-                    x.flags = s.shape | (s.causal ? kItemCausal : 0) | (direct ? kItemDirect : 0) | (run ? kItemRun : 0);
+                    x.lim0 = s.causal ? std::min(x.p1, s.p1 - (s.ntok - 1 - k)) : s.tree ? s.p1 - s.ntok : x.p1;
+                    x.flags = s.shape | (s.causal ? kItemCausal : 0) | (s.tree ? kItemTree : 0) | (direct ? kItemDirect : 0) | (run ? kItemRun : 0);
                     const std::vector<int> &pg = c.seqs[(size_t)seqs[s.first]].pages;
                     for (int u = 0; u < 8; u++) {
                         const size_t at_page = (size_t)(x.p0 >> c.shift) + (size_t)u;
@@ -851,11 +872,19 @@ sllm_status sllm_page_batch_begin(sllm_page_batch *batch, const int *seqs, const
                 }
         }
         b.items = n_items;
+        b.rows_at = h[kStepRowsAt];
+        b.seqs_at = h[kStepSeqsAt];
+        b.of_at = h[kStepOfAt];
         b.wide = false;
         for (const Segment &s : plan.segs) b.wide |= s.shape == 0 && s.ntok * rep > 16;
         b.seqs.assign(seqs, seqs + count);
         b.versions.resize((size_t)count);
-        for (int i = 0; i < count; i++) b.versions[(size_t)i] = c.seqs[(size_t)seqs[i]].version;
+        b.counts.assign(rows, rows + count);
+        b.bases.resize((size_t)count);
+        for (int i = 0; i < count; i++) {
+            b.versions[(size_t)i] = c.seqs[(size_t)seqs[i]].version;
+            b.bases[(size_t)i] = c.seqs[(size_t)seqs[i]].len - rows[i];
+        }
         b.rows = (int)total;
         st = [&]() -> sllm_status {
             if (at <= kSmallStep) {
@@ -876,6 +905,17 @@ sllm_status sllm_page_batch_begin(sllm_page_batch *batch, const int *seqs, const
     });
 }
 
+sllm_status sllm_page_batch_begin(sllm_page_batch *batch, const int *seqs, const int *rows, int count, void *stream) {
+    return begin_step(batch, seqs, rows, count, nullptr, stream);
+}
+
+sllm_status sllm_page_batch_begin_tree(sllm_page_batch *batch, const int *seqs, const int *rows, int count,
+                                       const int *parents, void *stream) {
+    for (int i = 0; !parents && rows && i < count; i++)
+        if (rows[i] > 0) return set_error(SLLM_ERR_ARG, "null pointer");
+    return begin_step(batch, seqs, rows, count, parents, stream);
+}
+
 sllm_status sllm_page_attention_dev(sllm_page_batch *batch, int layer, const sllm_attn_params *p, const float *q,
                                     const float *k, const float *v, float *out, void *stream) {
     if (!batch || !p || !q || !k || !v || !out) return set_error(SLLM_ERR_ARG, "null pointer");
@@ -894,12 +934,10 @@ sllm_status sllm_page_attention_dev(sllm_page_batch *batch, int layer, const sll
         return set_error(SLLM_ERR_ARG, "q, k, v and out must be 16-byte aligned");
     {
         std::lock_guard<std::mutex> lk(c.mu);
-        if (!b.begun) return set_error(SLLM_ERR_ARG, "the batch has no step: sllm_page_batch_begin first");
-        for (size_t i = 0; i < b.seqs.size(); i++)
-            if (c.seqs[(size_t)b.seqs[i]].version != b.versions[i])
-                return set_error(SLLM_ERR_ARG, "a sequence of the step was freed, cut or moved: begin it again");
+        const sllm_status st = step_stands(b);
+        if (st != SLLM_OK) return st;
     }
-    sllm_status st = on_device(c.device);
+    const sllm_status st = on_device(c.device);
     if (st != SLLM_OK) return st;
     hipStream_t s = (hipStream_t)stream;
     const bool capture = stream_capturing(s);

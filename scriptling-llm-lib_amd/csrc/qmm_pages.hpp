@@ -7,6 +7,7 @@
 #include <cstdint>
 #include <memory>
 #include <mutex>
+#include <new>
 #include <vector>
 
 #include "qmm_internal.hpp"
@@ -52,12 +53,15 @@ enum {
     kStepRows = 0,     // query rows
     kStepItems = 1,    // pieces
     kStepRowsAt = 2,   // StepRow of every query row (offset in ints)
-    kStepHeader = 16   // then the pieces (StepItem), query rows of segments, StepRows, tables
+    kStepSeqs = 3,     // sequences
+    kStepSeqsAt = 4,   // the first query row of each, and the number of all (offset)
+    kStepOfAt = 5,     // every query row's sequence (offset)
+    kStepHeader = 16   // then the pieces (StepItem), query rows of segments, StepRows, tables, the two above, trees
 };
 // The states of one query row in a segment: of the first piece and q head of the kv head, and the
 // distance to those of the next piece; how many pieces the row sees.
 struct StepPart {
-    int first, step, pieces, pad;
+    int first, step, pieces;
 };
 constexpr int kMaxParts = 3;  // segments of a row at most
 struct StepRow {
@@ -65,18 +69,26 @@ struct StepRow {
     int pos;         // its position
     int direct;      // its one piece writes the output itself
     StepPart parts[kMaxParts];  // (pieces 0 behind the last)
+    int end;         // rows of its sequence that precede it, itself included (its position + 1, but of a tree)
+    int tree;        // the rows of its tree that it sees (tree_half), -1 where these are all up to its own
+    int parent;      // the query row before it (of a tree: its parent), -1 for none
 };
+// What a row of a tree sees: a bit for each of its sequence's rows, 16 to an element, from the element with the
+// first row of the tree on (rows before the tree are seen); one more element, of zeros, behind them. `tree` counts
+// elements from the step's first.
+constexpr int kTreeRows = 1024;  // of a sequence's tree at most
+inline int tree_halves(int base, int n) { return ((base + n - 1) >> 4) - (base >> 4) + 2; }
 // A piece of a segment for a block of its query rows.
 struct StepItem {
     int table;     // page ids of the positions from 0 on (offset)
     int p0, p1;    // positions
     int tok, ntok; // the block's query rows: from tok on (kItemRun), or a list there (offset)
     int slot;      // state of its first row
-    int lim0;      // positions from here on are not seen by every row
+    int lim0;      // positions from here on are not seen by every row (of a tree: the position of its first row)
     int flags;
     int pages[8];  // the first page ids from p0 on: enough for every wave's first rows
 };
-enum { kItemShape = 3, kItemCausal = 4, kItemDirect = 8, kItemRun = 16 };  // shape: kShapeRows
+enum { kItemShape = 3, kItemCausal = 4, kItemDirect = 8, kItemRun = 16, kItemTree = 32 };  // shape: kShapeRows
 // The rows of a block of each shape (0: not there), as far as a wave's registers go: rows that all waves take
 // together, 16 and 32 rows of each wave's own. By d_k: up to 128, the same with f16 runs that are not whole, up to 192, above.
 constexpr int kShapeRows[4][3] = {{32, 64, 128}, {16, 64, 128}, {16, 64, 0}, {0, 64, 0}};
@@ -89,6 +101,7 @@ struct PageBatch {
     int n_heads = 0, max_seqs = 0, max_rows = 0;
     std::vector<int> seqs;           // the current step's sequences
     std::vector<uint32_t> versions;  // as they were at its begin
+    std::vector<int> counts, bases;  // their rows in the step, and before it
     int rows = 0;
     bool begun = false, captured = false;
     int *dev = nullptr;              // the step: header, rows, tables (device)
@@ -98,6 +111,7 @@ struct PageBatch {
     float *part = nullptr, *ml = nullptr;  // the pieces' states, slots for every kv head
     int slots = 0;
     int items = 0;
+    int rows_at = 0, seqs_at = 0, of_at = 0;  // as in the step's header
     bool wide = false;               // some block of the first shape has more than 16 rows
     int combine = 0;                 // most pieces that a row's states are merged of (0: none has several)
     // staging of a step on the host: a slot is written again when its upload is done
@@ -134,6 +148,32 @@ struct PageAttnArgs {
     int type;
 };
 
+// A C entry ends with a status, whatever the host's allocations do.
+template <class F>
+sllm_status guarded(F f) {
+    try {
+        return f();
+    } catch (const std::bad_alloc &) {
+        return set_error(SLLM_ERR_OOM, "out of memory");
+    } catch (...) {
+        return set_error(SLLM_ERR_ARG, "internal error");
+    }
+}
+inline sllm_status on_device(int device) {
+    int dev = 0;
+    SLLM_HIP(hipGetDevice(&dev));
+    if (dev != device) return set_error(SLLM_ERR_ARG, "the page cache is another device's");
+    return SLLM_OK;
+}
+// Whether calls on the batch's step are accepted (under the cache's mutex and the batch's).
+inline sllm_status step_stands(const PageBatch &b) {
+    if (!b.begun) return set_error(SLLM_ERR_ARG, "the batch has no step: sllm_page_batch_begin first");
+    for (size_t i = 0; i < b.seqs.size(); i++)
+        if (b.c->seqs[(size_t)b.seqs[i]].version != b.versions[i])
+            return set_error(SLLM_ERR_ARG, "a sequence of the step was freed, cut or moved: begin it again");
+    return SLLM_OK;
+}
+
 sllm_status launch_page_copies(const PageCache &c, const PageCopy *jobs, size_t n, hipStream_t s);
 sllm_status launch_page_attention(const PageAttnArgs &a, hipStream_t s);
 
@@ -144,3 +184,10 @@ bool stream_capturing(hipStream_t s);
 sllm_status stream_workspace(hipStream_t s, size_t need, void **out, size_t *cap);
 
 }  // namespace sllm
+
+struct sllm_page_cache {
+    std::shared_ptr<sllm::PageCache> c;
+};
+struct sllm_page_batch {
+    sllm::PageBatch b;
+};

@@ -235,7 +235,7 @@ __device__ __forceinline__ void plain_rows(const PageAttnArgs &a, const Piece &p
     const int dk = p.dk, d = 4 * lane, page_rows = 1 << a.shift;
     for (int v = v0; v < v1; v += dv) {
         const int row = p.row_of(v);
-        const int end = p.it.flags & kItemCausal ? min(p.it.p1, p.rows[row].pos + 1) : p.it.p1;
+        const int end = p.it.flags & (kItemCausal | kItemTree) ? min(p.it.p1, p.rows[row].end) : p.it.p1;
         const size_t pair = (size_t)row * a.n_heads + p.g * p.rep + v - p.nth(v) * p.rep;
         v4f q = {0.0f, 0.0f, 0.0f, 0.0f}, o = q;
         if (d < dk) {
@@ -248,7 +248,9 @@ __device__ __forceinline__ void plain_rows(const PageAttnArgs &a, const Piece &p
             }
         }
         float m = -INFINITY, l = 0.0f;
+        const uint16_t *sees = (const uint16_t *)p.step + p.rows[row].tree;
         for (int x = p.it.p0; x < end; x++) {
+            if (p.it.flags & kItemTree && x >= p.it.lim0 && !(sees[(x >> 4) - (p.it.lim0 >> 4)] >> (x & 15) & 1)) continue;
             const size_t at = (((size_t)p.table[x >> a.shift] * a.n_kv + p.g) * page_rows + (x & (page_rows - 1))) * dk + d;
             v4f k = {0.0f, 0.0f, 0.0f, 0.0f}, w = k;
             if (d < dk)
@@ -301,7 +303,7 @@ struct Rows : Shape<T, NB, FULL, VM> {
     v4f qf[F16 ? 1 : MT][F16 ? 1 : KS];
     v8h qh[F16 ? MT : 1][F16 ? KS : 1], ql[F16 ? MT : 1][F16 ? KS : 1];
     float sc[MT], m[MT], l[MT];
-    int lim[MT];
+    int lim[MT];  // positions from here on are not seen; of a tree: what the row sees of it (StepRow)
     v4f o[MT][NT], s[MT][H];
 
     // rows v0 .. of the block (those past its end repeat the last)
@@ -312,7 +314,7 @@ struct Rows : Shape<T, NB, FULL, VM> {
         for (int mt = 0; mt < MT; mt++) {
             const int v = min(v0 + mt * 16 + col, nv - 1);
             const int row = p.row_of(v);
-            lim[mt] = p.it.flags & kItemCausal ? min(p.it.p1, p.rows[row].pos + 1) : p.it.p1;
+            lim[mt] = p.it.flags & kItemTree ? p.rows[row].tree : p.it.flags & kItemCausal ? min(p.it.p1, p.rows[row].end) : p.it.p1;
             const size_t pair = (size_t)row * a.n_heads + p.g * p.rep + v - p.nth(v) * p.rep;
             sc[mt] = a.scale_log2;
             if constexpr (F16) {
@@ -372,11 +374,25 @@ struct Rows : Shape<T, NB, FULL, VM> {
     }
 
     // scores to weights, for the tile at position tp (masked: some row does not see all of it)
-    __device__ __forceinline__ void weights(int tp, bool masked) {
+    __device__ __forceinline__ void weights(const Piece &p, int tp, bool masked) {
         if (masked) {
             int lane = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
             asm volatile("" : "+v"(lane));
             const int qd = lane >> 4;
+            if (p.it.flags & kItemTree) {
+                // (tiles begin at multiples of 16 positions, as the rows' bits; those behind the tree's last 16 are 0)
+                const int half = (tp >> 4) - (p.it.lim0 >> 4);
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                    for (int h = 0; h < H; h++) {
+                        if (half + h < 0) continue;
+                        const unsigned sees = ((const uint16_t *)p.step)[lim[mt] + half + h] >> (4 * qd);
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            if (!(sees >> i & 1)) s[mt][h][i] = -INFINITY;
+                    }
+            } else
 #pragma unroll
             for (int mt = 0; mt < MT; mt++) {
                 const int left = lim[mt] - tp - 4 * qd;
@@ -644,7 +660,7 @@ __device__ __forceinline__ void run_split(const PageAttnArgs &a, const Piece &p,
         r.no_scores();
         r.template scores<0, KS>([&](int h, int j) { return kr[h][j]; });
         if constexpr (MORE) load_k(t + kWaves);
-        r.weights(p0 + t * TP, p0 + t * TP + TP > p.it.lim0);
+        r.weights(p, p0 + t * TP, p0 + t * TP + TP > p.it.lim0);
         r.values([&](int u, auto &x) {
 #pragma unroll
             for (int e = 0; e < S::VE; e++) x[e] = __builtin_bit_cast(typename Rows<T, NB, FULL, MT>::VU, vr[e][u]);
@@ -762,7 +778,7 @@ __device__ __forceinline__ void run_shared(const PageAttnArgs &a, const Piece &p
             lds_read(kr, at);
             r.template scores<4 * G / H, 4 * (G + 1) / H>([&](int h, int j) { return kr[j * H + h - 4 * G]; });
         });
-        r.weights(tp, tp + TP > p.it.lim0);
+        r.weights(p, tp, tp + TP > p.it.lim0);
         r.values([&](int u, auto &x) __attribute__((always_inline)) {
             constexpr int VE = S::VE;
             unsigned at[VE];

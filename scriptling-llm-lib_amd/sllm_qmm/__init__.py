@@ -61,6 +61,18 @@ class AttnParams(C.Structure):
                 ("q_norm_w", C.c_void_p), ("k_norm_w", C.c_void_p), ("norm_eps", C.c_float)]
 
 
+class LogitsParams(C.Structure):
+    """sllm_logits_params: device pointers and counts."""
+    _fields_ = [("rules", C.c_void_p), ("n_rules", C.c_int), ("history", C.c_void_p), ("n_history", C.c_int),
+                ("bias_tokens", C.c_void_p), ("bias_values", C.c_void_p), ("n_biases", C.c_int), ("masks", C.c_void_p),
+                ("n_masks", C.c_int), ("mask_ids", C.c_void_p), ("tokens", C.c_void_p)]
+
+
+# sllm_logits_rule: rules are made on the host as an array of this type and copied to the device
+LOGITS_RULE = np.dtype([("repeat", "<f4"), ("frequency", "<f4"), ("presence", "<f4"), ("history_at", "<i4"),
+                        ("history", "<i4"), ("bias_at", "<i4"), ("biases", "<i4"), ("reserved", "<i4")])
+
+
 def lib() -> C.CDLL:
     """Load libsllm_qmm.so (raises if it has not been built)."""
     global _lib
@@ -132,6 +144,10 @@ def lib() -> C.CDLL:
     L.sllm_page_batch_create.argtypes = [P, i32, i32, i32, C.POINTER(P)]
     L.sllm_page_batch_destroy.argtypes = [P]
     L.sllm_page_batch_begin.argtypes = [P, I, I, i32, P]
+    L.sllm_page_batch_begin_tree.argtypes = [P, I, I, i32, I, P]
+    L.sllm_page_accept_dev.argtypes = [P] * 7
+    L.sllm_page_keep_dev.argtypes = [P, P, P]
+    L.sllm_logits_rules_dev.argtypes = [P, i32, i32, C.POINTER(LogitsParams), P, P, P, P]
     L.sllm_page_attention_dev.argtypes = [P, i32, C.POINTER(AttnParams), P, P, P, P, P]
     L.sllm_lora_set_create.argtypes = [i32, i32, i32, i32, i32, C.POINTER(P)]
     L.sllm_lora_set_destroy.argtypes = [P]
@@ -593,6 +609,16 @@ class PageBatch:
             raise SllmError(1, "seqs and rows differ in length")
         _check(lib().sllm_page_batch_begin(self.handle, _ints(seqs), _ints(rows), len(seqs), C.c_void_p(stream)))
 
+    def begin_tree(self, seqs: list, rows: list, parents: list, stream: int = 0) -> None:
+        """A step of drafted tokens: rows[i] rows for sequence seqs[i], each continuing the row parents[..] of its
+        sequence's (-1: the sequence's last row before the step). parents: of all sequences, one after the other."""
+        if len(seqs) != len(rows):
+            raise SllmError(1, "seqs and rows differ in length")
+        if len(parents) != sum(rows):
+            raise SllmError(1, "parents must name a row for each of the step's")
+        _check(lib().sllm_page_batch_begin_tree(self.handle, _ints(seqs), _ints(rows), len(seqs), _ints(parents),
+                                                C.c_void_p(stream)))
+
 
 def page_attention_dev(batch: PageBatch, layer: int, params: AttnParams, q_ptr: int, k_ptr: int, v_ptr: int,
                        out_ptr: int, stream: int = 0) -> None:
@@ -600,6 +626,28 @@ def page_attention_dev(batch: PageBatch, layer: int, params: AttnParams, q_ptr: 
     sequence, one sequence after the other."""
     _check(lib().sllm_page_attention_dev(batch.handle, layer, C.byref(params), C.c_void_p(q_ptr), C.c_void_p(k_ptr),
                                          C.c_void_p(v_ptr), C.c_void_p(out_ptr), C.c_void_p(stream)))
+
+
+def page_accept_dev(batch: PageBatch, tokens_ptr: int, chosen_ptr: int, kept_ptr: int, counts_ptr: int, next_ptr: int,
+                    stream: int = 0) -> None:
+    """The path of the step's rows that the tokens chosen behind each row accept: per sequence its rows (kept), their
+    number and the token chosen behind the last."""
+    _check(lib().sllm_page_accept_dev(batch.handle, *(C.c_void_p(p) for p in (tokens_ptr, chosen_ptr, kept_ptr, counts_ptr,
+                                                                            next_ptr, stream))))
+
+
+def page_keep_dev(batch: PageBatch, kept_ptr: int, stream: int = 0) -> None:
+    """The accepted rows (page_accept_dev) moved to the front of their sequences' new rows, in every layer; the
+    sequences are then cut (PageCache.truncate)."""
+    _check(lib().sllm_page_keep_dev(batch.handle, C.c_void_p(kept_ptr), C.c_void_p(stream)))
+
+
+def logits_rules_dev(logits_ptr: int, rows: int, vocab: int, params: LogitsParams, dst_ptr: int, chosen_ptr: int,
+                     batch: PageBatch | None = None, stream: int = 0) -> None:
+    """Penalties for repeated tokens, biases and masks of rows of logits (dst; 0: not wanted), and the greedy token of
+    each row (chosen; 0: not wanted). With a batch the rows are those of its step."""
+    _check(lib().sllm_logits_rules_dev(C.c_void_p(logits_ptr), rows, vocab, C.byref(params), C.c_void_p(dst_ptr),
+                                       C.c_void_p(chosen_ptr), batch.handle if batch else None, C.c_void_p(stream)))
 
 
 class LoraSet:
