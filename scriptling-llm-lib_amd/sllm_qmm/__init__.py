@@ -632,22 +632,21 @@ def page_accept_dev(batch: PageBatch, tokens_ptr: int, chosen_ptr: int, kept_ptr
                     stream: int = 0) -> None:
     """The path of the step's rows that the tokens chosen behind each row accept: per sequence its rows (kept), their
     number and the token chosen behind the last."""
-    _check(lib().sllm_page_accept_dev(batch.handle, *(C.c_void_p(p) for p in (tokens_ptr, chosen_ptr, kept_ptr, counts_ptr,
-                                                                            next_ptr, stream))))
+    _check(lib().sllm_page_accept_dev(batch.handle, tokens_ptr, chosen_ptr, kept_ptr, counts_ptr, next_ptr, stream))
 
 
 def page_keep_dev(batch: PageBatch, kept_ptr: int, stream: int = 0) -> None:
     """The accepted rows (page_accept_dev) moved to the front of their sequences' new rows, in every layer; the
     sequences are then cut (PageCache.truncate)."""
-    _check(lib().sllm_page_keep_dev(batch.handle, C.c_void_p(kept_ptr), C.c_void_p(stream)))
+    _check(lib().sllm_page_keep_dev(batch.handle, kept_ptr, stream))
 
 
 def logits_rules_dev(logits_ptr: int, rows: int, vocab: int, params: LogitsParams, dst_ptr: int, chosen_ptr: int,
                      batch: PageBatch | None = None, stream: int = 0) -> None:
     """Penalties for repeated tokens, biases and masks of rows of logits (dst; 0: not wanted), and the greedy token of
     each row (chosen; 0: not wanted). With a batch the rows are those of its step."""
-    _check(lib().sllm_logits_rules_dev(C.c_void_p(logits_ptr), rows, vocab, C.byref(params), C.c_void_p(dst_ptr),
-                                       C.c_void_p(chosen_ptr), batch.handle if batch else None, C.c_void_p(stream)))
+    _check(lib().sllm_logits_rules_dev(logits_ptr, rows, vocab, C.byref(params), dst_ptr, chosen_ptr,
+                                       batch.handle if batch else None, stream))
 
 
 class LoraSet:
