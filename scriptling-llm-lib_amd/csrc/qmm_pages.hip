@@ -248,23 +248,41 @@ struct PieceCost {
         }
         state = 8.0 * (c.d_k + 2) * c.n_kv / read;
     }
+    // `x`: workgroups over those that run at a time. Fewer than CUs have more of the memory's rate each, but products do not end
+    // sooner for that (32 / 8 heads of 128, f16: a tile of 128 rows 1.5 us alone on a CU, 1.85 beside another; of 64 1.1, 1.15).
+    double time(int shape, double x) const {
+        static constexpr double least[3] = {0.27, 0.8, 0.6};
+        return tile[shape] * (x >= 0.5 ? 1.0 : std::max(least[shape], x));
+    }
 };
 
 // The segments' blocks and pieces: of a few lengths around a share of all the step's tiles the one whose pieces, taken by
-// workgroups one after the other, are estimated to end first; and no more states than the batch has room for. Returns
+// workgroups one after the other, are estimated to end first; and no more states than the batch has room for. Where CUs are left
+// without a workgroup also of smaller blocks than the rows fill, which read K and V more often. Returns
 // the number of pieces (for one kv head). (32 / 8 heads of 128; the longest share that all workgroups take at once, and
 // so chosen, us: f32, 64 sequences on a prefix of 4000 85.7, 70.8; 16 on 8000 48.8, 44.9; 5 prompts of 211 rows 161,
-// 147; f16, the 64 39.3, 35.2; others within 1. A step's begin with all of this takes the host 12 us for 16 sequences, 30 for
+// 147; f16, the 64 39.3, 35.2; others within 1. The largest block, and so chosen: a tree of 61 rows behind 1000, f16 24.3, 20.4;
+// f32 37.2, 28.1; of 16 behind 300, f32 22.2, 19.2. A step's begin with all of this takes the host 12 us for 16 sequences, 30 for
 // 64 on a prefix of 4000 in pages of 64, 90 on one of 16000 in pages of 16, 105 for 256 on 4000.)
 int cut(const PageCache &c, Plan *plan, int rep, int slots) {
     const int *most = kShapeRows[shape_class(c.d_k, c.type == SLLM_CACHE_F16)], n_kv = c.n_kv;
+    const PieceCost cost(c, most);
     int64_t all = 0;
-    for (Segment &s : plan->segs) {
-        const int64_t nv = (int64_t)s.ntok * rep;
-        s.shape = nv <= most[0] ? 0 : nv <= most[1] || !most[2] ? 1 : 2;
-        s.block = most[s.shape] / rep;
-        all += (int64_t)((s.ntok + s.block - 1) / s.block) * ((s.p1 - s.p0 + kPieceTile - 1) / kPieceTile);
-    }
+    // blocks of at most the shape `cap`; false where that is no other choice than before
+    auto shapes = [&](int cap) {
+        bool other = false;
+        all = 0;
+        for (Segment &s : plan->segs) {
+            const int64_t nv = (int64_t)s.ntok * rep;
+            int shape = nv <= most[0] ? 0 : nv <= most[1] || !most[2] ? 1 : 2;
+            shape = std::min(shape, std::max(cap, most[0] ? 0 : 1));
+            other |= shape != s.shape || !s.block;
+            s.shape = shape;
+            s.block = most[shape] / rep;
+            all += (int64_t)((s.ntok + s.block - 1) / s.block) * ((s.p1 - s.p0 + kPieceTile - 1) / kPieceTile);
+        }
+        return other;
+    };
     // pieces of up to `tiles` tiles: how many, and their states
     int64_t used = 0;
     auto pieces = [&](int64_t tiles) {
@@ -281,38 +299,47 @@ int cut(const PageCache &c, Plan *plan, int rep, int slots) {
         }
         return items;
     };
-    const int64_t share = std::max<int64_t>(kLeastTiles, (all * n_kv + kTargetPieces - 1) / kTargetPieces);
-    const PieceCost cost(c, most);
     std::vector<double> busy;
     auto estimate = [&](int64_t items) {
-        // fewer workgroups than CUs have more of the card each; a launch merges states where there are any (one row, 130
-        // positions of 9 / 3 heads of 64: 10.0 us in two pieces, 7.9 in one)
-        const double x = (double)items * n_kv / kTargetPieces, load = x >= 0.5 ? 1.0 : std::max(0.27, x);
+        // (a launch merges states where there are any: one row, 130 positions of 9 / 3 heads of 64 10.0 us in two pieces, 7.9
+        // in one)
+        const double x = (double)items * n_kv / kTargetPieces;
         busy.assign((size_t)std::max(1, kTargetPieces / n_kv), 0.0);  // a heap, the first to be free on top
         double end = 0.0;
-        for (const Segment &s : plan->segs)
+        for (const Segment &s : plan->segs) {
+            const double tile = cost.time(s.shape, x);
             for (int i = 0; i < s.pieces; i++) {
                 const int at = s.p0 + i * s.piece, n = (std::min(s.p1 - at, s.piece) + kPieceTile - 1) / kPieceTile;
-                const double t = cost.piece + n * load * cost.tile[s.shape];
+                const double t = cost.piece + n * tile;
                 for (int k = 0; k < s.ntok; k += s.block) {
                     std::pop_heap(busy.begin(), busy.end(), std::greater<>());
                     end = std::max(end, busy.back() += t);
                     std::push_heap(busy.begin(), busy.end(), std::greater<>());
                 }
             }
+        }
         return end + (used ? cost.merge : 0.0) + (double)used * cost.state;
     };
-    int64_t tiles = share;
+    int64_t tiles = 0;
+    int cap = 2;
     double best = -1.0;
-    for (const int64_t eighths : {4, 5, 6, 7, 8, 9, 10, 11, 12, 14, 16, 20}) {
-        const int64_t t = std::max<int64_t>(kLeastTiles, share * eighths / 8);
-        const int64_t n = pieces(t);
-        if (used > slots) continue;
-        const double e = estimate(n);
-        if (best >= 0.0 && e >= best) continue;
-        best = e;
-        tiles = t;
+    for (int k = 2; k >= 0; k--) {
+        if (!shapes(k) && k < 2) continue;
+        const int64_t share = std::max<int64_t>(kLeastTiles, (all * n_kv + kTargetPieces - 1) / kTargetPieces);
+        if (!tiles) tiles = share;
+        for (const int64_t eighths : {4, 5, 6, 7, 8, 9, 10, 11, 12, 14, 16, 20}) {
+            const int64_t t = std::max<int64_t>(kLeastTiles, share * eighths / 8);
+            const int64_t n = pieces(t);
+            // (smaller blocks than a segment's rows fill: while every workgroup has a CU for itself)
+            if (used > slots || (k < 2 && n * n_kv > kTargetPieces / 2)) continue;
+            const double e = estimate(n);
+            if (best >= 0.0 && e >= best) continue;
+            best = e;
+            tiles = t;
+            cap = k;
+        }
     }
+    shapes(cap);
     int64_t items = pieces(tiles);
     // (with one piece each the states fit: kMaxParts for every row)
     while (used > slots) items = pieces(tiles *= 2);
@@ -971,6 +998,7 @@ sllm_status sllm_page_attention_dev(sllm_page_batch *batch, int layer, const sll
     a.step = b.dev;
     a.qrot = b.qrot;
     a.qscale = b.qrot + (size_t)b.max_rows * b.n_heads * c.d_k;
+    a.rows_at = capture ? -1 : b.rows_at;
     a.part = b.part;
     a.ml = b.ml;
     a.slots = b.slots;

@@ -139,6 +139,7 @@ struct PageAttnArgs {
     float scale_log2;       // log2(e) / sqrt(d_k)
     char *pool_k, *pool_v;  // this layer
     const int *step;
+    int rows_at;            // as in the step's header; -1: as that says, where the step may also have fewer rows than the launch
     float *qrot, *qscale, *part, *ml;
     int slots;
     bool wide;                  // blocks of the first shape may have more than 16 rows

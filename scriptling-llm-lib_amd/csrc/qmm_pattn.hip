@@ -36,6 +36,11 @@ __device__ __forceinline__ void put4(_Float16 *dst, v4f x) {
     *(v4h *)dst = v4h{(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3]};
 }
 
+// The step's rows. (By value where the launch is the step's own: a read of memory less before everything else.)
+__device__ __forceinline__ const StepRow *step_rows(const PageAttnArgs &a) {
+    return (const StepRow *)(a.step + (a.rows_at >= 0 ? a.rows_at : a.step[kStepRowsAt]));
+}
+
 // A rotated q head (row pair of a.qrot: d_k floats) as the attention takes it. f32: as it is. f16 caches: two f16
 // values for each element, d_k leading parts, then d_k rests (together within 2^-23 of it or 2^-35 of the head's largest
 // element, whichever is more), of the head times a power of two that puts its largest element between 2^10 and 2^11, so
@@ -75,8 +80,8 @@ __global__ void __launch_bounds__(kPrepThreads) page_prep_kernel(PageAttnArgs a)
     __shared__ float rc[kMaxDk / 2], rs[kMaxDk / 2];
     constexpr int HG = kPrepThreads / LP;
     const int r = blockIdx.x, sub = threadIdx.x % LP;
-    if (r >= a.step[kStepRows]) return;
-    const StepRow &row = ((const StepRow *)(a.step + a.step[kStepRowsAt]))[r];
+    if (a.rows_at < 0 && r >= a.step[kStepRows]) return;
+    const StepRow &row = step_rows(a)[r];
     const int dk = a.d_k, d = 4 * sub, page_rows = 1 << a.shift;
     auto at_of = [&](int t) {
         return t < a.n_heads ? ((size_t)r * a.n_heads + t) * dk + d : ((size_t)r * a.n_kv + t - a.n_heads) * dk + d;
@@ -304,6 +309,7 @@ struct Rows : Shape<T, NB, FULL, VM> {
     v8h qh[F16 ? MT : 1][F16 ? KS : 1], ql[F16 ? MT : 1][F16 ? KS : 1];
     float sc[MT], m[MT], l[MT];
     int lim[MT];  // positions from here on are not seen; of a tree: what the row sees of it (StepRow)
+    unsigned sees[MT];  // of a tree: the tile's positions that the row sees, a bit for each
     v4f o[MT][NT], s[MT][H];
 
     // rows v0 .. of the block (those past its end repeat the last)
@@ -338,6 +344,7 @@ struct Rows : Shape<T, NB, FULL, VM> {
             }
             m[mt] = -INFINITY;
             l[mt] = 0.0f;
+            sees[mt] = 0;
 #pragma unroll
             for (int t = 0; t < NT; t++) o[mt][t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
         }
@@ -353,44 +360,68 @@ struct Rows : Shape<T, NB, FULL, VM> {
     template <int J0, int J1, class K>
     __device__ __forceinline__ void scores(K k) {
 #pragma unroll
-        for (int j = J0; j < J1; j++)
+        for (int j = J0; j < J1; j++) {
+            v4u kw[H];
 #pragma unroll
-            for (int h = 0; h < H; h++) {
-                const v4u kw = k(h, j);
+            for (int h = 0; h < H; h++) kw[h] = k(h, j);
+            // (an instruction's result is the next one's addend only after those of the other halves and rows)
+            if constexpr (F16) {
 #pragma unroll
-                for (int mt = 0; mt < MT; mt++) {
-                    if constexpr (F16) {
-                        const v8h x = __builtin_bit_cast(v8h, kw);
-                        s[mt][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, qh[mt][j], s[mt][h], 0, 0, 0);
-                        s[mt][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, ql[mt][j], s[mt][h], 0, 0, 0);
-                    } else {
-                        const v4f x = __builtin_bit_cast(v4f, kw);
+                for (int p = 0; p < 2; p++)
 #pragma unroll
-                        for (int c = 0; c < 4; c++)
-                            s[mt][h] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[c], qf[mt][j][c], s[mt][h], 0, 0, 0);
-                    }
-                }
+                    for (int h = 0; h < H; h++)
+#pragma unroll
+                        for (int mt = 0; mt < MT; mt++)
+                            s[mt][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, kw[h]), p ? ql[mt][j] : qh[mt][j],
+                                                                              s[mt][h], 0, 0, 0);
+            } else {
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+#pragma unroll
+                    for (int h = 0; h < H; h++)
+#pragma unroll
+                        for (int mt = 0; mt < MT; mt++)
+                            s[mt][h] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(v4f, kw[h])[c], qf[mt][j][c], s[mt][h], 0, 0, 0);
             }
+        }
     }
 
+    // What rows of a tree see of the tile at position tp, asked for before the tile's scores are formed. (Tiles begin at
+    // multiples of 16 positions, as the rows' elements of 16 bits; the one behind the tree's last is 0.)
+    __device__ __forceinline__ void look(const Piece &p, int tp) {
+        if (!(p.it.flags & kItemTree) || tp + TP <= p.it.lim0) return;
+        const int half = (tp >> 4) - (p.it.lim0 >> 4);
+        const uint16_t *from = (const uint16_t *)p.step + (half < 0 ? 0 : half);
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++) {
+            if constexpr (H == 1) {
+                sees[mt] = from[lim[mt]];
+            } else if (half < 0) {
+                sees[mt] = 0xffffu | (unsigned)from[lim[mt]] << 16;
+            } else {
+                __builtin_memcpy(&sees[mt], from + lim[mt], 4);
+            }
+        }
+    }
     // scores to weights, for the tile at position tp (masked: some row does not see all of it)
+    template <bool LOOK>
     __device__ __forceinline__ void weights(const Piece &p, int tp, bool masked) {
         if (masked) {
+
             int lane = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
             asm volatile("" : "+v"(lane));
             const int qd = lane >> 4;
             if (p.it.flags & kItemTree) {
-                // (tiles begin at multiples of 16 positions, as the rows' bits; those behind the tree's last 16 are 0)
                 const int half = (tp >> 4) - (p.it.lim0 >> 4);
 #pragma unroll
                 for (int mt = 0; mt < MT; mt++)
 #pragma unroll
                     for (int h = 0; h < H; h++) {
-                        if (half + h < 0) continue;
-                        const unsigned sees = ((const uint16_t *)p.step)[lim[mt] + half + h] >> (4 * qd);
+                        if (LOOK && half + h < 0) continue;
+                        const unsigned bits = LOOK ? (unsigned)((const uint16_t *)p.step)[lim[mt] + half + h] >> 4 * qd : sees[mt] >> (16 * h + 4 * qd);
 #pragma unroll
                         for (int i = 0; i < 4; i++)
-                            if (!(sees >> i & 1)) s[mt][h][i] = -INFINITY;
+                            if (!(bits >> i & 1)) s[mt][h][i] = -INFINITY;
                     }
             } else
 #pragma unroll
@@ -458,19 +489,26 @@ struct Rows : Shape<T, NB, FULL, VM> {
                 VU x[8];
                 v(u, x);
 #pragma unroll
-                for (int c = 0; c < VW; c++) {
-                    // the eight rows' element c of the lane's run
-                    v4u w;
+                for (int g = 0; g < VW; g += 4) {
+                    // the eight rows' elements g .. g + 3 of the lane's run
+                    v8h va[4];
 #pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        w[i] = __builtin_amdgcn_perm(x[2 * i + 1][c / 2], x[2 * i][c / 2], c & 1 ? 0x07060302u : 0x05040100u);
-                    const v8h va = __builtin_bit_cast(v8h, w);
+                    for (int c = 0; c < 4; c++) {
+                        v4u w;
 #pragma unroll
-                    for (int mt = 0; mt < MT; mt++) {
-                        v4f &d = o[mt][VW * u + c];
-                        d = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, ph[mt], d, 0, 0, 0);
-                        d = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl[mt], d, 0, 0, 0);
+                        for (int i = 0; i < 4; i++)
+                            w[i] = __builtin_amdgcn_perm(x[2 * i + 1][(g + c) / 2], x[2 * i][(g + c) / 2], c & 1 ? 0x07060302u : 0x05040100u);
+                        va[c] = __builtin_bit_cast(v8h, w);
                     }
+#pragma unroll
+                    for (int p = 0; p < 2; p++)
+#pragma unroll
+                        for (int c = 0; c < 4; c++)
+#pragma unroll
+                            for (int mt = 0; mt < MT; mt++) {
+                                v4f &d = o[mt][VW * u + g + c];
+                                d = __builtin_amdgcn_mfma_f32_16x16x32_f16(va[c], p ? pl[mt] : ph[mt], d, 0, 0, 0);
+                            }
                 }
             }
         } else {
@@ -657,10 +695,11 @@ __device__ __forceinline__ void run_split(const PageAttnArgs &a, const Piece &p,
     auto step = [&](int i, auto more) __attribute__((always_inline)) {
         constexpr bool MORE = decltype(more)::value;
         const int t = t0 + i * kWaves;
+        if constexpr (MT == 1) r.look(p, p0 + t * TP);  // (else later: there are no more registers beside the scores')
         r.no_scores();
         r.template scores<0, KS>([&](int h, int j) { return kr[h][j]; });
         if constexpr (MORE) load_k(t + kWaves);
-        r.weights(p, p0 + t * TP, p0 + t * TP + TP > p.it.lim0);
+        r.template weights<(MT > 1)>(p, p0 + t * TP, p0 + t * TP + TP > p.it.lim0);
         r.values([&](int u, auto &x) {
 #pragma unroll
             for (int e = 0; e < S::VE; e++) x[e] = __builtin_bit_cast(typename Rows<T, NB, FULL, MT>::VU, vr[e][u]);
@@ -752,19 +791,30 @@ __device__ __forceinline__ void run_shared(const PageAttnArgs &a, const Piece &p
     const int run = run_of(col);
     unsigned ka = base + col * RB + (qd ^ (col & (X - 1))) * 16;
     unsigned va = base + TP * RB + 4 * qd * RB + (run / VP ^ (4 * qd & (X - 1))) * 16 + run % VP * (16 / VP);
-    for (int t = 0; t < n; t++) {
-        // this tile's loads have landed when those of the ones behind it may be under way, everybody's behind the
-        // barrier; nobody reads the stage before it any more either
+    // before tile t: its loads have landed when those of the ones behind it may be under way, everybody's behind the
+    // barrier; nobody reads the stage before it any more either
+    auto turn = [&](int t) __attribute__((always_inline)) {
         constexpr int behind = (ST - 2) * 2 * IN;
         __builtin_amdgcn_s_waitcnt((behind & 15) | (behind >> 4 << 14) | 0x0f70);
         __builtin_amdgcn_s_barrier();
         asm volatile("" : "+v"(ka), "+v"(va), "+v"(fl) : : "memory");
         fill(t + ST - 1, ST - 1);
         pages(t + ST, ST - 1);
+    };
+    if (v0 >= nv) {
+        // (a loop of its own: with a way around the products in it the sums were copied for every tile)
+        for (int t = 0; t < n; t++) turn(t);
+        __syncthreads();
+        return;
+    }
+    for (int t = 0; t < n; t++) {
         const int tp = p0 + t * TP;
-        if (v0 >= nv) continue;
+        r.look(p, tp);  // (what is under way beside the ring's loads makes the wait for them a longer one, never shorter)
+        turn(t);
         const unsigned st = (unsigned)(t % ST) * TB;
         r.no_scores();
+        // (products before the other waves' weights: 64 sequences of 32 rows 72.7 us without, 71.5)
+        if constexpr (S::F16) __builtin_amdgcn_s_setprio(1);
         // four pieces of K at a time
         each(std::make_integer_sequence<int, H * KS / 4>{}, [&](auto part) __attribute__((always_inline)) {
             constexpr int G = decltype(part)::value;
@@ -778,7 +828,9 @@ __device__ __forceinline__ void run_shared(const PageAttnArgs &a, const Piece &p
             lds_read(kr, at);
             r.template scores<4 * G / H, 4 * (G + 1) / H>([&](int h, int j) { return kr[j * H + h - 4 * G]; });
         });
-        r.weights(p, tp, tp + TP > p.it.lim0);
+        if constexpr (S::F16) __builtin_amdgcn_s_setprio(0);
+        r.template weights<false>(p, tp, tp + TP > p.it.lim0);
+        if constexpr (S::F16) __builtin_amdgcn_s_setprio(1);
         r.values([&](int u, auto &x) __attribute__((always_inline)) {
             constexpr int VE = S::VE;
             unsigned at[VE];
@@ -788,8 +840,8 @@ __device__ __forceinline__ void run_shared(const PageAttnArgs &a, const Piece &p
             lds_read(x, at);
         });
     }
+    __builtin_amdgcn_s_setprio(0);
     __syncthreads();  // nothing is on its way and no stage is read: they are free for the next piece
-    if (v0 >= nv) return;
     r.sum_up();
     const Results res(a, p);
     bool bad = false;
@@ -833,7 +885,7 @@ page_attn_kernel(PageAttnArgs a) {
     p.per_rep = 1.0f / (float)a.rep;
     p.dk = a.d_k;
     p.step = a.step;
-    p.rows = (const StepRow *)(a.step + step[kStepRowsAt]);
+    p.rows = step_rows(a);
     for (int w = blockIdx.x; w < n; w += gridDim.x) {
         p.tid = threadIdx.x;
         asm volatile("" : "+v"(p.tid));
@@ -868,8 +920,8 @@ __global__ void __launch_bounds__(256) page_combine_kernel(PageAttnArgs a) {
     const int x = blockIdx.x * P + threadIdx.x / (LP * G);
     const int r = x / a.n_heads, h = x - r * a.n_heads;
     // (G > 1: all of a workgroup's threads have the same pair)
-    if (r >= a.step[kStepRows]) return;
-    const StepRow row = ((const StepRow *)(a.step + a.step[kStepRowsAt]))[r];
+    if (r >= (a.rows_at < 0 ? a.step[kStepRows] : a.grid_rows)) return;
+    const StepRow row = step_rows(a)[r];
     if (row.direct) return;
     const int g = h / a.rep, j = h - g * a.rep;
     const size_t base = (size_t)g * a.slots + j;
