@@ -250,9 +250,9 @@ struct PieceCost {
     }
     // `x`: workgroups over those that run at a time. Fewer than CUs have more of the memory's rate each, but products do not end
     // sooner for that (32 / 8 heads of 128, f16: a tile of 128 rows 1.5 us alone on a CU, 1.85 beside another; of 64 1.1, 1.15).
-    double time(int shape, double x) const {
+    double time(int shape, int rows, double x) const {
         static constexpr double least[3] = {0.27, 0.8, 0.6};
-        return tile[shape] * (x >= 0.5 ? 1.0 : std::max(least[shape], x));
+        return tile[shape] * (x >= 0.5 ? 1.0 : std::max(rows <= 16 ? 0.5 * least[shape] : least[shape], x));
     }
 };
 
@@ -268,7 +268,8 @@ int cut(const PageCache &c, Plan *plan, int rep, int slots) {
     const int *most = kShapeRows[shape_class(c.d_k, c.type == SLLM_CACHE_F16)], n_kv = c.n_kv;
     const PieceCost cost(c, most);
     int64_t all = 0;
-    // blocks of at most the shape `cap`; false where that is no other choice than before
+    // blocks of at most the shape `cap` (-1: of 16 rows, what one instruction takes); false where that is no other choice than
+    // before
     auto shapes = [&](int cap) {
         bool other = false;
         all = 0;
@@ -276,9 +277,10 @@ int cut(const PageCache &c, Plan *plan, int rep, int slots) {
             const int64_t nv = (int64_t)s.ntok * rep;
             int shape = nv <= most[0] ? 0 : nv <= most[1] || !most[2] ? 1 : 2;
             shape = std::min(shape, std::max(cap, most[0] ? 0 : 1));
-            other |= shape != s.shape || !s.block;
+            const int block = (cap < 0 && shape == 0 ? 16 : most[shape]) / rep;
+            other |= std::min(block, s.ntok) != std::min(s.block, s.ntok);
             s.shape = shape;
-            s.block = most[shape] / rep;
+            s.block = block;
             all += (int64_t)((s.ntok + s.block - 1) / s.block) * ((s.p1 - s.p0 + kPieceTile - 1) / kPieceTile);
         }
         return other;
@@ -307,7 +309,7 @@ int cut(const PageCache &c, Plan *plan, int rep, int slots) {
         busy.assign((size_t)std::max(1, kTargetPieces / n_kv), 0.0);  // a heap, the first to be free on top
         double end = 0.0;
         for (const Segment &s : plan->segs) {
-            const double tile = cost.time(s.shape, x);
+            const double tile = cost.time(s.shape, std::min(s.block, s.ntok) * rep, x);
             for (int i = 0; i < s.pieces; i++) {
                 const int at = s.p0 + i * s.piece, n = (std::min(s.p1 - at, s.piece) + kPieceTile - 1) / kPieceTile;
                 const double t = cost.piece + n * tile;
@@ -323,7 +325,7 @@ int cut(const PageCache &c, Plan *plan, int rep, int slots) {
     int64_t tiles = 0;
     int cap = 2;
     double best = -1.0;
-    for (int k = 2; k >= 0; k--) {
+    for (int k = 2; k >= -1; k--) {
         if (!shapes(k) && k < 2) continue;
         const int64_t share = std::max<int64_t>(kLeastTiles, (all * n_kv + kTargetPieces - 1) / kTargetPieces);
         if (!tiles) tiles = share;
@@ -903,7 +905,7 @@ static sllm_status begin_step(sllm_page_batch *batch, const int *seqs, const int
         b.seqs_at = h[kStepSeqsAt];
         b.of_at = h[kStepOfAt];
         b.wide = false;
-        for (const Segment &s : plan.segs) b.wide |= s.shape == 0 && s.ntok * rep > 16;
+        for (const Segment &s : plan.segs) b.wide |= s.shape == 0 && std::min(s.block, s.ntok) * rep > 16;
         b.seqs.assign(seqs, seqs + count);
         b.versions.resize((size_t)count);
         b.counts.assign(rows, rows + count);

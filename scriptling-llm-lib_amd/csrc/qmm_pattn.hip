@@ -309,7 +309,6 @@ struct Rows : Shape<T, NB, FULL, VM> {
     v8h qh[F16 ? MT : 1][F16 ? KS : 1], ql[F16 ? MT : 1][F16 ? KS : 1];
     float sc[MT], m[MT], l[MT];
     int lim[MT];  // positions from here on are not seen; of a tree: what the row sees of it (StepRow)
-    unsigned sees[MT];  // of a tree: the tile's positions that the row sees, a bit for each
     v4f o[MT][NT], s[MT][H];
 
     // rows v0 .. of the block (those past its end repeat the last)
@@ -344,7 +343,6 @@ struct Rows : Shape<T, NB, FULL, VM> {
             }
             m[mt] = -INFINITY;
             l[mt] = 0.0f;
-            sees[mt] = 0;
 #pragma unroll
             for (int t = 0; t < NT; t++) o[mt][t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
         }
@@ -386,25 +384,7 @@ struct Rows : Shape<T, NB, FULL, VM> {
         }
     }
 
-    // What rows of a tree see of the tile at position tp, asked for before the tile's scores are formed. (Tiles begin at
-    // multiples of 16 positions, as the rows' elements of 16 bits; the one behind the tree's last is 0.)
-    __device__ __forceinline__ void look(const Piece &p, int tp) {
-        if (!(p.it.flags & kItemTree) || tp + TP <= p.it.lim0) return;
-        const int half = (tp >> 4) - (p.it.lim0 >> 4);
-        const uint16_t *from = (const uint16_t *)p.step + (half < 0 ? 0 : half);
-#pragma unroll
-        for (int mt = 0; mt < MT; mt++) {
-            if constexpr (H == 1) {
-                sees[mt] = from[lim[mt]];
-            } else if (half < 0) {
-                sees[mt] = 0xffffu | (unsigned)from[lim[mt]] << 16;
-            } else {
-                __builtin_memcpy(&sees[mt], from + lim[mt], 4);
-            }
-        }
-    }
     // scores to weights, for the tile at position tp (masked: some row does not see all of it)
-    template <bool LOOK>
     __device__ __forceinline__ void weights(const Piece &p, int tp, bool masked) {
         if (masked) {
 
@@ -412,13 +392,15 @@ struct Rows : Shape<T, NB, FULL, VM> {
             asm volatile("" : "+v"(lane));
             const int qd = lane >> 4;
             if (p.it.flags & kItemTree) {
+                // (tiles begin at multiples of 16 positions, as the rows' elements; the one behind the tree's last is 0. Asked
+                // for before the scores, the bits came no sooner: 54.2 us against 53.9 behind 16000 rows)
                 const int half = (tp >> 4) - (p.it.lim0 >> 4);
 #pragma unroll
                 for (int mt = 0; mt < MT; mt++)
 #pragma unroll
                     for (int h = 0; h < H; h++) {
-                        if (LOOK && half + h < 0) continue;
-                        const unsigned bits = LOOK ? (unsigned)((const uint16_t *)p.step)[lim[mt] + half + h] >> 4 * qd : sees[mt] >> (16 * h + 4 * qd);
+                        if (half + h < 0) continue;
+                        const unsigned bits = (unsigned)((const uint16_t *)p.step)[lim[mt] + half + h] >> 4 * qd;
 #pragma unroll
                         for (int i = 0; i < 4; i++)
                             if (!(bits >> i & 1)) s[mt][h][i] = -INFINITY;
@@ -695,11 +677,10 @@ __device__ __forceinline__ void run_split(const PageAttnArgs &a, const Piece &p,
     auto step = [&](int i, auto more) __attribute__((always_inline)) {
         constexpr bool MORE = decltype(more)::value;
         const int t = t0 + i * kWaves;
-        if constexpr (MT == 1) r.look(p, p0 + t * TP);  // (else later: there are no more registers beside the scores')
         r.no_scores();
         r.template scores<0, KS>([&](int h, int j) { return kr[h][j]; });
         if constexpr (MORE) load_k(t + kWaves);
-        r.template weights<(MT > 1)>(p, p0 + t * TP, p0 + t * TP + TP > p.it.lim0);
+        r.weights(p, p0 + t * TP, p0 + t * TP + TP > p.it.lim0);
         r.values([&](int u, auto &x) {
 #pragma unroll
             for (int e = 0; e < S::VE; e++) x[e] = __builtin_bit_cast(typename Rows<T, NB, FULL, MT>::VU, vr[e][u]);
@@ -809,11 +790,10 @@ __device__ __forceinline__ void run_shared(const PageAttnArgs &a, const Piece &p
     }
     for (int t = 0; t < n; t++) {
         const int tp = p0 + t * TP;
-        r.look(p, tp);  // (what is under way beside the ring's loads makes the wait for them a longer one, never shorter)
         turn(t);
         const unsigned st = (unsigned)(t % ST) * TB;
         r.no_scores();
-        // (products before the other waves' weights: 64 sequences of 32 rows 72.7 us without, 71.5)
+        // (products before the other waves' weights: 32 trees of up to 32 rows 72.7 us without, 71.5; f32 no better)
         if constexpr (S::F16) __builtin_amdgcn_s_setprio(1);
         // four pieces of K at a time
         each(std::make_integer_sequence<int, H * KS / 4>{}, [&](auto part) __attribute__((always_inline)) {
@@ -829,7 +809,7 @@ __device__ __forceinline__ void run_shared(const PageAttnArgs &a, const Piece &p
             r.template scores<4 * G / H, 4 * (G + 1) / H>([&](int h, int j) { return kr[j * H + h - 4 * G]; });
         });
         if constexpr (S::F16) __builtin_amdgcn_s_setprio(0);
-        r.template weights<false>(p, tp, tp + TP > p.it.lim0);
+        r.weights(p, tp, tp + TP > p.it.lim0);
         if constexpr (S::F16) __builtin_amdgcn_s_setprio(1);
         r.values([&](int u, auto &x) __attribute__((always_inline)) {
             constexpr int VE = S::VE;
