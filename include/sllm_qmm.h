@@ -559,7 +559,7 @@ typedef struct sllm_logits_params {
  * batch (may be NULL): the rows are those of its step. Asynchronous on `stream`. Choosing
  * uses the stream's workspace (sllm_workspace_reserve; rows x (vocab / 512 + 64) bytes are enough); graphs captured on one
  * stream share it and must not overlap. A captured call with a batch follows its later steps as
- * sllm_page_attention_dev: `rows` then are those that the buffers hold, max_rows say.
+ * sllm_page_attention_dev: `rows` then has to be max_rows, as many as the buffers hold; a replay works on those of the step.
  */
 sllm_status sllm_logits_rules_dev(const float *logits_dev, int rows, int vocab, const sllm_logits_params *params,
                                   float *dst_dev, int *chosen_dev, const sllm_page_batch *batch, void *stream);

@@ -445,18 +445,20 @@ sllm_status sllm_logits_rules_dev(const float *logits, int rows, int vocab, cons
         if (vocab > (1 << 28)) return set_error(SLLM_ERR_SHAPE, "vocab must be at most 2^28");
         hipStream_t s = (hipStream_t)stream;
         LogitsArgs a{};
+        std::unique_lock<std::mutex> lb;  // (until the launches: the step that they are told of is then the batch's)
         if (batch) {
             PageBatch &b = const_cast<sllm_page_batch *>(batch)->b;
-            std::lock_guard<std::mutex> lb(b.mu);
+            lb = std::unique_lock<std::mutex>(b.mu);
             {
                 std::lock_guard<std::mutex> lk(b.c->mu);
                 const sllm_status st = step_stands(b);
                 if (st != SLLM_OK) return st;
             }
-            sllm_status st = on_device(b.c->device);
+            const sllm_status st = on_device(b.c->device);
             if (st != SLLM_OK) return st;
             const bool capture = stream_capturing(s);
-            if (capture ? rows < b.rows : rows != b.rows) return set_error(SLLM_ERR_SHAPE, "rows differ from those of the batch's step");
+            if (rows != (capture ? b.max_rows : b.rows))
+                return set_error(SLLM_ERR_SHAPE, capture ? "a captured call's rows are the batch's max_rows" : "rows differ from those of the batch's step");
             a.batch = true;
             a.follow = capture;
             a.step = step_ref(b, capture);

@@ -375,3 +375,10 @@ def test_refusals():
     with torch.cuda.graph(g, stream=st):
         assert status(lambda: batch.begin_tree([s], [1], [-1], st.cuda_stream)) == 1
     torch.cuda.synchronize()
+    # a captured call with a batch is for all rows that it may have
+    batch.begin_tree([s], [3], [-1, 0, 0])
+    g = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g, stream=st):
+        assert status(lambda: sq.logits_rules_dev(p, 3, 4, sq.LogitsParams(), 0, p, batch, st.cuda_stream)) == 3
+    torch.cuda.synchronize()
