@@ -168,7 +168,7 @@ __global__ void __launch_bounds__(kPrepThreads) page_prep_kernel(PageAttnArgs a)
 // A result that is not finite (a non-finite K or V element, also one that only other rows of the block
 // see, where the matrix instruction forms 0 * inf) is computed again, row by row, as the formula says.
 constexpr int kWaves = 4;
-constexpr int kFewPieces = 8;    // of a row, up to which one group of lanes merges them
+constexpr int kMergeThreads = 320000;  // of a launch that merges states, above which a pair has one group of lanes
 // log2 of the largest weight when m follows it, and from which on it follows
 template <class T>
 constexpr float kLead = sizeof(T) == 2 ? 13.0f : 0.0f;
@@ -888,24 +888,24 @@ page_attn_kernel(PageAttnArgs a) {
 }
 
 // The states of one (row, q head), merged by G groups of LP lanes of four dimensions, a group every G-th piece,
-// the groups' in LDS. Rows with one piece are written already. Bound by latency: one group takes
-// few pieces, eight long lists, four pieces' states in flight.
+// the groups' in LDS. Rows with one piece are written already. Bound by latency where there are few rows (long lists
+// are shared by groups, four pieces' states in flight), else by the states' bytes.
 template <int LP, int G>
 __global__ void __launch_bounds__(256) page_combine_kernel(PageAttnArgs a) {
     constexpr int P = 256 / (LP * G);  // pairs per workgroup
     constexpr int U = 4;
     __shared__ v4f os[G > 1 ? 256 : 1];
-    __shared__ v2f ss[G > 1 ? G : 1];
+    __shared__ v2f ss[G > 1 ? G * P : 1];
     const int sub = threadIdx.x % LP, grp = threadIdx.x / LP % G, d = sub * 4;
-    const int x = blockIdx.x * P + threadIdx.x / (LP * G);
+    const int pair = threadIdx.x / (LP * G), x = blockIdx.x * P + pair;
     const int r = x / a.n_heads, h = x - r * a.n_heads;
-    // (G > 1: all of a workgroup's threads have the same pair)
-    if (r >= (a.rows_at < 0 ? a.step[kStepRows] : a.grid_rows)) return;
-    const StepRow row = step_rows(a)[r];
-    if (row.direct) return;
+    bool live = r < (a.rows_at < 0 ? a.step[kStepRows] : a.grid_rows);
+    const StepRow row = step_rows(a)[live ? r : 0];
+    live = live && !row.direct;
+    if (G == 1 && !live) return;
     const int g = h / a.rep, j = h - g * a.rep;
     const size_t base = (size_t)g * a.slots + j;
-    const int n0 = row.parts[0].pieces, n1 = n0 + row.parts[1].pieces, all = n1 + row.parts[2].pieces;
+    const int n0 = row.parts[0].pieces, n1 = n0 + row.parts[1].pieces, all = live ? n1 + row.parts[2].pieces : 0;
     const int dc = d < a.d_k ? d : 0;
     float M = -INFINITY, L = 0.0f;
     v4f O = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -939,19 +939,20 @@ __global__ void __launch_bounds__(256) page_combine_kernel(PageAttnArgs a) {
     }
     if constexpr (G > 1) {
         os[threadIdx.x] = O;
-        if (sub == 0) ss[grp] = v2f{M, L};
+        if (sub == 0) ss[pair * G + grp] = v2f{M, L};
         __syncthreads();
-        if (grp) return;
+        if (grp || !live) return;
         float mn = M;
 #pragma unroll
-        for (int u = 1; u < G; u++) mn = fmaxf(mn, ss[u][0]);
+        for (int u = 1; u < G; u++) mn = fmaxf(mn, ss[pair * G + u][0]);
         const float f = M == -INFINITY ? 0.0f : exp2_(M - mn);
         L = L * f;
         O = O * f;
 #pragma unroll
         for (int u = 1; u < G; u++) {
-            const float w = ss[u][0] == -INFINITY ? 0.0f : exp2_(ss[u][0] - mn);
-            L = L + ss[u][1] * w;
+            const v2f s = ss[pair * G + u];
+            const float w = s[0] == -INFINITY ? 0.0f : exp2_(s[0] - mn);
+            L = L + s[1] * w;
             O = O + os[threadIdx.x + u * LP] * w;
         }
     }
@@ -988,10 +989,18 @@ sllm_status launch(const PageAttnArgs &a, hipStream_t s) {
     SLLM_HIP(hipGetLastError());
     if (!a.combine) return SLLM_OK;
     const int pairs = a.grid_rows * a.n_heads;
-    if (a.combine > kFewPieces)
-        hipLaunchKernelGGL((page_combine_kernel<LP, groups>), dim3(pairs), dim3(256), 0, s, a);
-    else
-        hipLaunchKernelGGL((page_combine_kernel<LP, 1>), dim3((pairs + groups - 1) / groups), dim3(256), 0, s, a);
+    // Groups of lanes to a pair: as many as have four pieces each, while the launch stays small (a captured one may meet any list).
+    // 8 rows of 32 heads, 60 pieces, us with one, two, four and eight: 54.4, 48.8, 46.5, 45.7 (attention in all); 64 rows, 13: 35.1,
+    // 34.3, 34.2, 35.0; 16 rows, 8: 32.1, 31.3, 31.7, 32.0; 700 rows, 3: 53.0, 53.7, 59.4, 65.7.
+    int g = groups;
+    while (a.combine != INT32_MAX && g > 1 && (4 * g > a.combine || (int64_t)pairs * g * LP > kMergeThreads)) g /= 2;
+    const dim3 grid((unsigned)((pairs + groups / g - 1) / (groups / g)));
+    switch (g) {
+    case 1: hipLaunchKernelGGL((page_combine_kernel<LP, 1>), grid, dim3(256), 0, s, a); break;
+    case 2: hipLaunchKernelGGL((page_combine_kernel<LP, 2>), grid, dim3(256), 0, s, a); break;
+    case 4: hipLaunchKernelGGL((page_combine_kernel<LP, 4>), grid, dim3(256), 0, s, a); break;
+    default: hipLaunchKernelGGL((page_combine_kernel<LP, groups>), grid, dim3(256), 0, s, a);
+    }
     SLLM_HIP(hipGetLastError());
     return SLLM_OK;
 }
