@@ -238,10 +238,10 @@ constexpr int kSpareStates = 8192; // of a kv head, beyond what a step's rows ne
 // when all workgroups run, and what a piece costs beside its tiles.
 struct PieceCost {
     double tile[3];  // by shape
-    double piece = 4.5, merge = 2.5;
+    double piece = 7.0, merge = 2.5;  // (q into registers, the first tiles, the states: 13400 cycles with 128 rows, 9200 with 64)
     double state;    // one row's state of all kv heads, written and read
     PieceCost(const PageCache &c, const int *most) {
-        const double read = 6.0e6, f16 = 0.4e9, f32 = 0.1e9;  // bytes, operations in a us
+        const double read = 6.0e6, f16 = 0.4e9, f32 = 0.13e9;  // bytes, operations in a us
         for (int i = 0; i < 3; i++) {
             const double bytes = 2.0 * kPieceTile * c.d_k * c.elem(), ops = 4.0 * kPieceTile * c.d_k * most[i];
             tile[i] = std::max(i ? 0.0 : bytes / read, ops / (c.elem() == 2 ? f16 : f32)) * kTargetPieces;
@@ -260,7 +260,7 @@ struct PieceCost {
 // workgroups one after the other, are estimated to end first; and no more states than the batch has room for. Where CUs are left
 // without a workgroup also of smaller blocks than the rows fill, which read K and V more often. Returns
 // the number of pieces (for one kv head). (32 / 8 heads of 128; the longest share that all workgroups take at once, and
-// so chosen, us: f32, 64 sequences on a prefix of 4000 85.7, 70.8; 16 on 8000 48.8, 44.9; 5 prompts of 211 rows 161,
+// so chosen, us: f32, 64 sequences on a prefix of 4000 85.7, 66.6; 16 on 8000 48.8, 44.9; 5 prompts of 211 rows 161,
 // 147; f16, the 64 39.3, 35.2; others within 1. The largest block, and so chosen: a tree of 61 rows behind 1000, f16 24.3, 20.4;
 // f32 37.2, 28.1; of 16 behind 300, f32 22.2, 19.2. A step's begin with all of this takes the host 12 us for 16 sequences, 30 for
 // 64 on a prefix of 4000 in pages of 64, 90 on one of 16000 in pages of 16, 105 for 256 on 4000.)
