@@ -43,16 +43,29 @@ struct LogitsArgs {
     int2 *best;  // of every row and chunk: the largest value's bits and its index
 };
 
-// The first of two candidates in value, then in index. (A NaN is never one.)
-__device__ __forceinline__ void better(float &v, int &i, float w, int j) {
-    if (w > v || (w == v && j < i)) {
-        v = w;
-        i = j;
-    }
+// The largest value and the lowest index of a wave, in all lanes: the lanes of a row of 16 among themselves, then the four rows'.
+template <class T, class F>
+__device__ __forceinline__ T wave_all(T v, F better) {
+    auto with = [&](auto moved) {
+        const T o = __builtin_bit_cast(T, moved);
+        v = better(o, v) ? o : v;
+    };
+    with(__builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0xb1, 0xf, 0xf, false));   // lane ^ 1
+    with(__builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x4e, 0xf, 0xf, false));   // lane ^ 2
+    with(__builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x141, 0xf, 0xf, false));  // the other quad of each 8 lanes
+    with(__builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x140, 0xf, 0xf, false));  // the other 8 lanes of each row
+    const int mine = __builtin_bit_cast(int, v);
+    v = __builtin_bit_cast(T, __builtin_amdgcn_readlane(mine, 0));
+    with(__builtin_amdgcn_readlane(mine, 16));
+    with(__builtin_amdgcn_readlane(mine, 32));
+    with(__builtin_amdgcn_readlane(mine, 48));
+    return v;
 }
-__device__ __forceinline__ void wave_best(float &v, int &i) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) better(v, i, __shfl_xor(v, o, 64), __shfl_xor(i, o, 64));
+__device__ __forceinline__ float wave_max(float v) {
+    return wave_all(v, [](float a, float b) { return a > b; });
+}
+__device__ __forceinline__ int wave_min(int v) {
+    return wave_all(v, [](int a, int b) { return a < b; });
 }
 
 // One workgroup per (row, chunk of the vocabulary), 4 V elements to a thread, which it holds in registers from the first
@@ -256,11 +269,7 @@ __global__ void __launch_bounds__(kRuleThreads) logits_rules_kernel(LogitsArgs a
 #pragma unroll
     for (int i = 0; i < 4 * V; i++) top = y[i] > top ? y[i] : top;
     const float own = top;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const float other = __shfl_xor(top, o, 64);
-        top = other > top ? other : top;
-    }
+    top = wave_max(top);
     if ((tid & 63) == 0) wv[tid >> 6] = top;
     lds_barrier();
 #pragma unroll
@@ -281,14 +290,20 @@ __global__ void __launch_bounds__(kRuleThreads) logits_rules_kernel(LogitsArgs a
 __global__ void __launch_bounds__(64) logits_choose_kernel(LogitsArgs a) {
     const int r = blockIdx.x;
     if (a.follow && r >= a.step.step[kStepRows]) return;
+    // (a lane's chunks ascend, and their indices)
     float v = -INFINITY;
     int i = INT_MAX;
     for (int c = threadIdx.x; c < a.chunks; c += 64) {
         const int2 b = a.best[(size_t)r * a.chunks + c];
-        better(v, i, __int_as_float(b.x), b.y);
+        const float x = __int_as_float(b.x);
+        if (x > v) {
+            v = x;
+            i = b.y;
+        }
     }
-    wave_best(v, i);
-    if (threadIdx.x == 0) a.chosen[r] = v == -INFINITY ? -1 : i;
+    const float top = wave_max(v);
+    i = wave_min(v == top ? i : INT_MAX);
+    if (threadIdx.x == 0) a.chosen[r] = top == -INFINITY ? -1 : i;
 }
 
 // ------------------------------------------------------- accepted paths ----
