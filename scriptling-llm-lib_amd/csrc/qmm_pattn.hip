@@ -919,7 +919,8 @@ __global__ void __launch_bounds__(256) page_combine_kernel(PageAttnArgs a) {
                            : c < n1 ? row.parts[1].first + (c - n0) * row.parts[1].step
                                     : row.parts[2].first + (c - n1) * row.parts[2].step;
             s[u] = *(const v2f *)(a.ml + (base + at) * 2);
-            o[u] = *(const v4f *)(a.part + (base + at) * a.d_k + dc);
+            // (each state is read once: 244 rows of 32 pieces 53.6 -> 52.2 us)
+            o[u] = __builtin_nontemporal_load((const v4f *)(a.part + (base + at) * a.d_k + dc));
         }
         float mn = M;
 #pragma unroll
