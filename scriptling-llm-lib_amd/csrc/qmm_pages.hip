@@ -267,12 +267,12 @@ struct PieceCost {
 int cut(const PageCache &c, Plan *plan, int rep, int slots) {
     const int *most = kShapeRows[shape_class(c.d_k, c.type == SLLM_CACHE_F16)], n_kv = c.n_kv;
     const PieceCost cost(c, most);
-    int64_t all = 0;
+    int64_t all = 0, blocks = 0;
     // blocks of at most the shape `cap` (-1: of 16 rows, what one instruction takes); false where that is no other choice than
     // before
     auto shapes = [&](int cap) {
         bool other = false;
-        all = 0;
+        all = blocks = 0;
         for (Segment &s : plan->segs) {
             const int64_t nv = (int64_t)s.ntok * rep;
             int shape = nv <= most[0] ? 0 : nv <= most[1] || !most[2] ? 1 : 2;
@@ -281,7 +281,9 @@ int cut(const PageCache &c, Plan *plan, int rep, int slots) {
             other |= std::min(block, s.ntok) != std::min(s.block, s.ntok);
             s.shape = shape;
             s.block = block;
-            all += (int64_t)((s.ntok + s.block - 1) / s.block) * ((s.p1 - s.p0 + kPieceTile - 1) / kPieceTile);
+            const int64_t n = (s.ntok + s.block - 1) / s.block;
+            blocks += n;
+            all += n * ((s.p1 - s.p0 + kPieceTile - 1) / kPieceTile);
         }
         return other;
     };
@@ -326,13 +328,14 @@ int cut(const PageCache &c, Plan *plan, int rep, int slots) {
     int cap = 2;
     double best = -1.0;
     for (int k = 2; k >= -1; k--) {
+        // (blocks of fewer rows than a segment has: while every workgroup has a CU for itself)
+        if (k < 2 && blocks * n_kv > kTargetPieces / 2) break;
         if (!shapes(k) && k < 2) continue;
         const int64_t share = std::max<int64_t>(kLeastTiles, (all * n_kv + kTargetPieces - 1) / kTargetPieces);
         if (!tiles) tiles = share;
         for (const int64_t eighths : {4, 5, 6, 7, 8, 9, 10, 11, 12, 14, 16, 20}) {
             const int64_t t = std::max<int64_t>(kLeastTiles, share * eighths / 8);
             const int64_t n = pieces(t);
-            // (smaller blocks than a segment's rows fill: while every workgroup has a CU for itself)
             if (used > slots || (k < 2 && n * n_kv > kTargetPieces / 2)) continue;
             const double e = estimate(n);
             if (best >= 0.0 && e >= best) continue;

@@ -495,6 +495,9 @@ LORA_TYPES = {"f32": 0, "f16": 1, "bf16": 2}
 
 
 def _ints(values):
+    if isinstance(values, np.ndarray):
+        values = np.ascontiguousarray(values, np.int32)
+        return values.ctypes.data_as(C.POINTER(C.c_int))  # (keeps the array)
     return (C.c_int * len(values))(*values)
 
 
@@ -611,7 +614,8 @@ class PageBatch:
 
     def begin_tree(self, seqs: list, rows: list, parents: list, stream: int = 0) -> None:
         """A step of drafted tokens: rows[i] rows for sequence seqs[i], each continuing the row parents[..] of its
-        sequence's (-1: the sequence's last row before the step). parents: of all sequences, one after the other."""
+        sequence's (-1: the sequence's last row before the step). parents: of all sequences, one after the other (an
+        int32 array is not copied)."""
         if len(seqs) != len(rows):
             raise SllmError(1, "seqs and rows differ in length")
         if len(parents) != sum(rows):
