@@ -29,7 +29,7 @@ StepRef step_ref(const PageBatch &b, bool capture) {
 
 // ----------------------------------------------------------------- logits ----
 
-// A workgroup's barrier for what it shares in LDS: __syncthreads also waits for all its loads and stores of memory.
+// A workgroup's barrier for what it shares in LDS; loads and stores of memory stay under way.
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 struct LogitsArgs {
@@ -69,13 +69,13 @@ __device__ __forceinline__ int wave_min(int v) {
 }
 
 // One workgroup per (row, chunk of the vocabulary), 4 V elements to a thread, which it holds in registers from the first
-// load to the store. The row's biases that lie in the chunk go into a table in LDS, an entry for each element, then
-// the counts of the row's tokens (its history, its node's path). Each workgroup reads all of its row's tokens: 32 chunks of
-// 4096 read 4000 of them from L2 in less than a microsecond. Bound by the bytes of the logits where there are many rows, by
-// the chain of loads (rule, tokens, elements) where there are few.
-// 64 rows of 128256, histories of up to 4000, 20 biases (67 MB): 17.4 us with the choice (28 with one value after the
-// other and both tables; 22.8 with the biases detected, counted and added in passes of their own, the heavy first
-// chunks all on one XCD). A table of the counted elements, worked off by a thread for each: 20.2.
+// load to the store. The row's biases that lie in the chunk go into a table in LDS, an entry for each element (of a token
+// named twice the later: the largest number), then, cleared, the counts of the row's tokens (its history, its node's path).
+// Each workgroup reads all of its row's tokens: 4000 tokens that are none of the vocabulary's cost 64 rows of 128256 1.9 us
+// beside the 14.1 of the logits alone. Bound by the bytes of the logits where there are many rows, by the chain of
+// loads (mask or rule, elements, tokens) where there are few.
+// 64 rows of 128256, histories of up to 4000, 20 biases (67 MB, 13 us at a copy's rate): 15.5 us with the choice. The counted
+// elements worked off from a list, a thread for each: 20.2; two tables, one value after the other: 30.8.
 constexpr int kRuleThreads = 256;
 template <int V>
 __global__ void __launch_bounds__(kRuleThreads) logits_rules_kernel(LogitsArgs a) {
@@ -87,9 +87,9 @@ __global__ void __launch_bounds__(kRuleThreads) logits_rules_kernel(LogitsArgs a
     const int r = blockIdx.y, tid = threadIdx.x;
     if (a.follow && r >= a.step.step[kStepRows]) return;
     const size_t row = (size_t)r * a.vocab;
-    // elements are numbered from the 16-byte boundary at or before the row's first, so that fours are aligned
-    // frequent tokens have low numbers: the rows' first chunks go to different XCDs
+    // frequent tokens have low numbers: the rows' first chunks go to different XCDs (22.6 -> 20.1 us at the time)
     const int chunk = (int)((blockIdx.x + blockIdx.y) % gridDim.x);
+    // elements are numbered from the 16-byte boundary at or before the row's first, so that fours are aligned
     const int lead = (int)(((uintptr_t)(a.x + row) >> 2) & 3), c0 = chunk * CH;
     const float *x = a.x + row - lead;
     float *dst = a.dst ? a.dst + row - lead : nullptr;
@@ -170,12 +170,8 @@ __global__ void __launch_bounds__(kRuleThreads) logits_rules_kernel(LogitsArgs a
     // tokens t0 .. t0 + nt - 1 are the chunk's, the first one's entry is i0
     const int t0 = max(c0 - lead, 0), nt = max(min(c0 - lead + CH, a.vocab) - t0, 0), i0 = t0 + lead - c0;
     auto mine = [&](int t) { return (unsigned)t - (unsigned)t0 < (unsigned)nt; };
-    // (The loops over a thread's fours stay loops: what few workgroups run costs them its length, as its instructions are not
-    // in the cache.)
-    typedef float Y __attribute__((ext_vector_type(4 * V)));
-    typedef int B __attribute__((ext_vector_type(4 * V)));
-    Y y;
-    B by;  // 1 + the number of the element's bias, 0 without one
+    float y[4 * V];
+    int by[4 * V];  // 1 + the number of the element's bias, 0 without one
     if (nb) {
         for (unsigned j = tid; j < nb; j += T) {
             const int t = bias_of[j];
@@ -227,7 +223,7 @@ __global__ void __launch_bounds__(kRuleThreads) logits_rules_kernel(LogitsArgs a
 #pragma unroll
     for (int i = 0; i < 4 * V; i++) y[i] = v[i / 4][i % 4];
     if ((nh || path) && some)
-#pragma unroll 1
+#pragma unroll
         for (int k = 0; k < V; k++) {
             const v4i n = ((const v4i *)table)[tid + k * T];
             if (!__ballot(n[0] | n[1] | n[2] | n[3])) continue;
@@ -241,7 +237,7 @@ __global__ void __launch_bounds__(kRuleThreads) logits_rules_kernel(LogitsArgs a
             for (int u = 0; u < 4; u++) y[4 * k + u] = z[u];
         }
     if (nb && biased)
-#pragma unroll 1
+#pragma unroll
         for (int i = 0; i < 4 * V; i++)
             if (by[i]) y[i] = y[i] + a.p.bias_values[b0 + by[i] - 1];
     if (!whole || masked)
@@ -252,8 +248,8 @@ __global__ void __launch_bounds__(kRuleThreads) logits_rules_kernel(LogitsArgs a
         for (int k = 0; k < V; k++) {
             const int e = c0 + 4 * (tid + k * T);
             if (aligned) {
-                // whole lines go past the caches (the kernel's instructions stay in L2: 19.2 -> 17.4 us); the rest of
-                // lines that were begun with -inf does not (16.4 -> 18.1)
+                // whole lines go past the caches (19.2 -> 17.4 us), the rest of lines that were begun with -inf does not
+                // (trees with masks 16.4, past them 18.1)
                 const v4f z = {y[4 * k], y[4 * k + 1], y[4 * k + 2], y[4 * k + 3]};
                 if (!masked) __builtin_nontemporal_store(z, (v4f *)(dst + e));
                 else if (ok >> 4 * k & 15) *(v4f *)(dst + e) = z;
@@ -309,7 +305,9 @@ __global__ void __launch_bounds__(64) logits_choose_kernel(LogitsArgs a) {
 // ------------------------------------------------------- accepted paths ----
 
 // One workgroup per sequence. A row follows its parent where it holds the token chosen behind it (of several such rows the
-// first); the path is the rows whose ancestors all follow.
+// first); the path is the rows whose ancestors all follow: each row looks whether a bit of those it sees is missing among the
+// bits of the rows that follow, so nothing walks from row to row (64 rows of a chain: 64 reads of LDS one after the other).
+// Bound by latency: two dependent loads behind the step's description; 2.7 us, 200 sequences of up to 64 rows 4.6.
 constexpr int kAcceptThreads = 256;
 __global__ void __launch_bounds__(kAcceptThreads) page_accept_kernel(StepRef st, const int *tokens, const int *chosen, int *kept,
                                                                      int *counts, int *next) {
@@ -390,7 +388,9 @@ struct KeepArgs {
 };
 
 // One workgroup per (sequence, K or V of a layer). A thread has one 16-byte column of a head and moves the path's rows
-// there in order: a row goes to a place at or before its own, so that nothing is overwritten before it has been read.
+// there in order, four loads before their stores: a row goes to a place at or before its own, so that nothing is overwritten
+// before it has been read. Bound by latency (path, places, rows: 3.6 us for one sequence of 30 layers) and the rows' bytes
+// (24 sequences of 32 layers, 31 MB read and written: 7.6 us).
 constexpr int kKeepThreads = 256;
 __global__ void __launch_bounds__(kKeepThreads) page_keep_kernel(KeepArgs a) {
     __shared__ int2 from[kKeepThreads], to[kKeepThreads];  // page and row of it
@@ -491,7 +491,7 @@ sllm_status sllm_logits_rules_dev(const float *logits, int rows, int vocab, cons
         if (!p->n_masks) a.p.masks = nullptr;
         // Chunks of 1024 while all of them run at once (eight workgroups to a CU), else of 4096, whose launch and tokens cost
         // less: 1 x 49152 7.5 us against 8.9, 7 x 32003 8.1 against 12.6, 16 x 128256 10.1 against 10.4; 32 x 128256 14.3
-        // against 12.4, 64 x 128256 25.4 against 19.2.
+        // against 12.4, 64 x 128256 25.4 against 19.2 (as the kernels were then, both sides alike).
         const int64_t small = 4 * kRuleThreads, n_small = ((int64_t)vocab + 3 + small - 1) / small;
         const bool four = n_small * rows > 2048;
         a.chunks = (int)(four ? (n_small + 3) / 4 : n_small);

@@ -263,3 +263,56 @@ def test_refusals():
     assert status(p, 65536, 4, none, p, p) == 3 and status(p, 1, (1 << 28) + 1, none, p, p) == 3
     sq.logits_rules_dev(p, 0, 4, none, p, p)
     torch.cuda.synchronize()
+
+
+def test_captured_calls_read_what_is_there():
+    """A graph replayed over other logits, rules and masks, with eager calls on the same stream between."""
+    rng = np.random.default_rng(8)
+    v, rows = 9001, 6
+    c, x = draw(v, rows, rng, 300, 10, 0.3)
+    st = torch.cuda.Stream()
+    sq.workspace_reserve(st.cuda_stream, 1 << 20)
+    src, dst = torch.zeros(rows, v, device="cuda"), torch.zeros(rows, v, device="cuda")
+    chosen = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=st):
+        sq.logits_rules_dev(src.data_ptr(), rows, v, c.params, dst.data_ptr(), chosen.data_ptr(), None, st.cuda_stream)
+    for i in range(4):
+        x = (rng.normal(size=(rows, v)) * 3).astype(F)
+        src.copy_(torch.from_numpy(x))
+        r = c.host.copy()
+        r["frequency"] = i / 4
+        c.keep["rules"].copy_(torch.from_numpy(r.view(np.int32)))
+        c.rules = [(a, i / 4, p, h, b) for a, _, p, h, b in c.rules]
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        for k in range(rows):
+            y, best = c.row(x[k], k, (), c.masks[k])
+            assert np.array_equal(dst[k].cpu().numpy(), y) and int(chosen[k]) == best
+        c.run(x[::-1].copy(), stream=st.cuda_stream)
+
+
+def test_two_threads():
+    """Calls of two threads, a stream each."""
+    import threading
+    rng = np.random.default_rng(12)
+    jobs = [(draw(30011, 9, rng, 700, 8, 0.2), torch.cuda.Stream()) for _ in range(2)]
+    torch.cuda.synchronize()
+    out = [[torch.zeros(9, dtype=torch.int32, device="cuda") for _ in range(20)] for _ in jobs]
+    src = [torch.from_numpy(x).cuda() for (_, x), _ in jobs]
+    torch.cuda.synchronize()
+
+    def work(i):
+        (c, x), st = jobs[i]
+        for o in out[i]:
+            sq.logits_rules_dev(src[i].data_ptr(), 9, 30011, c.params, 0, o.data_ptr(), None, st.cuda_stream)
+
+    t = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [a.start() for a in t]
+    [a.join() for a in t]
+    torch.cuda.synchronize()
+    for i, ((c, x), _) in enumerate(jobs):
+        want = [c.row(x[r], r, (), c.masks[r])[1] for r in range(9)]
+        assert all(o.tolist() == want for o in out[i])
