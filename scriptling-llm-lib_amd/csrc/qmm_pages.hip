@@ -722,6 +722,12 @@ static sllm_status begin_step(sllm_page_batch *batch, const int *seqs, const int
         PageCache &c = *b.c;
         std::lock_guard<std::mutex> lk(c.mu);
         int64_t total = 0, pages = 0, tree_ints = 0;
+        // (parents holds as many rows as these say: they are looked at first)
+        for (int i = 0; parents && i < count; i++) {
+            if (rows[i] < 0) return set_error(SLLM_ERR_ARG, "rows must not be negative");
+            if ((total += rows[i]) > b.max_rows) return set_error(SLLM_ERR_SHAPE, "more rows than max_rows");
+        }
+        total = 0;
         Plan plan;
         plan.tree.assign((size_t)count, 0);
         std::vector<int> sorted(seqs, seqs + count);

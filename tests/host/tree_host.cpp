@@ -5,6 +5,8 @@
 #include <set>
 #include <string>
 
+#include <sys/mman.h>
+
 #include "qmm_pages.hip"
 
 static std::string error;
@@ -171,6 +173,16 @@ static void refused() {
     CHECK(begin({3}, {-1, 2, 0}) == SLLM_ERR_ARG && same());  // a later one
     CHECK(begin({3}, {-2, 0, 0}) == SLLM_ERR_ARG && same());
     CHECK(begin({1, 2}, {-1, 0, 0}) == SLLM_ERR_ARG && same());  // (numbered within the sequence: its first cannot follow)
+    // parents with nothing readable behind them: as many as the rows say in all, but not in each sequence
+    char *guard = (char *)mmap(nullptr, 8192, PROT_READ | PROT_WRITE, MAP_PRIVATE | MAP_ANONYMOUS, -1, 0);
+    CHECK(guard != MAP_FAILED && mprotect(guard + 4096, 4096, PROT_NONE) == 0);
+    int *last_two = (int *)(guard + 4096) - 2;
+    last_two[0] = -1;
+    last_two[1] = 0;
+    const int signs[2] = {5, -3}, many[2] = {2, 1599};
+    CHECK(sllm_page_batch_begin_tree(b, s, signs, 2, last_two, nullptr) == SLLM_ERR_ARG && same());
+    CHECK(sllm_page_batch_begin_tree(b, s, many, 2, last_two, nullptr) == SLLM_ERR_SHAPE && same());
+    munmap(guard, 8192);
     const int two = 2, none = 0;
     CHECK(sllm_page_batch_begin_tree(b, s, &two, 1, nullptr, nullptr) == SLLM_ERR_ARG && same());
     CHECK(sllm_page_batch_begin_tree(b, s, &none, 1, nullptr, nullptr) == SLLM_OK && same());
