@@ -40,6 +40,19 @@ def test_parents_are_counted():
         assert e.value.status == 1
 
 
+@pytest.mark.parametrize("parents", [np.array([-1.0, 0.5]), np.zeros((2, 2), np.int32), np.zeros((2, 0), np.int32)])
+def test_arrays_of_other_kinds_are_refused(parents):
+    with pytest.raises(TypeError):
+        sq._ints(parents)
+
+
+@pytest.mark.parametrize("kind", [np.int32, np.int64, np.uint8])
+def test_arrays_of_integers(kind):
+    assert sq._ints(np.arange(12, dtype=kind)[::3])[:4] == [0, 3, 6, 9]
+    assert len(sq._ints(list(np.arange(3, dtype=kind)))) == 3
+    sq._ints(np.array([]))
+
+
 def test_a_rule_has_the_headers_layout():
     assert sq.LOGITS_RULE.itemsize == 32 and sq.LOGITS_RULE.isalignedstruct is False
     assert [sq.LOGITS_RULE.fields[n][1] for n in sq.LOGITS_RULE.names] == list(range(0, 32, 4))
