@@ -488,7 +488,7 @@ sllm_status sllm_page_batch_begin_tree(sllm_page_batch *batch, const int *seqs, 
  * Asynchronous on `stream`.
  * A captured call follows the batch's later steps when it is replayed (their begin
  * calls stay outside the graph), as long as they fit the buffer that it was captured with:
- * some twice the rows and page numbers of the step that last enlarged it (begin says
+ * some twice the rows and page numbers (and of trees the bits, one for each pair of rows) of the step that last enlarged it (begin says
  * SLLM_ERR_SHAPE where they don't; a new batch, captured again, takes them).
  * q, k, v and out must then hold max_rows rows, and every replay launches for max_rows:
  * captured decode steps want a batch of about their rows. The graph is replayed only while
@@ -557,7 +557,7 @@ typedef struct sllm_logits_params {
  * must not overlap it; NULL: not wanted) receives all logits, chosen_dev (rows ints; NULL: not wanted) the first token of
  * the largest value as argmaxF32 (float32_ops.go:812-822) but for NaN values, which are never chosen, and -1 where no value is above -inf.
  * batch (may be NULL): the rows are those of its step. Asynchronous on `stream`. Choosing
- * uses the stream's workspace (sllm_workspace_reserve; rows x (vocab / 512 + 64) bytes are enough); graphs captured on one
+ * uses the stream's workspace (sllm_workspace_reserve; rows x (vocab / 128 + 16) bytes are enough); graphs captured on one
  * stream share it and must not overlap. A captured call with a batch follows its later steps as
  * sllm_page_attention_dev: `rows` then has to be max_rows, as many as the buffers hold; a replay works on those of the step.
  */

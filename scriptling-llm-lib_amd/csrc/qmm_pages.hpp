@@ -70,7 +70,7 @@ struct StepRow {
     int direct;      // its one piece writes the output itself
     StepPart parts[kMaxParts];  // (pieces 0 behind the last)
     int end;         // rows of its sequence that precede it, itself included (its position + 1, but of a tree)
-    int tree;        // the rows of its tree that it sees (tree_half), -1 where these are all up to its own
+    int tree;        // the rows of its tree that it sees (tree_halves), -1 where these are all up to its own
     int parent;      // the query row before it (of a tree: its parent), -1 for none
 };
 // What a row of a tree sees: a bit for each of its sequence's rows, 16 to an element, from the element with the

@@ -387,7 +387,6 @@ struct Rows : Shape<T, NB, FULL, VM> {
     // scores to weights, for the tile at position tp (masked: some row does not see all of it)
     __device__ __forceinline__ void weights(const Piece &p, int tp, bool masked) {
         if (masked) {
-
             int lane = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
             asm volatile("" : "+v"(lane));
             const int qd = lane >> 4;
