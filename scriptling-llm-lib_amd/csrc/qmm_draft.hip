@@ -74,7 +74,7 @@ __device__ __forceinline__ int wave_min(int v) {
 // Each workgroup reads all of its row's tokens: 4000 tokens that are none of the vocabulary's cost 64 rows of 128256 1.9 us
 // beside the 14.1 of the logits alone. Bound by the bytes of the logits where there are many rows, by the chain of
 // loads (mask or rule, elements, tokens) where there are few.
-// 64 rows of 128256, histories of up to 4000, 20 biases (67 MB, 13 us at a copy's rate): 15.5 us with the choice. The counted
+// 64 rows of 128256, histories of up to 4000, 20 biases (67 MB, 13 us at a copy's rate): 15.2 us with the choice. The counted
 // elements worked off from a list, a thread for each: 20.2; two tables, one value after the other: 30.8.
 constexpr int kRuleThreads = 256;
 template <int V>
@@ -102,6 +102,13 @@ __global__ void __launch_bounds__(kRuleThreads) logits_rules_kernel(LogitsArgs a
     if (whole && !masked)
 #pragma unroll
         for (int k = 0; k < V; k++) v[k] = *(const v4f *)(x + c0 + 4 * (tid + k * T));
+    // (the mask's words are asked for before the rule is: both are waited for at once)
+    static_assert(CH / 32 + 2 <= T, "a word of the mask to a thread");
+    unsigned word = 0;
+    if (masked) {
+        const int words = (a.vocab + 31) / 32, w = (c0 ? c0 - 32 : 0) / 32 + tid;
+        if (tid < CH / 32 + 2 && w < words) word = ((const unsigned *)a.p.masks)[(size_t)mask * words + w];
+    }
     const int seq = a.batch ? a.step.of()[r] : r;
     sllm_logits_rule rule{1.0f, 0.0f, 0.0f, 0, 0, 0, 0, 0};
     if (seq < a.p.n_rules) rule = a.p.rules[seq];
@@ -125,15 +132,11 @@ __global__ void __launch_bounds__(kRuleThreads) logits_rules_kernel(LogitsArgs a
         first = INT_MAX;
         some = biased = 0;
     }
-    if (masked) {
-        const int words = (a.vocab + 31) / 32;
-        const unsigned *m = (const unsigned *)a.p.masks + (size_t)mask * words;
-        const int w = (c0 ? c0 - 32 : 0) / 32;
-        for (int i = tid; i < CH / 32 + 2; i += T) bits[i] = w + i < words ? m[w + i] : 0u;
-    }
+    if (masked && tid < CH / 32 + 2) bits[tid] = word;
     lds_barrier();
-    // which elements there are and are allowed, a bit for each of the thread's: what is not allowed need not be read, and
-    // can be written at once
+    // which elements there are and are allowed, a bit for each of the thread's: what is not allowed need not be read. (It is
+    // written with the rest: the tokens' loads wait for stores before them, and whole lines can go past the caches. -inf at
+    // once: trees with masks 14.9 us against 13.4, 64 rows of which 30 % are allowed 18.0 against 15.3)
     unsigned ok = ~0u;
     if (!whole || masked) {
         const int w0 = c0 ? c0 - 32 : 0;  // the element of bits' first bit (the first element may lie up to three before c0)
@@ -162,10 +165,6 @@ __global__ void __launch_bounds__(kRuleThreads) logits_rules_kernel(LogitsArgs a
 #pragma unroll
                 for (int u = 0; u < 4; u++) v[k][u] = x[min(max(c0 + 4 * (tid + k * T) + u, lead), end - 1)];
         }
-        if (dst && aligned)
-#pragma unroll
-            for (int k = 0; k < V; k++)
-                if (!(ok >> 4 * k & 15)) *(v4f *)(dst + c0 + 4 * (tid + k * T)) = none;
     }
     // tokens t0 .. t0 + nt - 1 are the chunk's, the first one's entry is i0
     const int t0 = max(c0 - lead, 0), nt = max(min(c0 - lead + CH, a.vocab) - t0, 0), i0 = t0 + lead - c0;
@@ -248,11 +247,9 @@ __global__ void __launch_bounds__(kRuleThreads) logits_rules_kernel(LogitsArgs a
         for (int k = 0; k < V; k++) {
             const int e = c0 + 4 * (tid + k * T);
             if (aligned) {
-                // whole lines go past the caches (19.2 -> 17.4 us), the rest of lines that were begun with -inf does not
-                // (trees with masks 16.4, past them 18.1)
+                // whole lines go past the caches (17.4 us without, 15.2; masked 14.8, 13.4)
                 const v4f z = {y[4 * k], y[4 * k + 1], y[4 * k + 2], y[4 * k + 3]};
-                if (!masked) __builtin_nontemporal_store(z, (v4f *)(dst + e));
-                else if (ok >> 4 * k & 15) *(v4f *)(dst + e) = z;
+                __builtin_nontemporal_store(z, (v4f *)(dst + e));
             } else {
 #pragma unroll
                 for (int u = 0; u < 4; u++)
