@@ -620,7 +620,7 @@ class PageBatch:
         int32 array is not copied)."""
         if len(seqs) != len(rows):
             raise SllmError(1, "seqs and rows differ in length")
-        if len(parents) != sum(rows):
+        if len(parents) != sum(int(n) for n in rows):  # (numbers of an array's type would wrap)
             raise SllmError(1, "parents must name a row for each of the step's")
         _check(lib().sllm_page_batch_begin_tree(self.handle, _ints(seqs), _ints(rows), len(seqs), _ints(parents),
                                                 C.c_void_p(stream)))
