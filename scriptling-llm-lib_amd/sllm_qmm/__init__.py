@@ -651,8 +651,10 @@ def logits_rules_dev(logits_ptr: int, rows: int, vocab: int, params: LogitsParam
                      batch: PageBatch | None = None, stream: int = 0) -> None:
     """Penalties for repeated tokens, biases and masks of rows of logits (dst; 0: not wanted), and the greedy token of
     each row (chosen; 0: not wanted). With a batch the rows are those of its step."""
+    if batch is not None and not batch.handle:
+        raise SllmError(1, "the batch is closed")
     _check(lib().sllm_logits_rules_dev(logits_ptr, rows, vocab, C.byref(params), dst_ptr, chosen_ptr,
-                                       batch.handle if batch else None, stream))
+                                       None if batch is None else batch.handle, stream))
 
 
 class LoraSet:

@@ -30,3 +30,8 @@ def test_rows_of_any_integers_are_added_up_whole(kind):
     for wrong in {n - 1, n + 1, max(wrapped, 0)} - {n}:
         assert "parents" in message(Closed().begin_tree, [0, 1, 2], rows, [-1] * wrong)
     assert "null pointer" in message(Closed().begin_tree, [0, 1, 2], rows, [-1] * n)
+
+
+def test_a_closed_batch_is_not_no_batch():
+    """logits_rules_dev without a batch is another call: rows are requests then."""
+    assert "closed" in message(sq.logits_rules_dev, 64, 1, 4, sq.LogitsParams(), 0, 64, Closed())
