@@ -495,9 +495,7 @@ LORA_TYPES = {"f32": 0, "f16": 1, "bf16": 2}
 
 
 def _ints(values):
-    if isinstance(values, np.ndarray):
-        if len(values) and (values.ndim != 1 or values.dtype.kind not in "iu"):
-            raise TypeError("a list of integers or an array of them, of one dimension")
+    if isinstance(values, np.ndarray) and values.ndim == 1 and values.dtype.kind in "iu":
         values = np.ascontiguousarray(values, np.int32)
         return values.ctypes.data_as(C.POINTER(C.c_int))  # (keeps the array)
     return (C.c_int * len(values))(*values)

@@ -35,3 +35,11 @@ def test_rows_of_any_integers_are_added_up_whole(kind):
 def test_a_closed_batch_is_not_no_batch():
     """logits_rules_dev without a batch is another call: rows are requests then."""
     assert "closed" in message(sq.logits_rules_dev, 64, 1, 4, sq.LogitsParams(), 0, 64, Closed())
+
+
+def test_arrays_that_hold_pythons_integers():
+    assert sq._ints(np.array([3, 4, 5], object))[:3] == [3, 4, 5]
+    assert len(sq._ints(np.array([], object))) == 0
+    for wrong in (np.array([3, 4.5], object), np.array([[1, 2]], object), np.array([3, "a"], object)):
+        with pytest.raises(TypeError):
+            sq._ints(wrong)
