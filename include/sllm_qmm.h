@@ -506,7 +506,7 @@ sllm_status sllm_page_attention_dev(sllm_page_batch *batch, int layer, const sll
  * first of the sequence's next step (0 and -1 for a sequence without rows). Also for steps of
  * sllm_page_batch_begin, whose rows each continue the one before. Integers of any value are allowed in tokens and chosen.
  * Asynchronous on `stream`; captured as sllm_page_attention_dev (tokens, chosen and kept then hold max_rows ints, counts
- * and next max_seqs).
+ * and next max_seqs). From 2^24 sequences on (captured: max_seqs) SLLM_ERR_SHAPE, of sllm_page_keep_dev too.
  */
 sllm_status sllm_page_accept_dev(sllm_page_batch *batch, const int *tokens_dev, const int *chosen_dev, int *kept_dev,
                                  int *counts_dev, int *next_dev, void *stream);

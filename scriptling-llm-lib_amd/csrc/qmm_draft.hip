@@ -306,6 +306,7 @@ __global__ void __launch_bounds__(64) logits_choose_kernel(LogitsArgs a) {
 // bits of the rows that follow, so nothing walks from row to row (64 rows of a chain: 64 reads of LDS one after the other).
 // Bound by latency: two dependent loads behind the step's description; 2.7 us, 200 sequences of up to 64 rows 4.6.
 constexpr int kAcceptThreads = 256;
+constexpr int kMostSeqs = 1 << 24;  // a launch has fewer than 2^32 threads: this kernel and the next have 256 to a sequence
 __global__ void __launch_bounds__(kAcceptThreads) page_accept_kernel(StepRef st, const int *tokens, const int *chosen, int *kept,
                                                                      int *counts, int *next) {
     __shared__ int child[kTreeRows];
@@ -525,8 +526,10 @@ sllm_status sllm_page_accept_dev(sllm_page_batch *batch, const int *tokens, cons
         if (st != SLLM_OK) return st;
         hipStream_t s = (hipStream_t)stream;
         const bool capture = stream_capturing(s);
-        if (b.seqs.empty() && !capture) return SLLM_OK;
-        hipLaunchKernelGGL(page_accept_kernel, dim3((unsigned)(capture ? b.max_seqs : (int)b.seqs.size())), dim3(kAcceptThreads), 0, s,
+        const int n = capture ? b.max_seqs : (int)b.seqs.size();
+        if (!n) return SLLM_OK;
+        if (n >= kMostSeqs) return set_error(SLLM_ERR_SHAPE, "accepted paths of 2^24 sequences or more");
+        hipLaunchKernelGGL(page_accept_kernel, dim3((unsigned)n), dim3(kAcceptThreads), 0, s,
                            step_ref(b, capture), tokens, chosen, kept, counts, next);
         SLLM_HIP(hipGetLastError());
         b.captured |= capture;
@@ -555,7 +558,9 @@ sllm_status sllm_page_keep_dev(sllm_page_batch *batch, const int *kept, void *st
         if (st != SLLM_OK) return st;
         hipStream_t s = (hipStream_t)stream;
         const bool capture = stream_capturing(s);
-        if (b.seqs.empty() && !capture) return SLLM_OK;
+        const int n = capture ? b.max_seqs : (int)b.seqs.size();
+        if (!n) return SLLM_OK;
+        if (n >= kMostSeqs) return set_error(SLLM_ERR_SHAPE, "kept rows of 2^24 sequences or more");
         KeepArgs a{};
         a.step = step_ref(b, capture);
         a.kept = kept;
@@ -566,8 +571,7 @@ sllm_status sllm_page_keep_dev(sllm_page_batch *batch, const int *kept, void *st
         a.page_rows = c.page_rows;
         a.pieces = c.d_k * c.elem() / 16;
         a.layer_bytes = (size_t)c.n_pages * c.n_kv * c.page_rows * c.d_k * c.elem();
-        hipLaunchKernelGGL(page_keep_kernel, dim3((unsigned)(capture ? b.max_seqs : (int)b.seqs.size()), 2u * (unsigned)c.n_layers),
-                           dim3(kKeepThreads), 0, s, a);
+        hipLaunchKernelGGL(page_keep_kernel, dim3((unsigned)n, 2u * (unsigned)c.n_layers), dim3(kKeepThreads), 0, s, a);
         SLLM_HIP(hipGetLastError());
         b.captured |= capture;
         return SLLM_OK;
