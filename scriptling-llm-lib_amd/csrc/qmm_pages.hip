@@ -234,25 +234,33 @@ constexpr int kLeastTiles = 4;     // of a piece: one for every wave
 
 constexpr int kSpareStates = 8192; // of a kv head, beyond what a step's rows need in one piece each
 
-// How long a piece takes (us), roughly: a tile's bytes or products at a workgroup's share of what the card reaches
-// when all workgroups run, and what a piece costs beside its tiles.
+// How long a piece takes (us), roughly: a tile's bytes or products at a workgroup's share of what the card gives when all
+// workgroups run, and what a piece costs beside its tiles (q into registers, the first tiles, the states: by the block's elements).
+// The constants are those under which the choices of `cut` come nearest to the best that it could make, as measured in 1124
+// steps: twelve head layouts (2 to 32 kv heads of 64 to 256), both types, rows alone, on shared prefixes, prompts; 1.5 % above
+// the best in the mean. Constants from 32 / 8 heads of 128 alone, 7.0 for every piece: 4.3 %, and where pieces are cheap they were too
+// few: 6 / 2 heads of 136, f32, one row behind 300 18.8 us against 14.4; 12 / 12 of 64, 64 rows on 4000 33.5, 29.3.
 struct PieceCost {
-    double tile[3];  // by shape
-    double piece = 7.0, merge = 2.5;  // (q into registers, the first tiles, the states: 13400 cycles with 128 rows, 9200 with 64)
-    double state;    // one row's state of all kv heads, written and read
+    double tile[3];                  // by shape
+    double merge = 4.5, state, row;  // state: one row's of all kv heads, written and read; row: its elements, of 8192
     PieceCost(const PageCache &c, const int *most) {
-        const double read = 6.0e6, f16 = 0.4e9, f32 = 0.13e9;  // bytes, operations in a us
+        const double read = 12.0e6, f16 = 0.54e9, f32 = 0.122e9;  // bytes, operations in a us
         for (int i = 0; i < 3; i++) {
             const double bytes = 2.0 * kPieceTile * c.d_k * c.elem(), ops = 4.0 * kPieceTile * c.d_k * most[i];
-            tile[i] = std::max(i ? 0.0 : bytes / read, ops / (c.elem() == 2 ? f16 : f32)) * kTargetPieces;
+            tile[i] = std::max(i ? 0.0 : bytes / read, ops / (c.elem() == 2 ? f16 : f32)) * kTargetPieces + 0.3;
         }
-        state = 8.0 * (c.d_k + 2) * c.n_kv / read;
+        state = 8.0 * (c.d_k + 2) * c.n_kv / 6.0e6;
+        row = c.d_k / 8192.0;
     }
-    // `x`: workgroups over those that run at a time. Fewer than CUs have more of the memory's rate each, but products do not end
-    // sooner for that (32 / 8 heads of 128, f16: a tile of 128 rows 1.5 us alone on a CU, 1.85 beside another; of 64 1.1, 1.15).
-    double time(int shape, int rows, double x) const {
-        static constexpr double least[3] = {0.27, 0.8, 0.6};
-        return tile[shape] * (x >= 0.5 ? 1.0 : std::max(rows <= 16 ? 0.5 * least[shape] : least[shape], x));
+    // Workgroups with a CU for themselves have more of the memory's rate each, but products do not end sooner for that (32 / 8
+    // heads of 128, f16: a tile of 128 rows 1.5 us alone on a CU, 1.85 beside another; of 64 1.1, 1.15).
+    double time(int shape, bool alone, double x) const {
+        static constexpr double least[3] = {0.505, 0.645, 0.585};
+        return tile[shape] * (alone ? std::max(least[shape], x) : 1.0);
+    }
+    double piece(int shape, int rows) const {
+        const double elements = (rows + 15) / 16 * 16 * row;
+        return shape ? 2.9 + 0.7 * elements : 3.4 + 1.6 * elements;
     }
 };
 
@@ -311,10 +319,11 @@ int cut(const PageCache &c, Plan *plan, int rep, int slots) {
         busy.assign((size_t)std::max(1, kTargetPieces / n_kv), 0.0);  // a heap, the first to be free on top
         double end = 0.0;
         for (const Segment &s : plan->segs) {
-            const double tile = cost.time(s.shape, std::min(s.block, s.ntok) * rep, x);
+            const double tile = cost.time(s.shape, items * n_kv <= kTargetPieces / 2, x);
+            const double piece = cost.piece(s.shape, std::min(s.block, s.ntok) * rep);
             for (int i = 0; i < s.pieces; i++) {
                 const int at = s.p0 + i * s.piece, n = (std::min(s.p1 - at, s.piece) + kPieceTile - 1) / kPieceTile;
-                const double t = cost.piece + n * tile;
+                const double t = piece + n * tile;
                 for (int k = 0; k < s.ntok; k += s.block) {
                     std::pop_heap(busy.begin(), busy.end(), std::greater<>());
                     end = std::max(end, busy.back() += t);
@@ -333,8 +342,11 @@ int cut(const PageCache &c, Plan *plan, int rep, int slots) {
         if (!shapes(k) && k < 2) continue;
         const int64_t share = std::max<int64_t>(kLeastTiles, (all * n_kv + kTargetPieces - 1) / kTargetPieces);
         if (!tiles) tiles = share;
+        int64_t last = 0;
         for (const int64_t eighths : {4, 5, 6, 7, 8, 9, 10, 11, 12, 14, 16, 20}) {
             const int64_t t = std::max<int64_t>(kLeastTiles, share * eighths / 8);
+            if (t == last) continue;
+            last = t;
             const int64_t n = pieces(t);
             if (used > slots || (k < 2 && n * n_kv > kTargetPieces / 2)) continue;
             const double e = estimate(n);
