@@ -1,6 +1,7 @@
 """How a step's rows and positions are cut into blocks and pieces (the host's part of a step's begin)."""
 import pytest
 
+import _blocks
 from _plans import CLANG, compile_program, plan
 
 
@@ -23,3 +24,17 @@ def program(tmp_path_factory):
 ])
 def test_positions_are_cut_finely_where_pieces_are_cheap(program, heads, kv, dk, prefix, owns, least):
     assert plan(program, heads, kv, dk, "f32", 32, prefix, owns, [1] * len(owns)).pieces >= least
+
+
+@pytest.mark.parametrize("step", _blocks.steps(), ids=lambda s: s.name)
+def test_steps_of_the_gpu_tests_plan_their_blocks(program, step):
+    """test_gpu_blocks.py reaches each kind of block by these steps."""
+    p = plan(program, step.heads, step.kv, step.dk, step.dtype, step.page, step.prefix, step.owns, step.rows,
+             _blocks.parents(step) if step.trees else None)
+    have = {(b.shape, b.tree, b.causal) for b in p.blocks}
+    assert step.wanted <= have, have
+    if len(step.rows) > 1:  # (that other choices are not looked at does not hang on the estimate)
+        rows = {(b.shape, b.tree, b.causal): 0 for b in p.blocks}
+        for b in p.blocks:
+            rows[b.shape, b.tree, b.causal] += b.many
+        assert sum(rows.values()) * step.kv > 256
