@@ -989,11 +989,12 @@ sllm_status launch(const PageAttnArgs &a, hipStream_t s) {
     SLLM_HIP(hipGetLastError());
     if (!a.combine) return SLLM_OK;
     const int pairs = a.grid_rows * a.n_heads;
-    // Groups of lanes to a pair: as many as have four pieces each, while the launch stays small (a captured one may meet any list).
-    // 8 rows of 32 heads, 60 pieces, us with one, two, four and eight: 54.4, 48.8, 46.5, 45.7 (attention in all); 64 rows, 13: 35.1,
-    // 34.3, 34.2, 35.0; 16 rows, 8: 32.1, 31.3, 31.7, 32.0; 700 rows, 3: 53.0, 53.7, 59.4, 65.7.
+    // Groups of lanes to a pair: as many as have two pieces each, while the launch stays small (a captured one may meet any list).
+    // us (attention in all) with one, two, four and eight: one row of 32 heads, 32 pieces 23.0, 19.9, 19.2, 18.8; 4 of 16, 9: 15.4,
+    // 14.7, 13.7, 13.7; 16 of 16, 8: 14.0, 13.2, 12.8, 12.8; 61 of 32, 32: 53.5, 52.1, 52.1, 52.8; 200 of 32, 4: 37.1, 36.1, 39.2,
+    // 41.4; 1055 of 32, 2: 86.5, 91.7, 96.3, 107.9. (Over 782 steps 0.4 % above the best in the mean; with four pieces each 1.2 %.)
     int g = groups;
-    while (a.combine != INT32_MAX && g > 1 && (4 * g > a.combine || (int64_t)pairs * g * LP > kMergeThreads)) g /= 2;
+    while (a.combine != INT32_MAX && g > 1 && (2 * g > a.combine || (int64_t)pairs * g * LP > kMergeThreads)) g /= 2;
     const dim3 grid((unsigned)((pairs + groups / g - 1) / (groups / g)));
     switch (g) {
     case 1: hipLaunchKernelGGL((page_combine_kernel<LP, 1>), grid, dim3(256), 0, s, a); break;

@@ -28,11 +28,13 @@ def test_positions_are_cut_finely_where_pieces_are_cheap(program, heads, kv, dk,
 
 @pytest.mark.parametrize("step", _blocks.steps(), ids=lambda s: s.name)
 def test_steps_of_the_gpu_tests_plan_their_blocks(program, step):
-    """test_gpu_blocks.py reaches each kind of block by these steps."""
+    """test_gpu_blocks.py reaches each kind of block, and each number of groups that merge states, by these steps."""
     p = plan(program, step.heads, step.kv, step.dk, step.dtype, step.page, step.prefix, step.owns, step.rows,
              _blocks.parents(step) if step.trees else None)
     have = {(b.shape, b.tree, b.causal) for b in p.blocks}
     assert step.wanted <= have, have
+    if step.groups is not None:
+        assert _blocks.merge_groups(p.pieces, sum(step.rows) * step.heads, step.dk) == step.groups, p.pieces
     if len(step.rows) > 1:  # (that other choices are not looked at does not hang on the estimate)
         rows = {(b.shape, b.tree, b.causal): 0 for b in p.blocks}
         for b in p.blocks:
