@@ -475,7 +475,6 @@ sllm_status sllm_logits_rules_dev(const float *logits, int rows, int vocab, cons
             a.batch = true;
             a.follow = capture;
             a.step = step_ref(b, capture);
-            b.captured |= capture;
         }
         if (!rows) return SLLM_OK;
         sllm_status st = library_init();
@@ -504,6 +503,7 @@ sllm_status sllm_logits_rules_dev(const float *logits, int rows, int vocab, cons
         if (four) hipLaunchKernelGGL(logits_rules_kernel<4>, grid, dim3(kRuleThreads), 0, s, a);
         else hipLaunchKernelGGL(logits_rules_kernel<1>, grid, dim3(kRuleThreads), 0, s, a);
         SLLM_HIP(hipGetLastError());
+        if (batch) const_cast<sllm_page_batch *>(batch)->b.captured |= a.follow;
         if (!chosen || a.chunks == 1) return SLLM_OK;
         hipLaunchKernelGGL(logits_choose_kernel, dim3((unsigned)rows), dim3(64), 0, s, a);
         SLLM_HIP(hipGetLastError());

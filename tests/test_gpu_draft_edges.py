@@ -41,3 +41,33 @@ def test_captured_calls_of_too_many_sequences():
         torch.cuda.synchronize()
         assert kept.tolist() == [0, 1] and counts.tolist() == [2, -7] and after.tolist() == [0, -7]
         cache.truncate(s, 0)
+
+
+def test_a_refused_capture_leaves_the_batch_free_to_grow():
+    """Rules whose candidates need more workspace than may be had record nothing: the batch's steps may grow afterwards."""
+    rows, v = 60000, 9001  # (three chunks of 8 bytes a row: 1.4 MB)
+    cache = sq.PageCache(1, 1, 8, 16, 60000)
+    batch = sq.PageBatch(cache, 1, 1, rows)
+    s = cache.add()
+    batch.begin_tree([s], [1], [-1])
+    x = torch.zeros(64, dtype=torch.int32, device="cuda")
+    p = x.data_ptr()
+    st = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    sq.set_param("workspace_max_mb", 1)
+    try:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            y = x * 2
+            try:
+                sq.logits_rules_dev(p, rows, v, sq.LogitsParams(), 0, p, batch, st.cuda_stream)
+                status = 0
+            except sq.SllmError as e:
+                status = e.status
+    finally:
+        sq.set_param("workspace_max_mb", 0)
+    torch.cuda.synchronize()
+    assert status == 5
+    del g, y
+    cache.extend(s, 16 * 59000)
+    batch.begin_tree([s], [1], [-1])
