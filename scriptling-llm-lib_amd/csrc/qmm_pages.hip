@@ -794,7 +794,7 @@ static sllm_status begin_step(sllm_page_batch *batch, const int *seqs, const int
         size_t dev_cap = b.dev_cap;
         if (dev_cap < bytes) {
             if (b.captured)
-                return set_error(SLLM_ERR_SHAPE, "the step has more pages than the batch held when it was captured");
+                return set_error(SLLM_ERR_SHAPE, "the rows, pages and trees of the step need more than the batch held when it was captured");
             b.retired.reserve(b.retired.size() + 1);
             void *p = nullptr;
             dev_cap = 2 * bytes + 65536;
