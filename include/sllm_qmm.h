@@ -398,7 +398,8 @@ typedef enum {
  * copies) is enqueued on the given stream. Work on one cache, its attention
  * calls included, has to be ordered on the device: one stream, or streams
  * ordered by the caller's events. Calls may come from several threads. None may
- * be made on a stream under capture, except sllm_page_attention_dev and those
+ * be made on a stream under capture, except those on a batch's step that has begun
+ * (sllm_page_attention_dev, sllm_page_accept_dev, sllm_page_keep_dev, sllm_logits_rules_dev) and those
  * without a stream argument. Calls need the cache's device as the current one
  * (else SLLM_ERR_ARG). A cache that is destroyed lives on until its last batch is.
  */
@@ -477,9 +478,9 @@ sllm_status sllm_page_batch_begin_tree(sllm_page_batch *batch, const int *seqs, 
  * n_heads*d_k), k and v (rows x n_kv_heads*d_k) hold the sequences' new rows
  * one sequence after the other, in the order of begin. Adds the biases,
  * RMSNorms with QNormW / KNormW, rotates (a row's position is its number in its
- * sequence), writes the k and v rows into their pages in the cache's type, and
- * then every row's causal attention over its sequence's rows (as the pages
- * hold them) to out (rows x n_heads*d_k). q, k, v and out must be 16-byte
+ * sequence, of a tree one more than its parent's), writes the k and v rows into their pages in the cache's type, and
+ * then every row's attention over its sequence's rows up to itself (as the pages
+ * hold them; of a tree over those that sllm_page_batch_begin_tree says it sees) to out (rows x n_heads*d_k). q, k, v and out must be 16-byte
  * aligned; q, k and v are not modified, rows of the pools beyond those appended
  * neither. Sums and softmax statistics are fp32, the weights the hardware's 32-bit
  * exponentials (sllm_attention_dev forms them in 64 bits). Over f16 pages q and the
@@ -518,7 +519,8 @@ sllm_status sllm_page_accept_dev(sllm_page_batch *batch, const int *tokens_dev, 
  * path has the position of its place. The host's lengths stay: sllm_page_seq_truncate takes the rows behind the path (and
  * ends the step). Other rows of the pools are not modified; the places behind the path keep their
  * contents. A page with rows of the step that another sequence holds too (a fork
- * since the step's begin) is refused (SLLM_ERR_ARG). Asynchronous on `stream`; captured as sllm_page_attention_dev.
+ * since the step's begin) is refused (SLLM_ERR_ARG). Asynchronous on `stream`; captured as sllm_page_attention_dev. A replay
+ * refuses nothing: where the call would be, it would move rows in the other sequence's page, so sequences are forked behind it.
  */
 sllm_status sllm_page_keep_dev(sllm_page_batch *batch, const int *kept_dev, void *stream);
 
