@@ -36,7 +36,7 @@ struct LogitsArgs {
     const float *x;
     float *dst;
     int *chosen;
-    int rows, vocab, chunks;
+    int vocab, chunks;
     sllm_logits_params p;
     bool batch, follow;  // follow: the step's rows are fewer than the launch has, maybe
     StepRef step;
@@ -381,7 +381,7 @@ struct KeepArgs {
     StepRef step;
     const int *kept;
     char *pool_k, *pool_v;
-    int n_pages, n_kv, page_rows, pieces;  // pieces: 16-byte pieces of a row of a head
+    int n_kv, page_rows, pieces;  // pieces: 16-byte pieces of a row of a head
     size_t layer_bytes;
 };
 
@@ -482,7 +482,6 @@ sllm_status sllm_logits_rules_dev(const float *logits, int rows, int vocab, cons
         a.x = logits;
         a.dst = dst;
         a.chosen = chosen;
-        a.rows = rows;
         a.vocab = vocab;
         a.p = *p;
         if (!p->n_masks) a.p.masks = nullptr;
@@ -566,7 +565,6 @@ sllm_status sllm_page_keep_dev(sllm_page_batch *batch, const int *kept, void *st
         a.kept = kept;
         a.pool_k = c.k;
         a.pool_v = c.v;
-        a.n_pages = c.n_pages;
         a.n_kv = c.n_kv;
         a.page_rows = c.page_rows;
         a.pieces = c.d_k * c.elem() / 16;

@@ -1002,7 +1002,6 @@ sllm_status sllm_page_attention_dev(sllm_page_batch *batch, int layer, const sll
     a.d_k = c.d_k;
     a.rep = b.n_heads / c.n_kv;
     a.shift = c.shift;
-    a.n_pages = c.n_pages;
     a.q_bias = p->q_bias_len ? p->q_bias : nullptr;
     a.k_bias = p->k_bias_len ? p->k_bias : nullptr;
     a.v_bias = p->v_bias_len ? p->v_bias : nullptr;

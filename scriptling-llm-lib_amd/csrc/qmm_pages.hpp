@@ -129,7 +129,7 @@ struct PageBatch {
 struct PageAttnArgs {
     const float *q, *k, *v;
     float *out;
-    int n_heads, n_kv, d_k, rep, shift, n_pages;
+    int n_heads, n_kv, d_k, rep, shift;
     const float *q_bias, *k_bias, *v_bias;
     int qb_len, kb_len, vb_len;
     const float *q_norm, *k_norm;
