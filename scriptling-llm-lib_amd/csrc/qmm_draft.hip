@@ -71,11 +71,12 @@ __device__ __forceinline__ int wave_min(int v) {
 // One workgroup per (row, chunk of the vocabulary), 4 V elements to a thread, which it holds in registers from the first
 // load to the store. The row's biases that lie in the chunk go into a table in LDS, an entry for each element (of a token
 // named twice the later: the largest number), then, cleared, the counts of the row's tokens (its history, its node's path).
-// Each workgroup reads all of its row's tokens: 4000 tokens that are none of the vocabulary's cost 64 rows of 128256 1.9 us
-// beside the 14.1 of the logits alone. Bound by the bytes of the logits where there are many rows, by the chain of
-// loads (mask or rule, elements, tokens) where there are few.
-// 64 rows of 128256, histories of up to 4000, 20 biases (67 MB, 13 us at a copy's rate): 15.2 us with the choice. The counted
-// elements worked off from a list, a thread for each: 20.2; two tables, one value after the other: 30.8.
+// Bound by the bytes of the logits where there are many rows, by the chain of loads (mask or rule, elements, tokens) where there are
+// few; and by the tokens where histories are long, since each workgroup reads all of its row's: 64 rows of 128256 with
+// no tokens, 4000 and 16000 to a row take 14.1, 17.4 and 23.1 us, without the values kept 9.8, 16.4 and 22.3 (4000 that are
+// none of the vocabulary's: 16.5 and 13.1).
+// 64 rows of 128256, histories of up to 4000, 2000 in the mean, 20 biases (67 MB, 13 us at a copy's rate): 15.2 us with the choice. The
+// counted elements worked off from a list, a thread for each: 20.2; two tables, one value after the other: 30.8.
 constexpr int kRuleThreads = 256;
 template <int V>
 __global__ void __launch_bounds__(kRuleThreads) logits_rules_kernel(LogitsArgs a) {
@@ -486,8 +487,10 @@ sllm_status sllm_logits_rules_dev(const float *logits, int rows, int vocab, cons
         a.p = *p;
         if (!p->n_masks) a.p.masks = nullptr;
         // Chunks of 1024 while all of them run at once (eight workgroups to a CU), else of 4096, whose launch and tokens cost
-        // less: 1 x 49152 7.5 us against 8.9, 7 x 32003 8.1 against 12.6, 16 x 128256 10.1 against 10.4; 32 x 128256 14.3
-        // against 12.4, 64 x 128256 25.4 against 19.2 (as the kernels were then, both sides alike).
+        // less. us with chunks of 1024 and of 4096, values kept, histories of 64: 1 x 49152 6.8, 8.5; 7 x 32003 6.0, 8.2; 8 x 128256 6.8, 7.2;
+        // 16 x 128256 8.2, 7.7; 24 x 128256 9.7, 8.4; 64 x 128256 16.9, 14.3 (4000: 25.4, 16.5). Chunks that are not whole read and
+        // write one element at a time, which costs more of the larger ones: short vocabularies, and those whose rows do
+        // not all begin at 16 bytes, stay faster with 1024 beyond that (80 x 32003 9.5, 11.8; 1000 x 4097, no tokens, 12.5, 21.3).
         const int64_t small = 4 * kRuleThreads, n_small = ((int64_t)vocab + 3 + small - 1) / small;
         const bool four = n_small * rows > 2048;
         a.chunks = (int)(four ? (n_small + 3) / 4 : n_small);

@@ -267,11 +267,11 @@ struct PieceCost {
 // The segments' blocks and pieces: of a few lengths around a share of all the step's tiles the one whose pieces, taken by
 // workgroups one after the other, are estimated to end first; and no more states than the batch has room for. Where CUs are left
 // without a workgroup also of smaller blocks than the rows fill, which read K and V more often. Returns
-// the number of pieces (for one kv head). (32 / 8 heads of 128; the longest share that all workgroups take at once, and
-// so chosen, us: f32, 64 sequences on a prefix of 4000 85.7, 66.6; 16 on 8000 48.8, 44.9; 5 prompts of 211 rows 161,
-// 147; f16, the 64 39.3, 35.2; others within 1. The largest block, and so chosen: a tree of 61 rows behind 1000, f16 24.3, 20.4;
-// f32 37.2, 28.1; of 16 behind 300, f32 22.2, 19.2. A step's begin with all of this takes the host 12 us for 16 sequences, 30 for
-// 64 on a prefix of 4000 in pages of 64, 90 on one of 16000 in pages of 16, 105 for 256 on 4000.)
+// the number of pieces (for one kv head). (32 / 8 heads of 128; pieces of an even share of the tiles, and so chosen, us: f32,
+// 64 sequences on a prefix of 4000 77.7, 73.6; 5 prompts of 211 rows on 1000 249, 237; f16, the 64 35.4, 33.8; f32, 16 on 8000 the
+// same pieces. The largest block, and so chosen: 61 rows behind 1000, f16 24.2, 19.1; f32 36.8, 25.6; 16 behind 300, f32 21.8, 15.3. A
+// step's begin with all of this takes the host 12 us for 16 sequences, 29 for 64 on a prefix of 4000 in pages of 64, 89 on
+// one of 16000 in pages of 16, 107 for 256 on 4000.)
 int cut(const PageCache &c, Plan *plan, int rep, int slots) {
     const int *most = kShapeRows[shape_class(c.d_k, c.type == SLLM_CACHE_F16)], n_kv = c.n_kv;
     const PieceCost cost(c, most);
