@@ -558,7 +558,7 @@ typedef struct sllm_logits_params {
  * become -inf. Each operation rounds once to float32, in this order. dst_dev (rows x vocab; may be logits_dev, else
  * must not overlap it; NULL: not wanted) receives all logits, chosen_dev (rows ints; NULL: not wanted) the first token of
  * the largest value as argmaxF32 (float32_ops.go:812-822) but for NaN values, which are never chosen, and -1 where no value is above -inf.
- * batch (may be NULL): the rows are those of its step. Asynchronous on `stream`. Choosing
+ * batch (may be NULL): the rows are those of its step. At most 65535 rows and 2^28 tokens (SLLM_ERR_SHAPE). Asynchronous on `stream`. Choosing
  * uses the stream's workspace (sllm_workspace_reserve; rows x (vocab / 128 + 16) bytes are enough); graphs captured on one
  * stream share it and must not overlap. A captured call with a batch follows its later steps as
  * sllm_page_attention_dev: `rows` then has to be max_rows, as many as the buffers hold; a replay works on those of the step.
